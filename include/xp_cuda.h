@@ -461,6 +461,102 @@ xp_status xp_bdec_generate(xp_bdec* b, uint32_t n, float* ms);
 xp_status xp_bdec_logits(xp_bdec* b, float* out, size_t n);
 xp_status xp_bdec_position(xp_bdec* b, uint32_t* pos);
 void xp_bdec_destroy(xp_bdec* b);
+/* ---- serving many sequences over one paged cache -----------------------------
+ * Operators for sequences of different lengths that share a cache made of
+ * pages: rotary positions, the quantising cache write and its read, attention
+ * over whole prompts, and attention of new tokens (one or many) over the pages.
+ * No counterpart in the reference, which serves one sequence from one flat
+ * cache. Every launch goes to `stream` and is ordered like any kernel there;
+ * nothing is allocated. The values of starts, tables, slots and lengths are
+ * device memory and are checked by the kernels, which touch nothing outside
+ * the buffers whatever they hold. */
+typedef enum xp_dtype { XP_F32 = 0, XP_F16 = 1, XP_BF16 = 2, XP_INT8 = 3, XP_FP8_E4M3 = 4 } xp_dtype;
+/* Rows of heads: value d of head h of token t is element
+ * t * token_stride + h * head_stride + d of `data` (strides in elements, so a
+ * slice of a fused q|k|v product needs no copy). F32, F16 or BF16. */
+typedef struct xp_rows {
+    void* data;
+    int64_t token_stride, head_stride;
+    uint32_t tokens, heads, dim;
+    uint32_t dtype;            /* xp_dtype */
+} xp_rows;
+/* A paged cache: k and v are [num_pages][kv_heads][page_size][head_dim]
+ * contiguous; 8-bit pages have one fp32 scale a row, [num_pages][kv_heads]
+ * [page_size], and the value of a code is code * scale. page_size is a power
+ * of two from 8 to 256; head_dim 64, 128 or 256. A row's slot number is
+ * page * page_size + row. */
+typedef struct xp_pages {
+    void *k, *v;
+    float *k_scale, *v_scale;  /* NULL for F16 and BF16 pages */
+    uint64_t num_pages;
+    uint32_t page_size, kv_heads, head_dim;
+    uint32_t dtype;            /* XP_F16, XP_BF16, XP_INT8 or XP_FP8_E4M3 */
+} xp_pages;
+/* Rotary positions: pair i of a head turns by positions[t] * turns[i] / 2^64
+ * of a circle. half: pairs (i, i + rot_dim / 2); interleaved: (2i, 2i + 1). */
+typedef enum xp_rope_layout { XP_ROPE_HALF = 0, XP_ROPE_INTERLEAVED = 1 } xp_rope_layout;
+typedef enum xp_rope_stretch {
+    XP_ROPE_PLAIN = 0,   /* f_i = theta^(-2i / rot_dim) radians a position */
+    XP_ROPE_LINEAR = 1,  /* f_i / factor */
+    XP_ROPE_BASE = 2,    /* theta * factor^(rot_dim / (rot_dim - 2)) in place of theta */
+    XP_ROPE_PARTS = 3    /* f_i (g + (1 - g) / factor): with r = original f_i / 2 pi turns over the original
+                          * context, g = clamp((r - slow) / (fast - slow), 0, 1); magnitude 0.1 ln factor + 1 */
+} xp_rope_stretch;
+typedef struct xp_rotary {
+    const uint64_t* turns;     /* device, [rot_dim / 2] */
+    const int32_t* positions;  /* device, one a token */
+    uint32_t rot_dim;          /* even, <= dim: the first rot_dim values of each head turn */
+    uint32_t layout;           /* xp_rope_layout */
+    float magnitude;           /* factor on the rotated values (1 unless stretched by parts) */
+    uint32_t inverse;          /* 1: turn back (the gradient of the forward rotation) */
+} xp_rotary;
+/* The table of a rotary embedding, on the host (turns[rot_dim / 2]); a 64-bit
+ * fraction of a turn makes the reduction of any position exact. *magnitude
+ * (may be NULL) is the factor that goes with it. */
+xp_status xp_rope_turns(uint64_t* turns, float* magnitude, uint32_t rot_dim, double theta, uint32_t stretch,
+                        double factor, double original, double slow, double fast);
+/* out = in with every head rotated; values past rot_dim are copied. out may be
+ * in (same data and strides); otherwise they must not overlap. */
+xp_status xp_rope_rows(void* stream, const xp_rows* out, const xp_rows* in, const xp_rotary* rope);
+/* Token t's k and v rows into slot slots[t] (device; a slot outside the cache
+ * is skipped, so -1 marks padding; no slot twice), k rotated first when `rope`
+ * is not NULL. 8-bit pages: top = max |x| of the row (at least 2^-100), code =
+ * x * (Q / top) rounded to nearest even, scale = top / Q, Q = 127 or 448; a
+ * row with an infinity or NaN gets a NaN scale and reads back as NaN. */
+xp_status xp_kv_write(void* stream, const xp_pages* pages, const xp_rows* k, const xp_rows* v, const int64_t* slots,
+                      const xp_rotary* rope);
+/* The rows in slots[0 .. tokens - 1] as values; a slot outside the cache gives
+ * zeros. */
+xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, const xp_rows* v, const int64_t* slots);
+/* Scratch of the two attentions: 16-byte aligned, zeroed once, one call at a
+ * time. Its uint32 at byte 4 is a sticky error word: 1 = a length past its
+ * table row (clamped), 2 = a page outside the cache (its rows read as zeros),
+ * 4 = a wait ran out, 8 = a sequence had more than q_most new tokens (the
+ * rest were left out). */
+#define XP_SERVING_SCRATCH_BYTES (48u << 20)
+/* Causal attention over whole prompts packed one after the other: sequence b
+ * is tokens starts[b] .. starts[b + 1] - 1 (device, [batch + 1]), and a token
+ * attends to those of its own sequence up to itself, the last `window` of them
+ * when window is not 0. Head h uses k and v head h / (heads / kv_heads).
+ * scale 0 = 1 / sqrt(dim). q, k, v and out of one type, F16 or BF16; dim 64,
+ * 128 or 256. Data and strides of 16 bytes. lse (may be NULL): [tokens][heads]
+ * natural log of the sum of the exponentiated scores, -inf for a token in no
+ * sequence, whose output is zero. What other sequences and later tokens hold,
+ * NaN included, does not matter. */
+xp_status xp_attention_packed(void* stream, const xp_rows* out, const xp_rows* q, const xp_rows* k, const xp_rows* v,
+                              const int32_t* starts, uint32_t batch, uint32_t window, float scale, float* lse,
+                              void* scratch);
+/* Attention of each sequence's newest tokens over its pages: sequence b's new
+ * tokens are q rows starts[b] .. starts[b + 1] - 1, its kv_lens[b] keys (those
+ * tokens' own included, already written) are in pages table[b * table_width
+ * ..], and new token i of n sits at position kv_lens[b] - n + i. A token whose
+ * position is negative sees nothing and gets zeros (lse -inf). q_most: the
+ * most new tokens of any sequence. 16-bit pages have q's type. The rest is as
+ * for xp_attention_packed. */
+xp_status xp_attention_paged(void* stream, const xp_rows* out, const xp_rows* q, const xp_pages* pages,
+                             const int32_t* table, uint32_t table_width, const int32_t* kv_lens,
+                             const int32_t* starts, uint32_t batch, uint32_t q_most, uint32_t window, float scale,
+                             float* lse, void* scratch);
 /* CUDA events on the session stream: stop = 0 records the start, 1 the end
  * and returns the elapsed device ms (brackets host-driven decode_step loops). */
 xp_status xp_session_timer(xp_session* s, int stop, float* ms);

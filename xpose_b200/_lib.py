@@ -54,6 +54,21 @@ class LayerWeights(C.Structure):
                                           "k_norm")]
 
 
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)] + \
+               [(n, C.c_uint32) for n in ("tokens", "heads", "dim", "dtype")]
+
+
+class Pages(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("num_pages", C.c_uint64)] + \
+               [(n, C.c_uint32) for n in ("page_size", "kv_heads", "head_dim", "dtype")]
+
+
+class Rotary(C.Structure):
+    _fields_ = [("turns", C.c_void_p), ("positions", C.c_void_p), ("rot_dim", C.c_uint32), ("layout", C.c_uint32),
+                ("magnitude", C.c_float), ("inverse", C.c_uint32)]
+
+
 _lib = None
 
 _SIGS = {
@@ -169,6 +184,14 @@ _SIGS = {
     "xp_session_profile_matvec": (C.c_int, [C.c_void_p, C.c_uint32, C.POINTER(C.c_float), C.POINTER(C.c_uint64),
                                             C.POINTER(C.c_uint32)]),
     "xp_session_timer": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(C.c_float)]),
+    "xp_rope_turns": (C.c_int, [C.c_void_p, C.POINTER(C.c_float), C.c_uint32, C.c_double, C.c_uint32] +
+                      [C.c_double] * 4),
+    "xp_rope_rows": (C.c_int, [C.c_void_p] * 4),
+    "xp_kv_write": (C.c_int, [C.c_void_p] * 6),
+    "xp_kv_read": (C.c_int, [C.c_void_p] * 5),
+    "xp_attention_packed": (C.c_int, [C.c_void_p] * 6 + [C.c_uint32, C.c_uint32, C.c_float, C.c_void_p, C.c_void_p]),
+    "xp_attention_paged": (C.c_int, [C.c_void_p] * 5 + [C.c_uint32] + [C.c_void_p] * 2 + [C.c_uint32] * 3 +
+                           [C.c_float, C.c_void_p, C.c_void_p]),
     "xp_session_trace": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32]),
 }
 

@@ -5,17 +5,20 @@
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libxp_cuda.so")
-SRC = os.path.join(HERE, "csrc", "xp_cuda.cu")
+OBJ = os.path.join(HERE, "build")
+# one translation unit each, compiled side by side and linked into the library
+UNITS = [os.path.join(HERE, "csrc", f) for f in ("xp_cuda.cu", "serving.cu")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc" if os.path.exists("/usr/local/cuda/bin/nvcc") else "nvcc")
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-diag-suppress", "1886,842",
 ]
 
@@ -29,16 +32,35 @@ def _stale(out, srcs):
     if not os.path.exists(out):
         return True
     t = os.path.getmtime(out)
-    return any(os.path.getmtime(s) > t for s in srcs)
+    return any(not os.path.exists(s) or os.path.getmtime(s) > t for s in srcs)
+
+
+def _includes(obj, unit):
+    """The files an object was made from, by the dependency file beside it."""
+    dep = obj + ".d"
+    if not os.path.exists(dep):
+        return _sources()
+    words = open(dep).read().replace("\\\n", " ").split(":", 1)[1].split()
+    return [unit] + [w for w in words if os.path.realpath(w).startswith(ROOT + os.sep)]
 
 
 def build_cuda(force=False, verbose=False):
     if not force and not _stale(LIB, _sources()):
         return LIB
-    cmd = [NVCC, *NVCC_FLAGS, "-o", LIB, SRC]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    os.makedirs(OBJ, exist_ok=True)
+
+    def compile_unit(unit):
+        obj = os.path.join(OBJ, os.path.basename(unit) + ".o")
+        if force or _stale(obj, _includes(obj, unit)):
+            cmd = [NVCC, *NVCC_FLAGS, "-MD", "-MF", obj + ".d", "-c", "-o", obj, unit]
+            if verbose:
+                print(" ".join(cmd))
+            subprocess.run(cmd, check=True)
+        return obj
+
+    with ThreadPoolExecutor(len(UNITS)) as pool:
+        objs = list(pool.map(compile_unit, UNITS))
+    subprocess.run([NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", LIB, *objs], check=True)
     return LIB
 
 

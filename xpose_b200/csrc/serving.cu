@@ -1,0 +1,317 @@
+// Serving entry points of libxp_cuda.so: rotary rows, the paged cache and its
+// attentions. A translation unit of its own, built beside xp_cuda.cu.
+#include <cmath>
+
+#include "host.cuh"
+#include "serving_attn.cuh"
+
+using namespace xp;
+
+namespace {
+
+#define REQUIRE(cond, ...)                                      \
+    do {                                                        \
+        if (!(cond)) return fail(XP_ERR_INVALID, __VA_ARGS__);  \
+    } while (0)
+
+xp_status launched(const char* who) {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return XP_OK;
+    return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+}
+
+size_t bytes_of(uint32_t dtype) { return dtype == XP_F32 ? 4 : dtype == XP_F16 || dtype == XP_BF16 ? 2 : 1; }
+
+// `align`: the elements every row has to be aligned to (a power of two)
+xp_status check_rows(const char* who, const char* name, const xp_rows* r, uint32_t align) {
+    REQUIRE(r, "%s: argument '%s' is null", who, name);
+    REQUIRE(r->data || r->tokens == 0, "%s: '%s' has no data", who, name);
+    REQUIRE(r->dtype <= XP_BF16, "%s: '%s' must be F32, F16 or BF16", who, name);
+    REQUIRE(r->heads && r->dim, "%s: '%s' has no heads or no values in a head", who, name);
+    REQUIRE(r->token_stride % align == 0 && r->head_stride % align == 0 &&
+                (uintptr_t)r->data % (align * bytes_of(r->dtype)) == 0,
+            "%s: the rows of '%s' must be aligned to %zu bytes", who, name, align * bytes_of(r->dtype));
+    return XP_OK;
+}
+bool same_shape(const xp_rows* a, const xp_rows* b) {
+    return a->tokens == b->tokens && a->heads == b->heads && a->dim == b->dim && a->dtype == b->dtype;
+}
+xp_status check_pages(const char* who, const xp_pages* p) {
+    REQUIRE(p, "%s: argument 'pages' is null", who);
+    REQUIRE(p->k && p->v, "%s: the pages have no data", who);
+    REQUIRE(p->dtype >= XP_F16 && p->dtype <= XP_FP8_E4M3, "%s: pages must be F16, BF16, INT8 or FP8_E4M3", who);
+    REQUIRE(p->page_size >= 8 && p->page_size <= 256 && !(p->page_size & (p->page_size - 1)),
+            "%s: page_size must be a power of two from 8 to 256 (got %u)", who, p->page_size);
+    REQUIRE(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256,
+            "%s: head_dim must be 64, 128 or 256 (got %u)", who, p->head_dim);
+    REQUIRE(p->kv_heads && p->num_pages && p->num_pages < (1ull << 31), "%s: the pages are empty or too many", who);
+    REQUIRE(bytes_of(p->dtype) > 1 || (p->k_scale && p->v_scale), "%s: 8-bit pages need scales", who);
+    REQUIRE((((uintptr_t)p->k | (uintptr_t)p->v) & 15) == 0 && (((uintptr_t)p->k_scale | (uintptr_t)p->v_scale) & 3) == 0,
+            "%s: pages must be 16-byte aligned", who);
+    return XP_OK;
+}
+xp_status check_rope(const char* who, const xp_rotary* r, uint32_t dim, uint32_t multiple) {
+    REQUIRE(r->rot_dim && r->rot_dim <= dim && r->rot_dim % multiple == 0,
+            "%s: rot_dim must be a multiple of %u up to %u (got %u)", who, multiple, dim, r->rot_dim);
+    REQUIRE(r->layout <= XP_ROPE_INTERLEAVED, "%s: unknown rotary layout %u", who, r->layout);
+    return XP_OK;
+}
+xp_status check_rope_data(const char* who, const xp_rotary* r) {
+    REQUIRE(r->turns && r->positions, "%s: a rotation needs turns and positions", who);
+    return XP_OK;
+}
+#define TRY(expr) \
+    if (xp_status s_ = (expr); s_ != XP_OK) return s_
+
+RowsArg rows_arg(const xp_rows* r) { return RowsArg{r->data, r->token_stride, r->head_stride}; }
+RopeArg rope_arg(const xp_rotary* r) {
+    if (!r) return RopeArg{};
+    return RopeArg{reinterpret_cast<const unsigned long long*>(r->turns), r->positions, r->rot_dim,
+                   r->layout == XP_ROPE_INTERLEAVED, r->magnitude, r->inverse ? -1.0f : 1.0f};
+}
+PagesArg pages_arg(const xp_pages* p) {
+    return PagesArg{p->k, p->v, p->k_scale, p->v_scale, p->num_pages * p->page_size,
+                    (uint32_t)__builtin_ctz(p->page_size), p->kv_heads};
+}
+
+// Calls f with a value of the type (and the W = dim / 64) that was asked for.
+template <class F> xp_status for_type(uint32_t dtype, F f) {
+    switch (dtype) {
+        case XP_F32: return f(float{});
+        case XP_F16: return f(__half{});
+        default: return f(bf16{});
+    }
+}
+template <class F> xp_status for_cache(uint32_t dtype, F f) {
+    switch (dtype) {
+        case XP_F16: return f(__half{});
+        case XP_BF16: return f(bf16{});
+        case XP_INT8: return f(int8c{});
+        default: return f(fp8c{});
+    }
+}
+template <class F> xp_status for_dim(uint32_t dim, F f) {
+    switch (dim) {
+        case 64: return f(std::integral_constant<int, 1>{});
+        case 128: return f(std::integral_constant<int, 2>{});
+        default: return f(std::integral_constant<int, 4>{});
+    }
+}
+
+xp_status grid_of(const char* who, uint64_t blocks, unsigned* grid) {
+    REQUIRE(blocks <= 0x7FFFFFFFull, "%s: too many rows for one launch", who);
+    *grid = (unsigned)blocks;
+    return XP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+xp_status xp_rope_turns(uint64_t* turns, float* magnitude, uint32_t rot_dim, double theta, uint32_t stretch,
+                        double factor, double original, double slow, double fast) {
+    const char* who = "rope_turns";
+    REQUIRE(turns, "%s: argument 'turns' is null", who);
+    REQUIRE(rot_dim >= 2 && rot_dim % 2 == 0, "%s: rot_dim must be even (got %u)", who, rot_dim);
+    REQUIRE(theta > 1.0 && std::isfinite(theta), "%s: theta must be above 1", who);
+    REQUIRE(stretch <= XP_ROPE_PARTS, "%s: unknown stretch %u", who, stretch);
+    REQUIRE(stretch == XP_ROPE_PLAIN || (factor >= 1.0 && std::isfinite(factor)), "%s: factor must be at least 1", who);
+    REQUIRE(stretch != XP_ROPE_BASE || rot_dim > 2, "%s: a stretched base needs rot_dim above 2", who);
+    REQUIRE(stretch != XP_ROPE_PARTS || (original > 0 && fast > slow), "%s: parts need original > 0 and fast > slow", who);
+    const double two_pi = 6.283185307179586476925286766559;
+    if (stretch == XP_ROPE_BASE) theta *= std::pow(factor, (double)rot_dim / (rot_dim - 2));
+    for (uint32_t i = 0; i < rot_dim / 2; ++i) {
+        double f = std::pow(theta, -2.0 * i / rot_dim);
+        if (stretch == XP_ROPE_LINEAR) f /= factor;
+        if (stretch == XP_ROPE_PARTS) {
+            const double g = std::fmin(1.0, std::fmax(0.0, (original * f / two_pi - slow) / (fast - slow)));
+            f *= g + (1.0 - g) / factor;
+        }
+        turns[i] = (uint64_t)std::ldexp(f / two_pi, 64);  // f <= 1: below 2^62
+    }
+    if (magnitude) *magnitude = stretch == XP_ROPE_PARTS ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return XP_OK;
+}
+
+xp_status xp_rope_rows(void* stream, const xp_rows* out, const xp_rows* in, const xp_rotary* rope) {
+    const char* who = "rope_rows";
+    TRY(check_rows(who, "out", out, 1));
+    TRY(check_rows(who, "in", in, 1));
+    REQUIRE(rope, "%s: argument 'rope' is null", who);
+    REQUIRE(same_shape(out, in), "%s: 'out' and 'in' differ in shape or type", who);
+    TRY(check_rope(who, rope, in->dim, 2));
+    if (in->tokens == 0) return XP_OK;
+    TRY(check_rope_data(who, rope));
+    // vectors of 16 bytes where every row allows them, else one pair a thread
+    const uint32_t vec = (uint32_t)(16 / bytes_of(in->dtype));
+    bool wide = rope->rot_dim % (2 * vec) == 0 && in->dim % vec == 0;
+    for (const xp_rows* r : {out, in})
+        wide = wide && r->token_stride % vec == 0 && r->head_stride % vec == 0 && (uintptr_t)r->data % 16 == 0;
+    const uint32_t vp = wide ? vec : 1;
+    const uint32_t units = rope->rot_dim / 2 / vp + (in->dim - rope->rot_dim + 2 * vp - 1) / (2 * vp);
+    // Heads a thread: enough to share the angles, as long as the GPU stays full.
+    uint32_t hpt = 1;
+    while (hpt < 8 && hpt < in->heads && (uint64_t)in->tokens * units * in->heads / (2 * hpt) >= (uint64_t)sm_count() * 2048)
+        hpt *= 2;
+    unsigned grid;
+    TRY(grid_of(who, ((uint64_t)in->tokens * ((in->heads + hpt - 1) / hpt) * units + 255) / 256, &grid));
+    const bool copy = out->data != in->data;
+    return for_type(in->dtype, [&](auto t) {
+        using T = decltype(t);
+        auto k = wide ? rope_rows_kernel<T, 16 / sizeof(T)> : rope_rows_kernel<T, 1>;
+        k<<<grid, 256, 0, (cudaStream_t)stream>>>(rows_arg(out), rows_arg(in), rope_arg(rope), in->tokens, in->heads,
+                                                  in->dim, hpt, units, copy);
+        return launched(who);
+    });
+}
+
+xp_status xp_kv_write(void* stream, const xp_pages* pages, const xp_rows* k, const xp_rows* v, const int64_t* slots,
+                      const xp_rotary* rope) {
+    const char* who = "kv_write";
+    TRY(check_pages(who, pages));
+    const uint32_t w = pages->head_dim / 64;
+    TRY(check_rows(who, "k", k, w));
+    TRY(check_rows(who, "v", v, w));
+    REQUIRE(same_shape(k, v) && k->heads == pages->kv_heads && k->dim == pages->head_dim,
+            "%s: 'k', 'v' and the pages differ in shape or type", who);
+    if (rope) TRY(check_rope(who, rope, k->dim, 2 * w));
+    if (k->tokens == 0) return XP_OK;
+    if (rope) TRY(check_rope_data(who, rope));
+    REQUIRE(slots, "%s: argument 'slots' is null", who);
+    unsigned grid;
+    TRY(grid_of(who, ((uint64_t)k->tokens * k->heads + 7) / 8, &grid));
+    return for_type(k->dtype, [&](auto t) {
+        return for_cache(pages->dtype, [&](auto c) {
+            return for_dim(k->dim, [&](auto d) {
+                kv_write_kernel<decltype(t), decltype(c), d.value><<<grid, 256, 0, (cudaStream_t)stream>>>(
+                    pages_arg(pages), rows_arg(k), rows_arg(v), slots, k->tokens, rope_arg(rope), rope != nullptr);
+                return launched(who);
+            });
+        });
+    });
+}
+
+xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, const xp_rows* v, const int64_t* slots) {
+    const char* who = "kv_read";
+    TRY(check_pages(who, pages));
+    TRY(check_rows(who, "k", k, 1));
+    TRY(check_rows(who, "v", v, 1));
+    const uint32_t vec = (uint32_t)(16 / bytes_of(k->dtype));
+    TRY(check_rows(who, "k", k, vec));
+    TRY(check_rows(who, "v", v, vec));
+    REQUIRE(same_shape(k, v) && k->heads == pages->kv_heads && k->dim == pages->head_dim,
+            "%s: 'k', 'v' and the pages differ in shape or type", who);
+    if (k->tokens == 0) return XP_OK;
+    REQUIRE(slots, "%s: argument 'slots' is null", who);
+    unsigned grid;
+    TRY(grid_of(who, ((uint64_t)k->tokens * k->heads * (k->dim / 16) + 255) / 256, &grid));
+    return for_type(k->dtype, [&](auto t) {
+        return for_cache(pages->dtype, [&](auto c) {
+            return for_dim(k->dim, [&](auto d) {
+                kv_read_kernel<decltype(t), decltype(c), d.value><<<grid, 256, 0, (cudaStream_t)stream>>>(
+                    pages_arg(pages), rows_arg(k), rows_arg(v), slots, k->tokens);
+                return launched(who);
+            });
+        });
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+xp_status attention(const char* who, void* stream, const xp_rows* out, const xp_rows* q, const xp_rows* k,
+                    const xp_rows* v, const xp_pages* pages, const int32_t* table, uint32_t table_width,
+                    const int32_t* kv_lens, const int32_t* starts, uint32_t batch, uint32_t q_most, uint32_t window,
+                    float scale, float* lse, void* scratch) {
+    TRY(check_rows(who, "q", q, 8));
+    TRY(check_rows(who, "out", out, 8));
+    REQUIRE(q->dtype != XP_F32, "%s: 'q' must be F16 or BF16", who);
+    REQUIRE(same_shape(q, out), "%s: 'q' and 'out' differ in shape or type", who);
+    REQUIRE(q->dim == 64 || q->dim == 128 || q->dim == 256, "%s: dim must be 64, 128 or 256 (got %u)", who, q->dim);
+    uint32_t kv_heads, cache;
+    if (pages) {
+        TRY(check_pages(who, pages));
+        REQUIRE(pages->head_dim == q->dim, "%s: 'q' and the pages differ in dim", who);
+        REQUIRE(bytes_of(pages->dtype) == 1 || pages->dtype == q->dtype, "%s: 16-bit pages must have q's type", who);
+        kv_heads = pages->kv_heads;
+        cache = pages->dtype;
+    } else {
+        TRY(check_rows(who, "k", k, 8));
+        TRY(check_rows(who, "v", v, 8));
+        REQUIRE(same_shape(k, v) && k->tokens == q->tokens && k->dim == q->dim && k->dtype == q->dtype,
+                "%s: 'q', 'k' and 'v' differ in shape or type", who);
+        kv_heads = k->heads;
+        cache = q->dtype;
+    }
+    REQUIRE(q->heads % kv_heads == 0, "%s: %u heads are no multiple of %u kv heads", who, q->heads, kv_heads);
+    REQUIRE(q->tokens <= 0x7FFFFFFFu && batch <= 0x7FFFFFFFu, "%s: too many tokens or sequences", who);
+    REQUIRE(std::isfinite(scale) && scale >= 0.0f, "%s: scale must be finite and not negative", who);
+    if (q->tokens == 0) return XP_OK;
+    REQUIRE(starts, "%s: argument 'starts' is null", who);
+    REQUIRE(scratch && (uintptr_t)scratch % 16 == 0, "%s: 'scratch' must be 16-byte aligned", who);
+    if (pages) {
+        REQUIRE(kv_lens, "%s: argument 'kv_lens' is null", who);
+        REQUIRE(table || table_width == 0, "%s: argument 'table' is null", who);
+        REQUIRE(((uint64_t)table_width * pages->page_size) < (1ull << 31), "%s: table rows of 2^31 keys or more", who);
+    }
+    ServeAttnArgs a{};
+    a.out = rows_arg(out);
+    a.q = rows_arg(q);
+    if (pages) {
+        a.pages = pages_arg(pages);
+    } else {
+        a.k = rows_arg(k);
+        a.v = rows_arg(v);
+    }
+    a.table = table;
+    a.table_width = table_width;
+    a.kv_lens = kv_lens;
+    a.starts = starts;
+    a.batch = batch;
+    a.tokens = q->tokens;
+    a.heads = q->heads;
+    a.kv_heads = kv_heads;
+    a.group = q->heads / kv_heads;
+    a.q_most = q_most;
+    a.window = window;
+    a.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)q->dim)) * 1.4426950408889634f;
+    a.lse = lse;
+    a.err = static_cast<uint32_t*>(scratch) + 1;
+    return for_type(q->dtype, [&](auto t) {
+        return for_cache(cache, [&](auto c) {
+            return for_dim(q->dim, [&](auto d) {
+                using T = decltype(t);
+                using C = decltype(c);
+                if constexpr (sizeof(T) == 2 && (sizeof(C) == 1 || std::is_same_v<C, T>)) {
+                    attn_rows_kernel<T, C, d.value><<<dim3(q->tokens, q->heads), 128, 0, (cudaStream_t)stream>>>(a);
+                    return launched(who);
+                } else {
+                    return fail(XP_ERR_UNSUPPORTED, "%s: no kernel for these types", who);
+                }
+            });
+        });
+    });
+}
+
+}  // namespace
+
+extern "C" {
+
+xp_status xp_attention_packed(void* stream, const xp_rows* out, const xp_rows* q, const xp_rows* k, const xp_rows* v,
+                              const int32_t* starts, uint32_t batch, uint32_t window, float scale, float* lse,
+                              void* scratch) {
+    return attention("attention_packed", stream, out, q, k, v, nullptr, nullptr, 0, nullptr, starts, batch, 0, window,
+                     scale, lse, scratch);
+}
+
+xp_status xp_attention_paged(void* stream, const xp_rows* out, const xp_rows* q, const xp_pages* pages,
+                             const int32_t* table, uint32_t table_width, const int32_t* kv_lens,
+                             const int32_t* starts, uint32_t batch, uint32_t q_most, uint32_t window, float scale,
+                             float* lse, void* scratch) {
+    REQUIRE(pages, "attention_paged: argument 'pages' is null");
+    return attention("attention_paged", stream, out, q, nullptr, nullptr, pages, table, table_width, kv_lens, starts,
+                     batch, q_most, window, scale, lse, scratch);
+}
+
+}  // extern "C"

@@ -134,7 +134,7 @@ XP_DEV void grid_barrier(uint64_t* counter, uint64_t target, uint32_t* err) {
 // and on a grid-barrier counter nothing increments, each with `limit` polls;
 // both waits give up, record their bits in *err and return, leaving the
 // context usable.
-__global__ void selftest_wait_kernel(uint64_t* counter, uint32_t* err, uint32_t limit) {
+static __global__ void selftest_wait_kernel(uint64_t* counter, uint32_t* err, uint32_t limit) {
     __shared__ uint64_t bar;
     if (threadIdx.x != 0) return;
     mbar_init(&bar, 1);
