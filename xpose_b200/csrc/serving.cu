@@ -3,7 +3,7 @@
 #include <cmath>
 
 #include "host.cuh"
-#include "serving_attn.cuh"
+#include "serving_tile.cuh"
 
 using namespace xp;
 
@@ -44,7 +44,9 @@ xp_status check_pages(const char* who, const xp_pages* p) {
             "%s: page_size must be a power of two from 8 to 256 (got %u)", who, p->page_size);
     REQUIRE(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256,
             "%s: head_dim must be 64, 128 or 256 (got %u)", who, p->head_dim);
-    REQUIRE(p->kv_heads && p->num_pages && p->num_pages < (1ull << 31), "%s: the pages are empty or too many", who);
+    REQUIRE(p->kv_heads && p->num_pages && p->num_pages < (1ull << 31) &&
+                p->num_pages * p->page_size < 0xFFFFFFFFull / p->kv_heads,
+            "%s: the pages are empty, or have 2^32 rows or more", who);
     REQUIRE(bytes_of(p->dtype) > 1 || (p->k_scale && p->v_scale), "%s: 8-bit pages need scales", who);
     REQUIRE((((uintptr_t)p->k | (uintptr_t)p->v) & 15) == 0 && (((uintptr_t)p->k_scale | (uintptr_t)p->v_scale) & 3) == 0,
             "%s: pages must be 16-byte aligned", who);
@@ -75,6 +77,33 @@ PagesArg pages_arg(const xp_pages* p) {
 }
 
 // Calls f with a value of the type (and the W = dim / 64) that was asked for.
+template <class T, class C, int W>
+xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, cudaStream_t st) {
+    using G = AtCfg<T, C, W>;
+    static_assert(G::smem <= 227 * 1024 && AT_MAX_BATCH * 4 <= G::row_off, "shared memory");
+    static std::atomic<bool> attr_set[kMaxDevices];
+    auto kernel = attn_tile_kernel<T, C, W>;
+    if (cudaError_t e = smem_attr_once(attr_set, kernel, G::smem); e != cudaSuccess)
+        return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count(), AT_MAX_CTAS);
+    AtWork w{};
+    w.slot_bytes = G::ROWS * (G::D * 4 + 8);
+    w.heads = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(scratch) + 256);
+    w.slots = static_cast<unsigned char*>(scratch) + 16384;
+    static_assert(256 + 2 * AT_MAX_CTAS * 16 <= 16384 &&
+                      16384 + 2ull * AT_MAX_CTAS * G::ROWS * (G::D * 4 + 8) <= XP_SERVING_SCRATCH_BYTES,
+                  "scratch");
+    w.sub_tokens = 128 / a.group;
+    w.tile_tokens = w.sub_tokens * G::NQ;
+    w.least_units = 2;
+    w.split_over = 3;
+    cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, false, a, w);
+    if (e == cudaSuccess)
+        e = launch_ex(attn_join_kernel<T, W, G::ROWS>, dim3(ctas, G::ROWS / 32), dim3(256), 0, st, 1, true, a, w, ctas);
+    if (e != cudaSuccess) return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    return XP_OK;
+}
+
 template <class F> xp_status for_type(uint32_t dtype, F f) {
     switch (dtype) {
         case XP_F32: return f(float{});
@@ -245,7 +274,9 @@ xp_status attention(const char* who, void* stream, const xp_rows* out, const xp_
         cache = q->dtype;
     }
     REQUIRE(q->heads % kv_heads == 0, "%s: %u heads are no multiple of %u kv heads", who, q->heads, kv_heads);
-    REQUIRE(q->tokens <= 0x7FFFFFFFu && batch <= 0x7FFFFFFFu, "%s: too many tokens or sequences", who);
+    REQUIRE(q->heads / kv_heads <= 128, "%s: more than 128 heads share a kv head", who);
+    REQUIRE(batch <= AT_MAX_BATCH, "%s: at most %u sequences a call", who, AT_MAX_BATCH);
+    REQUIRE(q->tokens <= 0x7FFFFFFFu, "%s: too many tokens", who);
     REQUIRE(std::isfinite(scale) && scale >= 0.0f, "%s: scale must be finite and not negative", who);
     if (q->tokens == 0) return XP_OK;
     REQUIRE(starts, "%s: argument 'starts' is null", who);
@@ -284,8 +315,11 @@ xp_status attention(const char* who, void* stream, const xp_rows* out, const xp_
                 using T = decltype(t);
                 using C = decltype(c);
                 if constexpr (sizeof(T) == 2 && (sizeof(C) == 1 || std::is_same_v<C, T>)) {
-                    attn_rows_kernel<T, C, d.value><<<dim3(q->tokens, q->heads), 128, 0, (cudaStream_t)stream>>>(a);
-                    return launched(who);
+                    if (pages && (uint64_t)q_most * a.group <= 16) {
+                        attn_rows_kernel<T, C, d.value><<<dim3(q->tokens, q->heads), 128, 0, (cudaStream_t)stream>>>(a);
+                        return launched(who);
+                    }
+                    return launch_tiles<T, C, d.value>(who, a, scratch, (cudaStream_t)stream);
                 } else {
                     return fail(XP_ERR_UNSUPPORTED, "%s: no kernel for these types", who);
                 }

@@ -1,0 +1,1061 @@
+// Attention of many rows on the 5th-generation tensor cores: whole prompts,
+// and chunks of new tokens over pages.
+//
+// One CTA an SM works through tiles of 128 * NQ rows. The rows of a tile are
+// whole tokens times the `group` query heads that share one kv head, so K and
+// V are read once for all of them. For each 128 keys:
+//   S = Q K^T        tcgen05.mma, operands in shared memory, S in TMEM
+//   P = 2^(S - m)    one thread a row, S and P in TMEM, P in 16 bits over S
+//   O += P V         tcgen05.mma with P from TMEM, O in TMEM
+// m is the row's maximum when it was last set: it follows a new maximum only
+// when that is more than 2^8 away (O and l are then scaled), so O is seldom
+// touched between two products; P up to 2^8 loses nothing in either type.
+//
+// dim 64 and 128: two row tiles (NQ = 2) share every K and V tile, and the
+// softmax of one runs beside the products of the other. dim 256: O fills half
+// of TMEM, so one row tile (NQ = 1) with two S buffers; the products of one
+// key tile run beside the softmax of the next.
+//
+// K and V move in 16 KB pieces through one ring (K: 128 keys x 64 dims, V:
+// 8192 / dim keys x dim), so a ring slot is free again as soon as its piece
+// is multiplied. Loader threads copy rows of 16 bytes (cp.async) into the
+// 128-byte swizzled layouts of the tensor core: the rows of a paged cache sit
+// anywhere, and keys outside the tile's range become zeros on the way, so
+// that nothing of a stale page is ever multiplied. 8-bit codes are turned
+// into exact 16-bit values by the loader; their scales never touch them: with
+// t_ij = s_ij ks_j + log2 vs_j the weight that multiplies v's code is 2^(t -
+// m), and l adds 2^(t - m) / vs_j. A weight is then rounded relative to the
+// largest contribution, whatever the scales.
+//
+// Work is split evenly: every CTA takes the same number of (row tile, key
+// tile) units, so the last tile of a call does not run alone. A row tile that
+// two or more CTAs share leaves partial sums (O, m, l) that a second, small
+// launch joins in a fixed order.
+#pragma once
+#include "serving_attn.cuh"
+#include "tk_primitives.cuh"
+
+namespace xp {
+
+constexpr int AT_KEYS = 128;        // keys of a tile
+constexpr int AT_PIECE = 16384;     // bytes of a ring slot
+constexpr uint32_t AT_NONE = 0xFFFFFFFFu;
+constexpr uint32_t AT_SPIN_LIMIT = 1u << 20;
+constexpr uint32_t AT_MAX_CTAS = 180;   // partial slots that the scratch holds
+constexpr uint32_t AT_MAX_BATCH = 16384;
+
+template <class T, class C, int W> struct AtCfg {
+    static constexpr int D = 64 * W;
+    static constexpr bool Q8 = sizeof(C) == 1;
+    static constexpr int NQ = W == 4 ? 1 : 2;     // row tiles of a CTA
+    static constexpr int NB = 2 / NQ;             // S buffers of a row tile
+    static constexpr int ROWS = 128 * NQ;
+    static constexpr int LAG = NB;                // K runs this many tiles ahead of V
+    static constexpr int NSLOT = (Q8 && W > 1) ? 9 : 10;
+    static constexpr int NPIECE = W;              // pieces of a K (or V) tile
+    static constexpr int VKEYS = AT_KEYS / W;     // keys of a V piece
+    static constexpr int NSTAGE = W == 1 ? 8 : 4; // tiles whose row numbers and scales are kept
+    static constexpr int THREADS = 128 * NQ + 256;
+    // pieces issued and not yet given to the tensor core. With two row tiles a
+    // slot is free only once the rest of its tile and the next K are in too.
+    static constexpr int DEPTH = Q8 ? 1 : W == 4 ? 6 : 5;
+    static_assert(DEPTH + (NQ == 2 ? 2 * W : 1) <= NSLOT, "the loader would wait for itself");
+    // shared memory
+    static constexpr int q_off = 0;
+    static constexpr int ring_off = NQ * W * AT_PIECE;
+    static constexpr int row_off = ring_off + NSLOT * AT_PIECE;       // [NSTAGE][128] row numbers
+    static constexpr int sc_off = row_off + NSTAGE * 512;             // [NSTAGE][3][128] floats, 8-bit pages
+    static constexpr int bar_off = sc_off + (Q8 ? NSTAGE * 1536 : 0);
+    static constexpr int smem = bar_off + 512;                        // barriers, plan, sums, flags
+};
+
+struct AtWork {
+    unsigned char* slots;   // partial sums: two of slot_bytes a CTA
+    uint32_t* heads;        // [2 * CTAs][4]: kind, b, h, tile of each
+    uint32_t slot_bytes;
+    uint32_t tile_tokens;   // tokens of a tile
+    uint32_t sub_tokens;    // tokens of one of its NQ row tiles
+    uint32_t least_units;   // units of a CTA, at least
+    uint32_t split_over;    // split tiles when the largest has this many units more than an even share
+};
+enum : uint32_t { AT_FULL = 0, AT_FIRST = 1, AT_MIDDLE = 2, AT_LAST = 3 };
+
+// ---- tcgen05 ------------------------------------------------------------------
+XP_DEV uint64_t at_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    // 128-byte swizzle (layout type 2), descriptor version 1
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+template <class T> XP_DEV uint32_t at_idesc(uint32_t n, bool b_mn) {
+    const uint32_t f = std::is_same_v<T, bf16> ? 1u : 0u;
+    return (1u << 4) | (f << 7) | (f << 10) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+XP_DEV void at_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+XP_DEV void at_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+        "r"(acc)
+        : "memory");
+}
+XP_DEV void at_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+XP_DEV void at_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+XP_DEV void at_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+#define AT_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define AT_I8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+// 32 columns of the thread's TMEM lane
+XP_DEV void at_ld32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : AT_R8(r, 0), AT_R8(r, 8), AT_R8(r, 16), AT_R8(r, 24)
+        : "r"(addr));
+}
+XP_DEV void at_st32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::AT_I8(r, 0),
+        AT_I8(r, 8), AT_I8(r, 16), AT_I8(r, 24), "r"(addr)
+        : "memory");
+}
+XP_DEV void at_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+XP_DEV void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N> XP_DEV void at_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> XP_DEV void at_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+XP_DEV bool at_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+// Bounded: a wait that runs out reports it and lets every later wait of the
+// CTA pass, so the kernel ends (with unspecified output).
+XP_DEV void at_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err) {
+    uint32_t it = 0;
+    while (!at_try(bar, parity)) {
+        if (*dead) return;
+        if (++it > AT_SPIN_LIMIT) {
+            *dead = 1;
+            atomicOr(err, SERVE_ERR_WAIT);
+            return;
+        }
+    }
+}
+XP_DEV void at_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+XP_DEV float at_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// two fp32 lanes at a time
+XP_DEV float2 at_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+          "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+XP_DEV float2 at_add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+template <class T> XP_DEV uint32_t at_pack(float lo, float hi) {
+    uint32_t r;
+    if constexpr (std::is_same_v<T, bf16>) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 4 codes -> 4 exact 16-bit values
+template <class T> XP_DEV uint2 at_codes(uint32_t w, int8c) {
+    uint2 r;
+    if constexpr (std::is_same_v<T, bf16>) {
+        // a biased code as the low bits of 2^23: exact fp32, then exact bf16 (8 bits)
+        const uint32_t u = w ^ 0x80808080u;
+        const float f0 = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)) - 8388736.0f;
+        const float f1 = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441)) - 8388736.0f;
+        const float f2 = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)) - 8388736.0f;
+        const float f3 = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - 8388736.0f;
+        r.x = at_pack<bf16>(f0, f1);
+        r.y = at_pack<bf16>(f2, f3);
+    } else {
+        // ... and of 2^10: 1024 + 128 + code, exact fp16
+        const uint32_t u = w ^ 0x80808080u;
+        const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+        uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(reinterpret_cast<__half2&>(a), bias), y = __hsub2(reinterpret_cast<__half2&>(b), bias);
+        r.x = reinterpret_cast<const uint32_t&>(x);
+        r.y = reinterpret_cast<const uint32_t&>(y);
+    }
+    return r;
+}
+template <class T> XP_DEV uint2 at_codes(uint32_t w, fp8c) {
+    uint32_t a, b;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"((uint16_t)w));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"((uint16_t)(w >> 16)));
+    if constexpr (std::is_same_v<T, bf16>) {
+        const float2 x = __half22float2(reinterpret_cast<__half2&>(a)), y = __half22float2(reinterpret_cast<__half2&>(b));
+        a = at_pack<bf16>(x.x, x.y);
+        b = at_pack<bf16>(y.x, y.y);
+    }
+    return make_uint2(a, b);
+}
+XP_DEV void at_cp16(uint32_t dst, const void* src, bool has) {
+    const uint32_t n = has ? 16u : 0u;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+template <int N> XP_DEV void at_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+XP_DEV void at_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+XP_DEV uint32_t at_lds(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+XP_DEV uint4 at_lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+XP_DEV void at_sts16(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// ---- the split of the work --------------------------------------------------------
+// Tile x of a sequence: tokens [x tt, ..), its key range [lo, hi) and the key
+// tiles that cover it.
+struct AtTile { int32_t lo, hi; uint32_t t0, n; };
+XP_DEV AtTile at_tile(const Seq& s, uint32_t x, uint32_t tt, uint32_t window) {
+    AtTile r;
+    const int32_t first = (int32_t)s.nkv - (int32_t)s.nq;
+    const uint32_t tok0 = x * tt, tok1 = min(tok0 + tt, s.nq);
+    r.hi = max(first + (int32_t)tok1, 0);
+    const int64_t lo = window ? (int64_t)first + tok0 + 1 - (int64_t)window : 0;
+    r.lo = (int32_t)min(max(lo, (int64_t)0), (int64_t)r.hi);
+    r.t0 = (uint32_t)r.lo / AT_KEYS;
+    r.n = r.hi > r.lo ? ((uint32_t)r.hi + AT_KEYS - 1) / AT_KEYS - r.t0 : 0;
+    return r;
+}
+
+// Where a CTA starts in the list of units: head h, sequence b, tile x. A tile
+// without keys counts as one unit.
+struct AtPlan {
+    uint32_t h, b, x, skip;   // skip: key tiles of the first tile that an earlier CTA has
+    int64_t todo;             // units from there; whole tiles: those that start within them
+    bool split;
+};
+
+XP_DEV uint32_t at_scan(uint32_t v, uint32_t* warp_sums, uint32_t nthreads, uint32_t& total) {
+    // inclusive scan over the CTA; warp_sums: 32 words of shared memory
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= (uint32_t)o) v += y;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    uint32_t before = 0, sum = 0;
+    for (uint32_t i = 0; i < nthreads / 32; ++i) {
+        const uint32_t y = warp_sums[i];
+        if (i < warp) before += y;
+        sum += y;
+    }
+    total = sum;
+    return v + before;
+}
+
+// Every thread of every CTA computes the same plan from the lengths alone.
+// `ends`: shared memory for one word a sequence.
+template <int THREADS>
+XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends, uint32_t* sums, AtPlan* out) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t tiles = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += THREADS) {
+        const uint32_t b = b0 + tid;
+        const uint32_t n = b < a.batch ? (seq_of(a, b).nq + w.tile_tokens - 1) / w.tile_tokens : 0;
+        uint32_t sum;
+        const uint32_t end = tiles + at_scan(n, sums, THREADS, sum);
+        if (b < a.batch) ends[b] = end;
+        tiles += sum;
+    }
+    __syncthreads();
+    // units of a tile; its sequence by bisection
+    auto units = [&](uint32_t i, uint32_t& b, uint32_t& x) {
+        uint32_t lo = 0, hi = a.batch - 1;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (ends[mid] > i) hi = mid;
+            else lo = mid + 1;
+        }
+        b = lo;
+        x = i - (lo ? ends[lo - 1] : 0);
+        return max(at_tile(seq_of(a, b), x, w.tile_tokens, a.window).n, 1u);
+    };
+    uint64_t all = 0;
+    uint32_t most = 0, b = 0, x = 0;
+    for (uint32_t i0 = 0; i0 < tiles; i0 += THREADS) {
+        const uint32_t i = i0 + tid, n = i < tiles ? units(i, b, x) : 0;
+        uint32_t sum;
+        at_scan(n, sums, THREADS, sum);
+        all += sum;
+        most = max(most, n);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    __syncthreads();
+    if ((tid & 31) == 0) sums[tid >> 5] = most;
+    if (tid == 0) out->todo = 0;
+    __syncthreads();
+    for (int i = 0; i < THREADS / 32; ++i) most = max(most, sums[i]);
+    __syncthreads();
+    if (all == 0) return;
+    // no CTA has less than a unit, so the parts of a tile are in consecutive CTAs
+    const uint64_t total = all * a.kv_heads, c = blockIdx.x;
+    const uint64_t g = min((uint64_t)gridDim.x, max(total / w.least_units, (uint64_t)1));
+    if (c >= g) return;
+    const uint64_t u0 = total * c / g, u1 = total * (c + 1) / g;
+    const bool split = most > (total + g - 1) / g + w.split_over;
+    if (u0 == u1) return;
+    // the first tile of the range: split, the one that holds u0; else the
+    // first that starts at or after it
+    const uint32_t h0 = (uint32_t)(u0 / all);
+    for (uint32_t h = h0; h < a.kv_heads && h <= h0 + 1; ++h) {
+        uint64_t at = all * h;
+        bool found = false;
+        for (uint32_t i0 = 0; i0 < tiles && !found; i0 += THREADS) {
+            const uint32_t i = i0 + tid, n = i < tiles ? units(i, b, x) : 0;
+            uint32_t sum;
+            const uint64_t end = at + at_scan(n, sums, THREADS, sum), begin = end - n;
+            const bool mine = n && (split ? begin <= u0 && u0 < end : begin >= u0 && begin < u1);
+            if (split) {
+                if (mine) *out = AtPlan{h, b, x, (uint32_t)(u0 - begin), (int64_t)(u1 - u0), true};
+                found = __syncthreads_or(mine);
+            } else {
+                // lowest index among the candidates
+                const uint32_t best = __reduce_min_sync(0xffffffffu, mine ? i : AT_NONE);
+                __syncthreads();
+                if ((tid & 31) == 0) sums[tid >> 5] = best;
+                __syncthreads();
+                uint32_t low = AT_NONE;
+                for (int j = 0; j < THREADS / 32; ++j) low = min(low, sums[j]);
+                if (mine && i == low) *out = AtPlan{h, b, x, 0, (int64_t)(u1 - begin), false};
+                found = low != AT_NONE;
+                __syncthreads();
+            }
+            at += sum;
+        }
+        if (found || split) break;
+    }
+    __syncthreads();
+}
+
+// The pieces of a CTA's range, one row tile each: every role walks the same list.
+struct AtSeg {
+    uint32_t h, b, x, kind;
+    Seq s;
+    AtTile t;
+    uint32_t k0, n;     // first key tile (in keys / 128) and how many
+};
+struct AtWalk {
+    AtPlan p;
+    Seq s;
+    uint32_t have;      // s is sequence have
+    XP_DEV void start(const AtPlan& plan) { p = plan; have = AT_NONE; }
+    XP_DEV bool next(const ServeAttnArgs& a, const AtWork& w, AtSeg& g) {
+        if (p.todo <= 0) return false;
+        for (;;) {
+            if (have != p.b) {
+                s = seq_of(a, p.b);
+                have = p.b;
+            }
+            if (p.x * w.tile_tokens < s.nq) break;
+            p.x = 0;
+            if (++p.b == a.batch) {
+                p.b = 0;
+                if (++p.h >= a.kv_heads) return false;
+            }
+        }
+        g.h = p.h;
+        g.b = p.b;
+        g.x = p.x;
+        g.s = s;
+        g.t = at_tile(s, p.x, w.tile_tokens, a.window);
+        const uint32_t n = max(g.t.n, 1u);
+        const uint32_t take = p.split ? (uint32_t)min((int64_t)(n - p.skip), p.todo) : n;
+        g.kind = p.skip == 0 ? (take == n ? AT_FULL : AT_FIRST) : (p.skip + take == n ? AT_LAST : AT_MIDDLE);
+        g.k0 = g.t.t0 + p.skip;
+        g.n = g.t.n ? take : 0;
+        p.todo -= take;
+        p.skip = 0;
+        ++p.x;
+        return true;
+    }
+};
+
+// Some row of the tile does not see some key of key tile kt that is loaded.
+XP_DEV bool at_masked(const ServeAttnArgs& a, const AtWork& w, const AtSeg& g, uint32_t kt) {
+    const int64_t p0 = (int64_t)g.s.nkv - g.s.nq + (int64_t)g.x * w.tile_tokens;
+    const int64_t p1 = (int64_t)g.t.hi - 1;
+    const int64_t k0 = max((int64_t)kt * AT_KEYS, (int64_t)g.t.lo), k1 = min((int64_t)(kt + 1) * AT_KEYS, (int64_t)g.t.hi);
+    return k1 > p0 + 1 || (a.window && k0 < p1 - (int64_t)a.window + 1);
+}
+XP_DEV bool at_odd16(uint32_t w, uint32_t exp_mask) {  // an infinity or NaN in either half
+    return (w & exp_mask) == exp_mask || (w & (exp_mask << 16)) == (exp_mask << 16);
+}
+
+template <class T, class C, int W>
+__global__ void __launch_bounds__(AtCfg<T, C, W>::THREADS, 1)
+attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ AtWork w) {
+    using G = AtCfg<T, C, W>;
+    constexpr int D = G::D, NQ = G::NQ, NSLOT = G::NSLOT, NSTAGE = G::NSTAGE;
+    // no static shared memory: the dynamic part then starts on a 1 KB boundary,
+    // which the swizzled layouts need, without a byte lost
+    extern __shared__ __align__(1024) unsigned char sm[];
+    const uint32_t smb = smem_u32(sm);
+    struct Small {
+        AtPlan plan;
+        uint32_t sums[32], bad[4], tmem, dead;
+    };
+    static_assert((2 * NSLOT + 8) * 8 + sizeof(Small) <= 512, "small data");
+    Small& small = *reinterpret_cast<Small*>(sm + G::bar_off + (2 * NSLOT + 8) * 8);
+    AtPlan& s_plan = small.plan;
+    uint32_t *const s_sums = small.sums, *const s_bad = small.bad;
+    volatile uint32_t& s_dead = small.dead;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // barriers
+    const uint32_t b_full = smb + G::bar_off, b_empty = b_full + NSLOT * 8, b_q = b_empty + NSLOT * 8;
+    const uint32_t b_s = b_q + 16, b_p = b_s + 16, b_o = b_p + 16;
+
+    if (smb & 1023) {  // cannot be multiplied from
+        if (tid == 0) atomicOr(a.err, SERVE_ERR_WAIT);
+        return;
+    }
+    if (tid == 0) {
+        uint64_t* m = reinterpret_cast<uint64_t*>(sm + G::bar_off);
+        for (int i = 0; i < NSLOT; ++i) {
+            mbar_init(m + i, 4);
+            mbar_init(m + NSLOT + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(m + 2 * NSLOT + i, 4);
+            mbar_init(m + 2 * NSLOT + 2 + i, 1);
+            mbar_init(m + 2 * NSLOT + 4 + i, 4);
+            mbar_init(m + 2 * NSLOT + 6 + i, 1);
+        }
+        fence_mbar_init();
+        s_dead = 0;
+        for (int i = 0; i < 4; ++i) s_bad[i] = 0;
+    }
+    if (warp == NQ * 4 + 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&small.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // rows of q in no sequence
+    {
+        const uint32_t lo = (uint32_t)min(max(__ldg(a.starts), 0), (int32_t)a.tokens);
+        const uint32_t hi = (uint32_t)min(max(__ldg(a.starts + a.batch), 0), (int32_t)a.tokens);
+        const uint32_t n = lo + (a.tokens - max(hi, lo));
+        for (uint64_t i = (uint64_t)blockIdx.x * G::THREADS + tid; i < (uint64_t)n * a.heads * (D / 8);
+             i += (uint64_t)gridDim.x * G::THREADS) {
+            const uint32_t d = (uint32_t)(i % (D / 8)) * 8, h = (uint32_t)(i / (D / 8) % a.heads);
+            uint32_t tok = (uint32_t)(i / (D / 8) / a.heads);
+            if (tok >= lo) tok += max(hi, lo) - lo;
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out.data) + (int64_t)tok * a.out.ts + (int64_t)h * a.out.hs + d) =
+                make_uint4(0, 0, 0, 0);
+            if (a.lse && d == 0) a.lse[(uint64_t)tok * a.heads + h] = -INFINITY;
+        }
+    }
+    at_make_plan<G::THREADS>(a, w, reinterpret_cast<uint32_t*>(sm), s_sums, &s_plan);
+    at_fence_before();
+    __syncthreads();
+    at_fence_after();
+    pdl_launch_dependents();
+    const uint32_t tmem = small.tmem;
+    AtWalk walk;
+    walk.start(s_plan);
+    AtSeg g;
+    uint32_t* const err = a.err;
+
+    if (warp < NQ * 4) {
+        // ------------------------------ softmax ------------------------------
+        if constexpr (NQ == 2) at_regs_up<192>();
+        else at_regs_up<232>();
+        const uint32_t wg = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (warp & 3) * 32 << 16;
+        const uint32_t o_tm = tmem + lanes + 256 + wg * D;
+        if (tid == 0) {
+            w.heads[(2 * blockIdx.x) * 4] = AT_FULL;
+            w.heads[(2 * blockIdx.x + 1) * 4] = AT_FULL;
+        }
+        const uint32_t qrow0 = wg * w.sub_tokens;  // first token of this row tile in its CTA's tile
+        uint32_t stage = 0, nsfull[2] = {0, 0}, npv = 0, seg = 0;
+        while (walk.next(a, w, g)) {
+            ++seg;
+            // this thread's row
+            const uint32_t rt = row / a.group, rg = row - rt * a.group;
+            const uint32_t tok = g.x * w.tile_tokens + qrow0 + rt;
+            const bool real = rt < w.sub_tokens && tok < g.s.nq;
+            const int32_t pos = (int32_t)g.s.nkv - (int32_t)g.s.nq + (int32_t)tok;
+            int32_t klo = 0, khi = 0x7FFFFFFF;  // a padding row masks nothing: its scores are zeros
+            if (real) {
+                khi = max(pos + 1, 0);
+                klo = a.window ? (int32_t)max((int64_t)pos + 1 - (int64_t)a.window, (int64_t)0) : 0;
+            }
+            if (g.n) {
+                // Q into the swizzled layout: 8 values a piece, neighbouring threads along a row
+                const uint32_t qs = smb + G::q_off + wg * W * AT_PIECE;
+                constexpr int PR = D / 8;  // 16-byte pieces of a row
+#pragma unroll 1
+                for (uint32_t i0 = 0; i0 < (uint32_t)PR; i0 += 8) {
+                    uint4 v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t id = (i0 + i) * 128 + row, r = id / PR, c = id % PR;
+                        const uint32_t t1 = r / a.group, g1 = r - t1 * a.group;
+                        const uint32_t tk = g.x * w.tile_tokens + qrow0 + t1;
+                        v[i] = make_uint4(0, 0, 0, 0);
+                        if (t1 < w.sub_tokens && tk < g.s.nq)
+                            v[i] = __ldg(reinterpret_cast<const uint4*>(
+                                static_cast<const T*>(a.q.data) + (int64_t)(g.s.q0 + tk) * a.q.ts +
+                                (int64_t)(g.h * a.group + g1) * a.q.hs + c * 8));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t id = (i0 + i) * 128 + row, r = id / PR, c = id % PR;
+                        at_sts16(qs + (c >> 3) * AT_PIECE + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[i]);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) at_arrive(b_q + 8 * wg);
+            }
+            float m = -INFINITY, ref = 0.0f;
+            float2 l2[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+#pragma unroll 1
+            for (uint32_t t = 0; t < g.n; ++t) {
+                const uint32_t buf = NQ == 2 ? wg : (t & 1);
+                const uint32_t s_tm = tmem + lanes + buf * 128;
+                at_wait(b_s + 8 * buf, nsfull[NQ == 2 ? 0 : buf]++ & 1, &s_dead, err);
+                at_fence_after();
+                float s[128];
+                {
+                    uint32_t* r = reinterpret_cast<uint32_t*>(s);
+                    at_ld32(s_tm, r);
+                    at_ld32(s_tm + 32, r + 32);
+                    at_ld32(s_tm + 64, r + 64);
+                    at_ld32(s_tm + 96, r + 96);
+                    at_wait_ld();
+                }
+                const float* sc = reinterpret_cast<const float*>(sm + G::sc_off) + stage * 384;
+                if constexpr (G::Q8) {
+#pragma unroll
+                    for (int j = 0; j < 128; j += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4*>(sc + j);
+                        const float4 v4 = *reinterpret_cast<const float4*>(sc + 128 + j);
+                        const float2 x = at_fma2({s[j], s[j + 1]}, {k4.x, k4.y}, {v4.x, v4.y});
+                        const float2 y = at_fma2({s[j + 2], s[j + 3]}, {k4.z, k4.w}, {v4.z, v4.w});
+                        s[j] = x.x;
+                        s[j + 1] = x.y;
+                        s[j + 2] = y.x;
+                        s[j + 3] = y.y;
+                    }
+                }
+                const int32_t kt = (int32_t)((g.k0 + t) * AT_KEYS);
+                if (__any_sync(0xffffffffu, kt < klo || khi - kt < AT_KEYS)) {
+                    const uint32_t off = (uint32_t)(kt - klo), span = (uint32_t)(khi > klo ? khi - klo : 0);
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (off + j >= span) s[j] = -INFINITY;
+                }
+                float mx = fmaxf(s[0], s[1]), mx1 = fmaxf(s[2], s[3]);
+#pragma unroll
+                for (int j = 4; j < 128; j += 4) {
+                    mx = fmaxf(mx, fmaxf(s[j], s[j + 1]));
+                    mx1 = fmaxf(mx1, fmaxf(s[j + 2], s[j + 3]));
+                }
+                mx = fmaxf(mx, mx1);
+                if constexpr (!G::Q8) mx *= a.scale_log2;
+                const bool up = mx > m + 8.0f || (m == -INFINITY && mx > -INFINITY);
+                if (__any_sync(0xffffffffu, up)) {
+                    const float f = up ? at_ex2(m - mx) : 1.0f;
+                    if (up) m = ref = mx;
+                    if (t != 0) {
+                        // O so far by the same factor, once the product before this one is in it
+                        at_wait(b_o + 8 * wg, (npv - 1) & 1, &s_dead, err);
+                        at_fence_after();
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            float o[32];
+                            at_ld32(o_tm + c, reinterpret_cast<uint32_t*>(o));
+                            at_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= f;
+                            at_st32(o_tm + c, reinterpret_cast<uint32_t*>(o));
+                        }
+                        at_wait_st();
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            l2[i].x *= f;
+                            l2[i].y *= f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int j = 0; j < 64; j += 4) {
+                        float* x = s + half * 64 + j;
+                        float2 e0, e1;
+                        if constexpr (G::Q8) {
+                            e0 = at_add2({x[0], x[1]}, {-ref, -ref});
+                            e1 = at_add2({x[2], x[3]}, {-ref, -ref});
+                        } else {
+                            const float2 k2 = {a.scale_log2, a.scale_log2}, r2 = {-ref, -ref};
+                            e0 = at_fma2({x[0], x[1]}, k2, r2);
+                            e1 = at_fma2({x[2], x[3]}, k2, r2);
+                        }
+                        e0 = {at_ex2(e0.x), at_ex2(e0.y)};
+                        e1 = {at_ex2(e1.x), at_ex2(e1.y)};
+                        if constexpr (G::Q8) {
+                            const float4 r4 = *reinterpret_cast<const float4*>(sc + 256 + half * 64 + j);
+                            l2[0] = at_fma2(e0, {r4.x, r4.y}, l2[0]);
+                            l2[1] = at_fma2(e1, {r4.z, r4.w}, l2[1]);
+                        } else {
+                            l2[0] = at_add2(l2[0], e0);
+                            l2[1] = at_add2(l2[1], e1);
+                        }
+                        p[j / 2] = at_pack<T>(e0.x, e0.y);
+                        p[j / 2 + 1] = at_pack<T>(e1.x, e1.y);
+                    }
+                    at_st32(s_tm + half * 32, p);
+                }
+                at_wait_st();
+                at_fence_before();
+                __syncwarp();
+                if (lane == 0) at_arrive(b_p + 8 * buf);
+                ++npv;
+                stage = stage + 1 == NSTAGE ? 0 : stage + 1;
+            }
+            // ---- the row tile's result ----
+            const float l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
+            if (g.n) {
+                if (NQ == 1 && g.n > 1) at_wait(b_o + 8 * wg, (npv - 2) & 1, &s_dead, err);
+                at_wait(b_o + 8 * wg, (npv - 1) & 1, &s_dead, err);
+                at_fence_after();
+            }
+            const bool bad = !G::Q8 && *reinterpret_cast<volatile uint32_t*>(&s_bad[seg & 3]) == seg;
+            const bool whole = g.kind == AT_FULL;
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;   // l is 0 where the row saw nothing
+            const uint32_t slot = 2 * blockIdx.x + (g.kind == AT_FIRST ? 1 : 0);
+            unsigned char* part = w.slots + (size_t)slot * w.slot_bytes;
+            const uint64_t orow = (uint64_t)(g.s.q0 + tok), ohead = g.h * a.group + rg;
+            T* op = static_cast<T*>(a.out.data) + (int64_t)orow * a.out.ts + (int64_t)ohead * a.out.hs;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
+                if (g.n) {
+                    at_ld32(o_tm + c, reinterpret_cast<uint32_t*>(o));
+                    at_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                }
+                if (bad && real) {
+                    // infinities and NaN of v were left out of the products of tiles
+                    // where not every row sees every key: they go to the rows that do
+                    for (uint32_t t = 0; t < g.n; ++t) {
+                        if (!at_masked(a, w, g, g.k0 + t)) continue;
+                        const int32_t j0 = max((int32_t)((g.k0 + t) * AT_KEYS), klo);
+                        const int32_t j1 = min(min((int32_t)((g.k0 + t + 1) * AT_KEYS), khi), g.t.hi);
+                        for (int32_t j = j0; j < j1; ++j) {
+                            const T* vp;
+                            if (a.pages.k) {
+                                const int32_t page = __ldg(a.table + (uint64_t)g.b * a.table_width + (j >> a.pages.page_shift));
+                                const uint64_t sl = ((uint64_t)(uint32_t)page << a.pages.page_shift) + (j & ((1u << a.pages.page_shift) - 1));
+                                if (page < 0 || sl >= a.pages.slots) continue;
+                                vp = static_cast<const T*>(a.pages.v) + page_row(a.pages, sl, g.h) * D + c;
+                            } else {
+                                vp = static_cast<const T*>(a.v.data) + (int64_t)(g.s.q0 + j) * a.v.ts + (int64_t)g.h * a.v.hs + c;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float v = to_f32(vp[i]);
+                                if (!(fabsf(v) <= 3.4028235e38f)) o[i] += v;
+                            }
+                        }
+                    }
+                }
+                if (whole) {
+                    if (real) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint4 r;
+                            r.x = at_pack<T>(o[i] * inv, o[i + 1] * inv);
+                            r.y = at_pack<T>(o[i + 2] * inv, o[i + 3] * inv);
+                            r.z = at_pack<T>(o[i + 4] * inv, o[i + 5] * inv);
+                            r.w = at_pack<T>(o[i + 6] * inv, o[i + 7] * inv);
+                            *reinterpret_cast<uint4*>(op + c + i) = r;
+                        }
+                    }
+                } else if (real) {
+                    float4* pp = reinterpret_cast<float4*>(part) + (size_t)(c / 4) * G::ROWS + wg * 128 + row;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) pp[(size_t)(i / 4) * G::ROWS] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            at_fence_before();
+            if (whole) {
+                if (a.lse && real)
+                    a.lse[orow * a.heads + ohead] = l != 0.0f ? (ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            } else {
+                float2* ml = reinterpret_cast<float2*>(part + (size_t)G::ROWS * D * 4);
+                ml[wg * 128 + row] = make_float2(ref, l);
+                if (tid == 0) *reinterpret_cast<uint4*>(w.heads + slot * 4) = make_uint4(g.kind, g.b, g.h, g.x);
+            }
+        }
+    } else if (warp < NQ * 4 + 4) {
+        // ------------------------------ loader ------------------------------
+        if constexpr (NQ == 2) at_regs_down<80>();
+        else at_regs_down<136>();
+        const uint32_t lt = tid - NQ * 128;
+        uint32_t pieces = 0, given = 0;  // pieces issued, and given to the tensor core
+        uint32_t check = 0;              // bit i: the piece issued i before the last is of a V tile to be looked over
+        uint32_t stage = 0, seg = 0;
+        uint4 raw[4];                 // 8-bit: the codes of the piece issued last
+        uint32_t raw_kind = 0;        // ... 0 none, 1 K, 2 V
+        const uint32_t rows0 = smb + G::row_off;
+        // thread -> 16-byte units of a piece: unit u of rows r0, r0 + step, ..
+        constexpr int KU = G::Q8 ? 4 : 8, VU = (G::Q8 ? 4 : 8) * W, NU = G::Q8 ? 4 : 8;
+        // where unit u of key r of a V piece goes: blocks of 64 dims, keys in rows of 128 bytes
+        auto v_at = [&](uint32_t r, uint32_t c) { return (c >> 3) * (G::VKEYS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+        auto k_at = [&](uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); };
+
+        // a piece is in: give it to the tensor core
+        auto publish = [&](uint32_t index, bool look) {
+            const uint32_t slot = index % NSLOT, base = smb + G::ring_off + slot * AT_PIECE;
+            if (!G::Q8 && look) {
+                constexpr uint32_t mask = std::is_same_v<T, bf16> ? 0x7F80u : 0x7C00u;
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t r = lt / VU + i * (128 / VU), c = lt % VU, at = base + v_at(r, c);
+                    uint4 v = at_lds16(at);
+                    if (at_odd16(v.x, mask) || at_odd16(v.y, mask) || at_odd16(v.z, mask) || at_odd16(v.w, mask)) {
+                        odd = true;
+                        uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+                        for (int j = 0; j < 4; ++j) {
+                            if ((x[j] & mask) == mask) x[j] &= 0xFFFF0000u;
+                            if ((x[j] & (mask << 16)) == (mask << 16)) x[j] &= 0xFFFFu;
+                        }
+                        at_sts16(at, v);
+                    }
+                }
+                if (odd) s_bad[seg & 3] = seg;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) at_arrive(b_full + 8 * slot);
+        };
+        // 8-bit: the codes in `raw` into their slot, as 16-bit values
+        auto convert = [&]() {
+            if constexpr (G::Q8) {
+            if (raw_kind == 0) return;
+            const uint32_t index = pieces - 1, slot = index % NSLOT, base = smb + G::ring_off + slot * AT_PIECE;
+            if (index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint2 x0 = at_codes<T>(raw[i].x, C{}), x1 = at_codes<T>(raw[i].y, C{});
+                const uint2 x2 = at_codes<T>(raw[i].z, C{}), x3 = at_codes<T>(raw[i].w, C{});
+                uint32_t d0, d1;
+                if (raw_kind == 1) {
+                    const uint32_t r = lt / KU + i * (128 / KU), c = 2 * (lt % KU);
+                    d0 = k_at(r, c);
+                    d1 = k_at(r, c + 1);
+                } else {
+                    const uint32_t r = lt / VU + i * (128 / VU), c = 2 * (lt % VU);
+                    d0 = v_at(r, c);
+                    d1 = v_at(r, c + 1);
+                }
+                at_sts16(base + d0, make_uint4(x0.x, x0.y, x1.x, x1.y));
+                at_sts16(base + d1, make_uint4(x2.x, x2.y, x3.x, x3.y));
+            }
+            publish(index, false);
+            raw_kind = 0;
+            }
+        };
+        auto piece = [&](bool is_v, uint32_t c, uint32_t st, bool look) {
+            const uint32_t u = is_v ? lt % VU : lt % KU, r0 = is_v ? lt / VU : lt / KU;
+            const uint32_t step = is_v ? 128 / VU : 128 / KU, key0 = is_v ? c * G::VKEYS : 0;
+            const uint32_t d = (is_v ? u : c * KU + u) * (G::Q8 ? 16 : 8);
+            const C* src;
+            int64_t stride;
+            if (a.pages.k) {
+                src = static_cast<const C*>(is_v ? a.pages.v : a.pages.k) + d;
+                stride = D;
+            } else {
+                const RowsArg& x = is_v ? a.v : a.k;
+                src = static_cast<const C*>(x.data) + (int64_t)g.h * x.hs + d;
+                stride = x.ts;
+            }
+            if constexpr (G::Q8) {
+                uint4 now[4];
+#pragma unroll
+                for (int i = 0; i < NU; ++i) {
+                    const uint32_t r = at_lds(rows0 + st * 512 + (key0 + r0 + i * step) * 4);
+                    now[i] = make_uint4(0, 0, 0, 0);
+                    if (r != AT_NONE) now[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * stride));
+                }
+                convert();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[i] = now[i];
+                raw_kind = is_v ? 2 : 1;
+                ++pieces;
+            } else {
+                const uint32_t slot = pieces % NSLOT, base = smb + G::ring_off + slot * AT_PIECE;
+                if (pieces >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (pieces / NSLOT - 1) & 1, &s_dead, err);
+#pragma unroll
+                for (int i = 0; i < NU; ++i) {
+                    const uint32_t rr = r0 + i * step, r = at_lds(rows0 + st * 512 + (key0 + rr) * 4);
+                    const bool has = r != AT_NONE;
+                    at_cp16(base + (is_v ? v_at(rr, u) : k_at(rr, u)), src + (has ? (int64_t)r * stride : 0), has);
+                }
+                at_cp_commit();
+                ++pieces;
+                check = (check << 1) | (look ? 1u : 0u);
+                if (pieces - given > (uint32_t)G::DEPTH) {
+                    at_cp_wait<G::DEPTH>();
+                    publish(given, check >> (pieces - 1 - given) & 1);
+                    ++given;
+                }
+            }
+        };
+        // the row numbers (and scales) of key tile kt into stage st
+        auto page_of = [&](uint32_t kt) -> int32_t {
+            const int32_t key = (int32_t)(kt * AT_KEYS + lt);
+            if (!a.pages.k || key < g.t.lo || key >= g.t.hi) return -1;
+            return __ldg(a.table + (uint64_t)g.b * a.table_width + (key >> a.pages.page_shift));
+        };
+        while (walk.next(a, w, g)) {
+            ++seg;
+            int32_t page = g.n ? page_of(g.k0) : -1;
+            uint32_t kst = stage;
+            auto resolve = [&](uint32_t t) {
+                const int32_t key = (int32_t)((g.k0 + t) * AT_KEYS + lt);
+                const bool in = key >= g.t.lo && key < g.t.hi;
+                uint32_t r = AT_NONE;
+                if (in) {
+                    if (a.pages.k) {
+                        const uint64_t slot = ((uint64_t)(uint32_t)page << a.pages.page_shift) +
+                                              ((uint32_t)key & ((1u << a.pages.page_shift) - 1));
+                        if (page < 0 || slot >= a.pages.slots) atomicOr(err, SERVE_ERR_PAGE);
+                        else r = (uint32_t)page_row(a.pages, slot, g.h);
+                    } else {
+                        r = g.s.q0 + (uint32_t)key;
+                    }
+                }
+                if (t + 1 < g.n) page = page_of(g.k0 + t + 1);
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 512 + lt * 4), "r"(r) : "memory");
+                if constexpr (G::Q8) {
+                    float* sc = reinterpret_cast<float*>(sm + G::sc_off) + kst * 384;
+                    float ks = 0.0f, lv = 0.0f, rv = in ? 1.0f : 0.0f;
+                    if (r != AT_NONE) {
+                        ks = a.pages.ks[r] * a.scale_log2;
+                        const float vs = a.pages.vs[r];
+                        lv = log2f(vs);
+                        rv = 1.0f / vs;
+                    }
+                    sc[lt] = ks;
+                    sc[128 + lt] = lv;
+                    sc[256 + lt] = rv;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            };
+            for (uint32_t t = 0; t < (uint32_t)G::LAG && t < g.n; ++t) {
+                resolve(t);
+                for (int c = 0; c < W; ++c) piece(false, c, kst, false);
+                kst = kst + 1 == NSTAGE ? 0 : kst + 1;
+            }
+            for (uint32_t t = 0; t < g.n; ++t) {
+                const bool look = !G::Q8 && at_masked(a, w, g, g.k0 + t);
+                for (int c = 0; c < W; ++c) piece(true, c, stage, look);
+                stage = stage + 1 == NSTAGE ? 0 : stage + 1;
+                if (t + G::LAG < g.n) {
+                    resolve(t + G::LAG);
+                    for (int c = 0; c < W; ++c) piece(false, c, kst, false);
+                    kst = kst + 1 == NSTAGE ? 0 : kst + 1;
+                }
+            }
+            // everything in before the next row tile (seg names it in s_bad)
+            if constexpr (G::Q8) {
+                convert();
+            } else if (g.n) {
+                at_cp_wait<0>();
+                for (; given != pieces; ++given) publish(given, check >> (pieces - 1 - given) & 1);
+            }
+        }
+    } else {
+        if constexpr (NQ == 2) at_regs_down<48>();
+        else at_regs_down<136>();
+        if (warp == NQ * 4 + 4 && lane == 0) {
+            // ------------------------------ products ------------------------------
+            const uint32_t iqk = at_idesc<T>(AT_KEYS, false), ipv = at_idesc<T>(D, true);
+            const uint32_t q0 = smb + G::q_off, ring = smb + G::ring_off;
+            uint32_t kp = 0;              // ring index of the next K piece to multiply, by its order of arrival
+            uint32_t np[2] = {0, 0}, nq = 0;
+            while (walk.next(a, w, g)) {
+                if (!g.n) continue;
+                // pieces arrive K(0) .. K(LAG - 1), V(0), K(LAG), V(1), ..
+                const uint32_t base = kp;
+                auto k_piece = [&](uint32_t t) { return base + (t < (uint32_t)G::LAG ? t * W : (2 * t - G::LAG + 1) * W); };
+                auto v_piece = [&](uint32_t t) {
+                    // V(t) comes after K(0 .. min(n, t + LAG) - 1) and V(0 .. t - 1)
+                    return base + (min(g.n, t + G::LAG) + t) * W;
+                };
+                auto qk = [&](uint32_t t, uint32_t qi, uint32_t buf, bool first, bool last) {
+                    for (int c = 0; c < W; ++c) {
+                        const uint32_t i = k_piece(t) + c, slot = i % NSLOT;
+                        if (first) at_wait(b_full + 8 * slot, (i / NSLOT) & 1, &s_dead, err);
+                        at_fence_after();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            at_mma_ss(tmem + buf * 128, at_desc(q0 + (qi * W + c) * AT_PIECE + k * 32, 16, 1024),
+                                      at_desc(ring + slot * AT_PIECE + k * 32, 16, 1024), iqk, c || k);
+                        if (last) at_commit(b_empty + 8 * slot);
+                    }
+                    at_commit(b_s + 8 * buf);
+                };
+                auto pv = [&](uint32_t t, uint32_t qi, uint32_t buf, bool first, bool last) {
+                    for (int c = 0; c < W; ++c) {
+                        const uint32_t i = v_piece(t) + c, slot = i % NSLOT;
+                        if (first) at_wait(b_full + 8 * slot, (i / NSLOT) & 1, &s_dead, err);
+                        at_fence_after();
+#pragma unroll
+                        for (int k = 0; k < G::VKEYS / 16; ++k)
+                            at_mma_ts(tmem + 256 + qi * D, tmem + buf * 128 + (c * G::VKEYS + k * 16) / 2,
+                                      at_desc(ring + slot * AT_PIECE + k * 2048, G::VKEYS * 128, 1024), ipv, t || c || k);
+                        if (last) at_commit(b_empty + 8 * slot);
+                    }
+                    at_commit(b_o + 8 * qi);
+                };
+                for (int i = 0; i < NQ; ++i) {
+                    at_wait(b_q + 8 * i, nq & 1, &s_dead, err);
+                }
+                ++nq;
+                at_fence_after();
+                if constexpr (NQ == 2) {
+                    qk(0, 0, 0, true, false);
+                    qk(0, 1, 1, false, true);
+                    for (uint32_t t = 0; t < g.n; ++t)
+                        for (uint32_t i = 0; i < 2; ++i) {
+                            at_wait(b_p + 8 * i, np[i]++ & 1, &s_dead, err);
+                            at_fence_after();
+                            pv(t, i, i, i == 0, i == 1);
+                            if (t + 1 < g.n) qk(t + 1, i, i, i == 0, i == 1);
+                        }
+                } else {
+                    qk(0, 0, 0, true, true);
+                    if (g.n > 1) qk(1, 0, 1, true, true);
+                    for (uint32_t t = 0; t < g.n; ++t) {
+                        const uint32_t i = t & 1;
+                        at_wait(b_p + 8 * i, np[i]++ & 1, &s_dead, err);
+                        at_fence_after();
+                        pv(t, 0, i, true, true);
+                        if (t + 2 < g.n) qk(t + 2, 0, i, true, true);
+                    }
+                }
+                kp = base + 2 * g.n * W;
+            }
+        }
+        __syncwarp();
+    }
+    at_fence_before();
+    __syncthreads();
+    if (warp == NQ * 4 + 4) {
+        at_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+// The row tiles that CTAs share: 32 rows of one tile a CTA, the parts added in
+// the order of their keys. blockIdx.x is the CTA that has the tile's first keys.
+template <class T, int W, int ROWS>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ AtWork w,
+                                                        uint32_t ctas) {
+    constexpr int D = 64 * W, NC = D / 32;
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
+    const uint4 head = __ldcg(reinterpret_cast<const uint4*>(w.heads) + 2 * c0 + 1);
+    if (head.x != AT_FIRST) return;
+    uint32_t parts = 0;  // that follow the first
+    for (uint32_t j = c0 + 1; j < ctas; j += 32) {
+        const uint32_t kind = j + lane < ctas ? __ldcg(w.heads + (size_t)(2 * (j + lane)) * 4) : (uint32_t)AT_LAST;
+        const uint32_t last = __ballot_sync(0xffffffffu, kind == AT_LAST);
+        parts += last ? __ffs(last) : 32;
+        if (last) break;
+    }
+    const uint32_t row = blockIdx.y * 32 + lane;
+    auto part = [&](uint32_t i) { return w.slots + (size_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * w.slot_bytes; };
+    float m = -INFINITY;
+    for (uint32_t i = 0; i <= parts; ++i) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(part(i) + (size_t)ROWS * D * 4) + row);
+        if (v.y != 0.0f) m = fmaxf(m, v.x);
+    }
+    float l = 0.0f;
+    float4 o[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+    for (uint32_t i = 0; i <= parts; ++i) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(part(i) + (size_t)ROWS * D * 4) + row);
+        const float4* p = reinterpret_cast<const float4*>(part(i)) + (size_t)warp * NC * ROWS + row;
+        float4 x[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) x[c] = __ldcg(p + (size_t)c * ROWS);
+        if (v.y == 0.0f) continue;
+        const float f = at_ex2(v.x - m);
+        l += f * v.y;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            o[c].x += f * x[c].x;
+            o[c].y += f * x[c].y;
+            o[c].z += f * x[c].z;
+            o[c].w += f * x[c].w;
+        }
+    }
+    const Seq s = seq_of(a, head.y);
+    const uint32_t r = row & 127, rt = r / a.group, rg = r - rt * a.group;
+    const uint32_t tok = head.w * w.tile_tokens + (row >> 7) * w.sub_tokens + rt;
+    if (rt >= w.sub_tokens || tok >= s.nq) return;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const uint64_t orow = s.q0 + tok, ohead = head.z * a.group + rg;
+    T* op = static_cast<T*>(a.out.data) + (int64_t)orow * a.out.ts + (int64_t)ohead * a.out.hs + warp * NC * 4;
+#pragma unroll
+    for (int c = 0; c < NC; c += 2) {
+        uint4 y;
+        y.x = at_pack<T>(o[c].x * inv, o[c].y * inv);
+        y.y = at_pack<T>(o[c].z * inv, o[c].w * inv);
+        y.z = at_pack<T>(o[c + 1].x * inv, o[c + 1].y * inv);
+        y.w = at_pack<T>(o[c + 1].z * inv, o[c + 1].w * inv);
+        *reinterpret_cast<uint4*>(op + c * 4) = y;
+    }
+    if (a.lse && warp == 0)
+        a.lse[orow * a.heads + ohead] = l != 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+}  // namespace xp
