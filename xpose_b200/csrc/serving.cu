@@ -1,5 +1,9 @@
 // Serving entry points of libxp_cuda.so: rotary rows, the paged cache and its
 // attentions. A translation unit of its own, built beside xp_cuda.cu.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
 #include <cmath>
 
 #include "host.cuh"
@@ -77,6 +81,33 @@ PagesArg pages_arg(const xp_pages* p) {
 }
 
 // Calls f with a value of the type (and the W = dim / 64) that was asked for.
+// The driver's tensor map encoder (the library does not link libcuda).
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 f = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return f;
+}
+// 16-bit rows as boxes of 64 values x `rows` rows, 128-byte swizzled.
+// Packed: [tokens][heads][dim], rows along tokens; paged: [pages * heads][page][dim].
+xp_status row_map(const char* who, CUtensorMap* m, bool is_bf16, void* data, uint64_t dim, const uint64_t (&n)[2],
+                  const uint64_t (&stride)[2], const uint32_t (&box)[2]) {
+    const auto encode = map_encoder();
+    if (!encode) return fail(XP_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available", who);
+    const cuuint64_t dims[3] = {dim, n[0], n[1]}, strides[2] = {stride[0], stride[1]};
+    const cuuint32_t boxes[3] = {64, box[0], box[1]}, ones[3] = {1, 1, 1};
+    const CUresult r = encode(m, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, data,
+                              dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(XP_ERR_INVALID, "%s: the rows do not fit a tensor map (%d)", who, (int)r);
+    return XP_OK;
+}
+
 template <class T, class C, int W>
 xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, cudaStream_t st) {
     using G = AtCfg<T, C, W>;
@@ -97,7 +128,32 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
     w.tile_tokens = w.sub_tokens * G::NQ;
     w.least_units = 2;
     w.split_over = 3;
-    cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, false, a, w);
+    CUtensorMap km{}, vm{};
+    if constexpr (!G::Q8) {
+        const bool b = std::is_same_v<T, bf16>;
+        if (a.pages.k) {
+            const uint32_t ps = 1u << a.pages.page_shift;
+            const uint64_t n[2] = {ps, (a.pages.slots >> a.pages.page_shift) * a.kv_heads};
+            const uint64_t stride[2] = {G::D * 2, (uint64_t)ps * G::D * 2};
+            const uint32_t kbox[2] = {std::min<uint32_t>(ps, AT_KEYS), 1}, vbox[2] = {std::min<uint32_t>(ps, G::VKEYS), 1};
+            TRY(row_map(who, &km, b, a.pages.k, G::D, n, stride, kbox));
+            TRY(row_map(who, &vm, b, a.pages.v, G::D, n, stride, vbox));
+        } else {
+            // a lone head or token has no stride of its own; one head for all (stride 0) is a lone head
+            w.head_step = 1;
+            const uint32_t heads = a.kv_heads;
+            for (const RowsArg* r : {&a.k, &a.v})
+                if (heads > 1 && r->hs == 0) w.head_step = 0;
+            const uint32_t mh = w.head_step ? heads : 1;
+            const uint64_t n[2] = {mh, a.tokens};
+            const uint32_t kbox[2] = {1, AT_KEYS}, vbox[2] = {1, G::VKEYS};
+            const uint64_t ks[2] = {mh > 1 ? (uint64_t)a.k.hs * 2 : G::D * 2, a.tokens > 1 ? (uint64_t)a.k.ts * 2 : G::D * 2};
+            const uint64_t vs[2] = {mh > 1 ? (uint64_t)a.v.hs * 2 : G::D * 2, a.tokens > 1 ? (uint64_t)a.v.ts * 2 : G::D * 2};
+            TRY(row_map(who, &km, b, a.k.data, G::D, n, ks, kbox));
+            TRY(row_map(who, &vm, b, a.v.data, G::D, n, vs, vbox));
+        }
+    }
+    cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, false, a, w, km, vm);
     if (e == cudaSuccess)
         e = launch_ex(attn_join_kernel<T, W, G::ROWS>, dim3(ctas, G::ROWS / 32), dim3(256), 0, st, 1, true, a, w, ctas);
     if (e != cudaSuccess) return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
@@ -268,6 +324,11 @@ xp_status attention(const char* who, void* stream, const xp_rows* out, const xp_
     } else {
         TRY(check_rows(who, "k", k, 8));
         TRY(check_rows(who, "v", v, 8));
+        for (const xp_rows* r : {k, v})
+            REQUIRE(r->token_stride >= 0 && r->head_stride >= 0 && (r->token_stride > 0 || r->tokens <= 1),
+                    "%s: 'k' and 'v' need strides that are not negative, and a token stride", who);
+        REQUIRE((k->head_stride == 0) == (v->head_stride == 0) || k->heads <= 1,
+                "%s: one of 'k' and 'v' has one head for all, the other not", who);
         REQUIRE(same_shape(k, v) && k->tokens == q->tokens && k->dim == q->dim && k->dtype == q->dtype,
                 "%s: 'q', 'k' and 'v' differ in shape or type", who);
         kv_heads = k->heads;

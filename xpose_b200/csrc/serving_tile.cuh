@@ -18,20 +18,25 @@
 //
 // K and V move in 16 KB pieces through one ring (K: 128 keys x 64 dims, V:
 // 8192 / dim keys x dim), so a ring slot is free again as soon as its piece
-// is multiplied. Loader threads copy rows of 16 bytes (cp.async) into the
-// 128-byte swizzled layouts of the tensor core: the rows of a paged cache sit
-// anywhere, and keys outside the tile's range become zeros on the way, so
-// that nothing of a stale page is ever multiplied. 8-bit codes are turned
-// into exact 16-bit values by the loader; their scales never touch them: with
-// t_ij = s_ij ks_j + log2 vs_j the weight that multiplies v's code is 2^(t -
-// m), and l adds 2^(t - m) / vs_j. A weight is then rounded relative to the
-// largest contribution, whatever the scales.
+// is multiplied. 16-bit rows come by TMA, a box a page, straight into the
+// 128-byte swizzled layouts of the tensor core; a page that a tile must not
+// touch is read past the end of the tensor, which gives zeros. What a tile's
+// last page or the next sequence holds past the tile's keys must not be
+// multiplied even by 0 (it may be NaN): in the few V tiles where some row does
+// not see some key, loader threads put zeros there, and take infinities and
+// NaN of v out; those go to the rows that do see them at the end. 8-bit codes
+// are turned into exact 16-bit values by the loader threads; their scales
+// never touch them: with t_ij = s_ij ks_j + log2 vs_j the weight that
+// multiplies v's code is 2^(t - m), and l adds 2^(t - m) / vs_j. A weight is
+// then rounded relative to the largest contribution, whatever the scales.
 //
 // Work is split evenly: every CTA takes the same number of (row tile, key
 // tile) units, so the last tile of a call does not run alone. A row tile that
 // two or more CTAs share leaves partial sums (O, m, l) that a second, small
 // launch joins in a fixed order.
 #pragma once
+#include <cuda.h>
+
 #include "serving_attn.cuh"
 #include "tk_primitives.cuh"
 
@@ -56,29 +61,26 @@ template <class T, class C, int W> struct AtCfg {
     static constexpr int VKEYS = AT_KEYS / W;     // keys of a V piece
     static constexpr int NSTAGE = W == 1 ? 8 : 4; // tiles whose row numbers and scales are kept
     static constexpr int THREADS = 128 * NQ + 256;
-    // pieces issued and not yet given to the tensor core. With two row tiles a
-    // slot is free only once the rest of its tile and the next K are in too.
-    static constexpr int DEPTH = Q8 ? 1 : W == 4 ? 6 : 5;
-    static_assert(DEPTH + (NQ == 2 ? 2 * W : 1) <= NSLOT, "the loader would wait for itself");
     // shared memory
     static constexpr int q_off = 0;
     static constexpr int ring_off = NQ * W * AT_PIECE;
-    static constexpr int row_off = ring_off + NSLOT * AT_PIECE;       // [NSTAGE][128] row numbers
-    static constexpr int sc_off = row_off + NSTAGE * 512;             // [NSTAGE][3][128] floats, 8-bit pages
+    static constexpr int row_off = ring_off + NSLOT * AT_PIECE;       // [NSTAGE][128] row numbers, 8-bit pages
+    static constexpr int sc_off = row_off + (Q8 ? NSTAGE * 512 : 0);  // [NSTAGE][3][128] floats, 8-bit pages
     static constexpr int bar_off = sc_off + (Q8 ? NSTAGE * 1536 : 0);
-    static constexpr int smem = bar_off + 512;                        // barriers, plan, sums, flags
+    static constexpr int smem = bar_off + 1024;                       // barriers, plan, row tiles, flags
 };
 
 struct AtWork {
     unsigned char* slots;   // partial sums: two of slot_bytes a CTA
     uint32_t* heads;        // [2 * CTAs][4]: kind, b, h, tile of each
     uint32_t slot_bytes;
+    uint32_t head_step;     // packed: k and v heads a kv head apart in the tensor maps (0: one for all)
     uint32_t tile_tokens;   // tokens of a tile
     uint32_t sub_tokens;    // tokens of one of its NQ row tiles
     uint32_t least_units;   // units of a CTA, at least
     uint32_t split_over;    // split tiles when the largest has this many units more than an even share
 };
-enum : uint32_t { AT_FULL = 0, AT_FIRST = 1, AT_MIDDLE = 2, AT_LAST = 3 };
+enum : uint32_t { AT_FULL = 0, AT_FIRST = 1, AT_MIDDLE = 2, AT_LAST = 3, AT_END = 4 };
 
 // ---- tcgen05 ------------------------------------------------------------------
 XP_DEV uint64_t at_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
@@ -151,6 +153,10 @@ XP_DEV void at_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint
         }
     }
 }
+// ... and after such a failure: for what is still on its way, whatever `dead` says
+XP_DEV void at_wait_flight(uint32_t bar, uint32_t parity) {
+    for (uint32_t it = 0; it < AT_SPIN_LIMIT && !at_try(bar, parity); ++it) {}
+}
 XP_DEV void at_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -215,12 +221,6 @@ template <class T> XP_DEV uint2 at_codes(uint32_t w, fp8c) {
     }
     return make_uint2(a, b);
 }
-XP_DEV void at_cp16(uint32_t dst, const void* src, bool has) {
-    const uint32_t n = has ? 16u : 0u;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-template <int N> XP_DEV void at_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-XP_DEV void at_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 XP_DEV uint32_t at_lds(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -364,11 +364,13 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
     __syncthreads();
 }
 
-// The pieces of a CTA's range, one row tile each: every role walks the same list.
+// The part of a row tile that a CTA computes. One warp walks the CTA's range
+// and hands these to the others through shared memory.
 struct AtSeg {
     uint32_t h, b, x, kind;
     Seq s;
-    AtTile t;
+    int32_t lo, hi;     // the tile's keys
+    int32_t p0;         // position of its first token
     uint32_t k0, n;     // first key tile (in keys / 128) and how many
 };
 struct AtWalk {
@@ -394,12 +396,15 @@ struct AtWalk {
         g.b = p.b;
         g.x = p.x;
         g.s = s;
-        g.t = at_tile(s, p.x, w.tile_tokens, a.window);
-        const uint32_t n = max(g.t.n, 1u);
+        const AtTile t = at_tile(s, p.x, w.tile_tokens, a.window);
+        g.lo = t.lo;
+        g.hi = t.hi;
+        g.p0 = (int32_t)s.nkv - (int32_t)s.nq + (int32_t)(p.x * w.tile_tokens);
+        const uint32_t n = max(t.n, 1u);
         const uint32_t take = p.split ? (uint32_t)min((int64_t)(n - p.skip), p.todo) : n;
         g.kind = p.skip == 0 ? (take == n ? AT_FULL : AT_FIRST) : (p.skip + take == n ? AT_LAST : AT_MIDDLE);
-        g.k0 = g.t.t0 + p.skip;
-        g.n = g.t.n ? take : 0;
+        g.k0 = t.t0 + p.skip;
+        g.n = t.n ? take : 0;
         p.todo -= take;
         p.skip = 0;
         ++p.x;
@@ -407,12 +412,11 @@ struct AtWalk {
     }
 };
 
-// Some row of the tile does not see some key of key tile kt that is loaded.
-XP_DEV bool at_masked(const ServeAttnArgs& a, const AtWork& w, const AtSeg& g, uint32_t kt) {
-    const int64_t p0 = (int64_t)g.s.nkv - g.s.nq + (int64_t)g.x * w.tile_tokens;
-    const int64_t p1 = (int64_t)g.t.hi - 1;
-    const int64_t k0 = max((int64_t)kt * AT_KEYS, (int64_t)g.t.lo), k1 = min((int64_t)(kt + 1) * AT_KEYS, (int64_t)g.t.hi);
-    return k1 > p0 + 1 || (a.window && k0 < p1 - (int64_t)a.window + 1);
+// V of key tile kt needs a look: a loaded row lies outside the tile's keys, or
+// some row of the tile does not see some key.
+XP_DEV bool at_look(const ServeAttnArgs& a, int32_t lo, int32_t hi, int32_t p0, uint32_t kt) {
+    const int64_t k0 = (int64_t)kt * AT_KEYS, k1 = k0 + AT_KEYS;
+    return k0 < lo || k1 > hi || k1 > (int64_t)p0 + 1 || (a.window && k0 < (int64_t)hi - (int64_t)a.window);
 }
 XP_DEV bool at_odd16(uint32_t w, uint32_t exp_mask) {  // an infinity or NaN in either half
     return (w & exp_mask) == exp_mask || (w & (exp_mask << 16)) == (exp_mask << 16);
@@ -420,26 +424,38 @@ XP_DEV bool at_odd16(uint32_t w, uint32_t exp_mask) {  // an infinity or NaN in 
 
 template <class T, class C, int W>
 __global__ void __launch_bounds__(AtCfg<T, C, W>::THREADS, 1)
-attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ AtWork w) {
+attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ AtWork w,
+                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using G = AtCfg<T, C, W>;
     constexpr int D = G::D, NQ = G::NQ, NSLOT = G::NSLOT, NSTAGE = G::NSTAGE;
     // no static shared memory: the dynamic part then starts on a 1 KB boundary,
     // which the swizzled layouts need, without a byte lost
     extern __shared__ __align__(1024) unsigned char sm[];
     const uint32_t smb = smem_u32(sm);
+    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 9 + 2 * NSEG;
     struct Small {
         AtPlan plan;
+        AtSeg segs[NSEG];
         uint32_t sums[32], bad[4], tmem, dead;
     };
-    static_assert((2 * NSLOT + 8) * 8 + sizeof(Small) <= 512, "small data");
-    Small& small = *reinterpret_cast<Small*>(sm + G::bar_off + (2 * NSLOT + 8) * 8);
+    static_assert(NBAR * 8 + sizeof(Small) <= 1024 && NBAR * 8 % 8 == 0, "small data");
+    Small& small = *reinterpret_cast<Small*>(sm + G::bar_off + NBAR * 8);
     AtPlan& s_plan = small.plan;
     uint32_t *const s_sums = small.sums, *const s_bad = small.bad;
     volatile uint32_t& s_dead = small.dead;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // barriers
-    const uint32_t b_full = smb + G::bar_off, b_empty = b_full + NSLOT * 8, b_q = b_empty + NSLOT * 8;
-    const uint32_t b_s = b_q + 16, b_p = b_s + 16, b_o = b_p + 16;
+    const uint32_t b_full = smb + G::bar_off;       // [NSLOT] a piece is in
+    const uint32_t b_empty = b_full + NSLOT * 8;    // [NSLOT] ... multiplied
+    // a piece that needs a look arrives on its own ring, in order: no wait of
+    // the threads that look may skip a phase of its barrier
+    const uint32_t b_raw = b_empty + NSLOT * 8;     // [NSLOT] a V piece to look over is in
+    const uint32_t b_clean = b_raw + NSLOT * 8;     // [NSLOT] ... looked over
+    const uint32_t b_q = b_clean + NSLOT * 8;       // [NQ] Q is in
+    const uint32_t b_s = b_q + 16, b_p = b_s + 16;  // [2] S made, P made (by S buffer)
+    const uint32_t b_o = b_p + 16;                  // [NQ] P V added
+    const uint32_t b_seg = b_o + 16, b_free = b_seg + NSEG * 8;  // [NSEG] a row tile given, done with
+    const uint32_t b_end = b_free + NSEG * 8;       // products in flight after a failed wait
 
     if (smb & 1023) {  // cannot be multiplied from
         if (tid == 0) atomicOr(a.err, SERVE_ERR_WAIT);
@@ -448,15 +464,23 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     if (tid == 0) {
         uint64_t* m = reinterpret_cast<uint64_t*>(sm + G::bar_off);
         for (int i = 0; i < NSLOT; ++i) {
-            mbar_init(m + i, 4);
+            mbar_init(m + i, G::Q8 ? 4 : 1);
             mbar_init(m + NSLOT + i, 1);
+            mbar_init(m + 2 * NSLOT + i, 1);
+            mbar_init(m + 3 * NSLOT + i, 4);
         }
+        m += 4 * NSLOT;
         for (int i = 0; i < 2; ++i) {
-            mbar_init(m + 2 * NSLOT + i, 4);
-            mbar_init(m + 2 * NSLOT + 2 + i, 1);
-            mbar_init(m + 2 * NSLOT + 4 + i, 4);
-            mbar_init(m + 2 * NSLOT + 6 + i, 1);
+            mbar_init(m + i, 4);
+            mbar_init(m + 2 + i, 1);
+            mbar_init(m + 4 + i, 4);
+            mbar_init(m + 6 + i, 1);
         }
+        for (int i = 0; i < NSEG; ++i) {
+            mbar_init(m + 8 + i, 1);
+            mbar_init(m + 8 + NSEG + i, NQ * 4 + 4 + 1 + (G::Q8 ? 0 : 1));
+        }
+        mbar_init(m + 8 + 2 * NSEG, 1);
         fence_mbar_init();
         s_dead = 0;
         for (int i = 0; i < 4; ++i) s_bad[i] = 0;
@@ -486,14 +510,22 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     at_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = small.tmem;
-    AtWalk walk;
-    walk.start(s_plan);
-    AtSeg g;
     uint32_t* const err = a.err;
+    // the next row tile of this CTA: given to every role in turn
+    uint32_t seg = 0;
+    auto take = [&]() -> const AtSeg& {
+        at_wait(b_seg + 8 * (seg % NSEG), (seg / NSEG) & 1, &s_dead, err);
+        return small.segs[seg % NSEG];
+    };
+    auto done = [&]() {
+        __syncwarp();
+        if (lane == 0) at_arrive(b_free + 8 * (seg % NSEG));
+        ++seg;
+    };
 
     if (warp < NQ * 4) {
         // ------------------------------ softmax ------------------------------
-        if constexpr (NQ == 2) at_regs_up<192>();
+        if constexpr (NQ == 2) at_regs_up<184>();
         else at_regs_up<232>();
         const uint32_t wg = warp >> 2, row = tid & 127;
         const uint32_t lanes = (warp & 3) * 32 << 16;
@@ -503,9 +535,11 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             w.heads[(2 * blockIdx.x + 1) * 4] = AT_FULL;
         }
         const uint32_t qrow0 = wg * w.sub_tokens;  // first token of this row tile in its CTA's tile
-        uint32_t stage = 0, nsfull[2] = {0, 0}, npv = 0, seg = 0;
-        while (walk.next(a, w, g)) {
-            ++seg;
+        uint32_t stage = 0, s_phase = 0, npv = 0;  // s_phase: a bit for each S buffer
+        for (;; done()) {
+            const AtSeg& g = take();
+            if (g.kind == AT_END || s_dead) break;
+            const uint32_t n = g.n, kfirst = g.k0;
             // this thread's row
             const uint32_t rt = row / a.group, rg = row - rt * a.group;
             const uint32_t tok = g.x * w.tile_tokens + qrow0 + rt;
@@ -547,10 +581,11 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             float m = -INFINITY, ref = 0.0f;
             float2 l2[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
 #pragma unroll 1
-            for (uint32_t t = 0; t < g.n; ++t) {
+            for (uint32_t t = 0; t < n; ++t) {
                 const uint32_t buf = NQ == 2 ? wg : (t & 1);
                 const uint32_t s_tm = tmem + lanes + buf * 128;
-                at_wait(b_s + 8 * buf, nsfull[NQ == 2 ? 0 : buf]++ & 1, &s_dead, err);
+                at_wait(b_s + 8 * buf, s_phase >> buf & 1, &s_dead, err);
+                s_phase ^= 1u << buf;
                 at_fence_after();
                 float s[128];
                 {
@@ -575,7 +610,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         s[j + 3] = y.y;
                     }
                 }
-                const int32_t kt = (int32_t)((g.k0 + t) * AT_KEYS);
+                const int32_t kt = (int32_t)((kfirst + t) * AT_KEYS);
                 if (__any_sync(0xffffffffu, kt < klo || khi - kt < AT_KEYS)) {
                     const uint32_t off = (uint32_t)(kt - klo), span = (uint32_t)(khi > klo ? khi - klo : 0);
 #pragma unroll
@@ -659,7 +694,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 at_wait(b_o + 8 * wg, (npv - 1) & 1, &s_dead, err);
                 at_fence_after();
             }
-            const bool bad = !G::Q8 && *reinterpret_cast<volatile uint32_t*>(&s_bad[seg & 3]) == seg;
+            const bool bad = !G::Q8 && *reinterpret_cast<volatile uint32_t*>(&s_bad[seg & 3]) == seg + 1;
             const bool whole = g.kind == AT_FULL;
             const float inv = l != 0.0f ? 1.0f / l : 0.0f;   // l is 0 where the row saw nothing
             const uint32_t slot = 2 * blockIdx.x + (g.kind == AT_FIRST ? 1 : 0);
@@ -680,9 +715,9 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     // infinities and NaN of v were left out of the products of tiles
                     // where not every row sees every key: they go to the rows that do
                     for (uint32_t t = 0; t < g.n; ++t) {
-                        if (!at_masked(a, w, g, g.k0 + t)) continue;
+                        if (!at_look(a, g.lo, g.hi, g.p0, g.k0 + t)) continue;
                         const int32_t j0 = max((int32_t)((g.k0 + t) * AT_KEYS), klo);
-                        const int32_t j1 = min(min((int32_t)((g.k0 + t + 1) * AT_KEYS), khi), g.t.hi);
+                        const int32_t j1 = min(min((int32_t)((g.k0 + t + 1) * AT_KEYS), khi), g.hi);
                         for (int32_t j = j0; j < j1; ++j) {
                             const T* vp;
                             if (a.pages.k) {
@@ -734,144 +769,132 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
         if constexpr (NQ == 2) at_regs_down<80>();
         else at_regs_down<136>();
         const uint32_t lt = tid - NQ * 128;
-        uint32_t pieces = 0, given = 0;  // pieces issued, and given to the tensor core
-        uint32_t check = 0;              // bit i: the piece issued i before the last is of a V tile to be looked over
-        uint32_t stage = 0, seg = 0;
-        uint4 raw[4];                 // 8-bit: the codes of the piece issued last
-        uint32_t raw_kind = 0;        // ... 0 none, 1 K, 2 V
-        const uint32_t rows0 = smb + G::row_off;
-        // thread -> 16-byte units of a piece: unit u of rows r0, r0 + step, ..
-        constexpr int KU = G::Q8 ? 4 : 8, VU = (G::Q8 ? 4 : 8) * W, NU = G::Q8 ? 4 : 8;
-        // where unit u of key r of a V piece goes: blocks of 64 dims, keys in rows of 128 bytes
-        auto v_at = [&](uint32_t r, uint32_t c) { return (c >> 3) * (G::VKEYS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+        // where 16 bytes c of row r of a piece go: rows of 128 bytes, swizzled;
+        // a V piece has a block of rows for every 64 dims
         auto k_at = [&](uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); };
-
-        // a piece is in: give it to the tensor core
-        auto publish = [&](uint32_t index, bool look) {
-            const uint32_t slot = index % NSLOT, base = smb + G::ring_off + slot * AT_PIECE;
-            if (!G::Q8 && look) {
-                constexpr uint32_t mask = std::is_same_v<T, bf16> ? 0x7F80u : 0x7C00u;
-                bool odd = false;
+        auto v_at = [&](uint32_t r, uint32_t c) { return (c >> 3) * (G::VKEYS * 128) + k_at(r, c & 7); };
+        if constexpr (!G::Q8) {
+            // 16-bit pieces come by TMA: only V tiles that need a look pass here
+            uint32_t before = 0, cleaned = 0;  // pieces of the row tiles before this one, pieces looked over
+            for (;; done()) {
+                const AtSeg& g = take();
+                if (g.kind == AT_END || s_dead) break;
+                const int32_t lo = g.lo, hi = g.hi, p0 = g.p0;
+                const uint32_t n = g.n, k0 = g.k0;
+                for (uint32_t t = 0; t < n; ++t) {
+                    if (!at_look(a, lo, hi, p0, k0 + t)) continue;
+                    for (int c = 0; c < W; ++c) {
+                        const uint32_t i = before + (min(n, t + G::LAG) + t) * W + c, slot = i % NSLOT;
+                        at_wait(b_raw + 8 * (cleaned % NSLOT), (cleaned / NSLOT) & 1, &s_dead, err);
+                        const uint32_t base = smb + G::ring_off + slot * AT_PIECE;
+                        constexpr uint32_t mask = std::is_same_v<T, bf16> ? 0x7F80u : 0x7C00u, VU = 8 * W;
+                        bool odd = false;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t r = lt / VU + i * (128 / VU), c = lt % VU, at = base + v_at(r, c);
-                    uint4 v = at_lds16(at);
-                    if (at_odd16(v.x, mask) || at_odd16(v.y, mask) || at_odd16(v.z, mask) || at_odd16(v.w, mask)) {
-                        odd = true;
-                        uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-                        for (int j = 0; j < 4; ++j) {
-                            if ((x[j] & mask) == mask) x[j] &= 0xFFFF0000u;
-                            if ((x[j] & (mask << 16)) == (mask << 16)) x[j] &= 0xFFFFu;
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t r = lt / VU + j * (128 / VU), at = base + v_at(r, lt % VU);
+                            const int32_t key = (int32_t)((k0 + t) * AT_KEYS + c * G::VKEYS + r);
+                            if (key < lo || key >= hi) {
+                                at_sts16(at, make_uint4(0, 0, 0, 0));
+                                continue;
+                            }
+                            uint4 v = at_lds16(at);
+                            if (at_odd16(v.x, mask) || at_odd16(v.y, mask) || at_odd16(v.z, mask) || at_odd16(v.w, mask)) {
+                                odd = true;
+                                uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    if ((x[q] & mask) == mask) x[q] &= 0xFFFF0000u;
+                                    if ((x[q] & (mask << 16)) == (mask << 16)) x[q] &= 0xFFFFu;
+                                }
+                                at_sts16(at, make_uint4(x[0], x[1], x[2], x[3]));
+                            }
                         }
-                        at_sts16(at, v);
+                        if (odd) s_bad[seg & 3] = seg + 1;
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) at_arrive(b_clean + 8 * (cleaned % NSLOT));
+                        ++cleaned;
                     }
                 }
-                if (odd) s_bad[seg & 3] = seg;
+                before += 2 * n * W;
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) at_arrive(b_full + 8 * slot);
-        };
-        // 8-bit: the codes in `raw` into their slot, as 16-bit values
-        auto convert = [&]() {
-            if constexpr (G::Q8) {
-            if (raw_kind == 0) return;
-            const uint32_t index = pieces - 1, slot = index % NSLOT, base = smb + G::ring_off + slot * AT_PIECE;
-            if (index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
+        } else {
+            uint32_t pieces = 0, stage = 0;
+            uint4 raw[4];                 // the codes of the piece issued last
+            uint32_t raw_kind = 0;        // ... 0 none, 1 K, 2 V
+            const uint32_t rows0 = smb + G::row_off;
+            // thread -> 16 codes: unit u of rows r0, r0 + step, ..
+            constexpr int KU = 4, VU = 4 * W;
+            // the codes in `raw` into their slot, as 16-bit values
+            auto convert = [&]() {
+                if (raw_kind == 0) return;
+                const uint32_t index = pieces - 1, slot = index % NSLOT, base = smb + G::ring_off + slot * AT_PIECE;
+                if (index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint2 x0 = at_codes<T>(raw[i].x, C{}), x1 = at_codes<T>(raw[i].y, C{});
-                const uint2 x2 = at_codes<T>(raw[i].z, C{}), x3 = at_codes<T>(raw[i].w, C{});
-                uint32_t d0, d1;
-                if (raw_kind == 1) {
-                    const uint32_t r = lt / KU + i * (128 / KU), c = 2 * (lt % KU);
-                    d0 = k_at(r, c);
-                    d1 = k_at(r, c + 1);
-                } else {
-                    const uint32_t r = lt / VU + i * (128 / VU), c = 2 * (lt % VU);
-                    d0 = v_at(r, c);
-                    d1 = v_at(r, c + 1);
+                for (int i = 0; i < 4; ++i) {
+                    const uint2 x0 = at_codes<T>(raw[i].x, C{}), x1 = at_codes<T>(raw[i].y, C{});
+                    const uint2 x2 = at_codes<T>(raw[i].z, C{}), x3 = at_codes<T>(raw[i].w, C{});
+                    uint32_t d0, d1;
+                    if (raw_kind == 1) {
+                        const uint32_t r = lt / KU + i * (128 / KU), c = 2 * (lt % KU);
+                        d0 = k_at(r, c);
+                        d1 = k_at(r, c + 1);
+                    } else {
+                        const uint32_t r = lt / VU + i * (128 / VU), c = 2 * (lt % VU);
+                        d0 = v_at(r, c);
+                        d1 = v_at(r, c + 1);
+                    }
+                    at_sts16(base + d0, make_uint4(x0.x, x0.y, x1.x, x1.y));
+                    at_sts16(base + d1, make_uint4(x2.x, x2.y, x3.x, x3.y));
                 }
-                at_sts16(base + d0, make_uint4(x0.x, x0.y, x1.x, x1.y));
-                at_sts16(base + d1, make_uint4(x2.x, x2.y, x3.x, x3.y));
-            }
-            publish(index, false);
-            raw_kind = 0;
-            }
-        };
-        auto piece = [&](bool is_v, uint32_t c, uint32_t st, bool look) {
-            const uint32_t u = is_v ? lt % VU : lt % KU, r0 = is_v ? lt / VU : lt / KU;
-            const uint32_t step = is_v ? 128 / VU : 128 / KU, key0 = is_v ? c * G::VKEYS : 0;
-            const uint32_t d = (is_v ? u : c * KU + u) * (G::Q8 ? 16 : 8);
-            const C* src;
-            int64_t stride;
-            if (a.pages.k) {
-                src = static_cast<const C*>(is_v ? a.pages.v : a.pages.k) + d;
-                stride = D;
-            } else {
-                const RowsArg& x = is_v ? a.v : a.k;
-                src = static_cast<const C*>(x.data) + (int64_t)g.h * x.hs + d;
-                stride = x.ts;
-            }
-            if constexpr (G::Q8) {
-                uint4 now[4];
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) at_arrive(b_full + 8 * slot);
+                raw_kind = 0;
+            };
+            for (;; done()) {
+                const AtSeg& g = take();
+                if (g.kind == AT_END || s_dead) break;
+                const int32_t lo = g.lo, hi = g.hi;
+                const uint32_t n = g.n, k0 = g.k0, head = g.h;
+                const int32_t* const table = a.table + (uint64_t)g.b * a.table_width;
+                auto piece = [&](bool is_v, uint32_t c, uint32_t st) {
+                    const uint32_t u = is_v ? lt % VU : lt % KU, r0 = is_v ? lt / VU : lt / KU;
+                    const uint32_t step = is_v ? 128 / VU : 128 / KU, key0 = is_v ? c * G::VKEYS : 0;
+                    const uint32_t d = (is_v ? u : c * KU + u) * 16;
+                    const C* src = static_cast<const C*>(is_v ? a.pages.v : a.pages.k) + d;
+                    uint4 now[4];
 #pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    const uint32_t r = at_lds(rows0 + st * 512 + (key0 + r0 + i * step) * 4);
-                    now[i] = make_uint4(0, 0, 0, 0);
-                    if (r != AT_NONE) now[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * stride));
-                }
-                convert();
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t r = at_lds(rows0 + st * 512 + (key0 + r0 + i * step) * 4);
+                        now[i] = make_uint4(0, 0, 0, 0);
+                        if (r != AT_NONE) now[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
+                    }
+                    convert();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) raw[i] = now[i];
-                raw_kind = is_v ? 2 : 1;
-                ++pieces;
-            } else {
-                const uint32_t slot = pieces % NSLOT, base = smb + G::ring_off + slot * AT_PIECE;
-                if (pieces >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (pieces / NSLOT - 1) & 1, &s_dead, err);
-#pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    const uint32_t rr = r0 + i * step, r = at_lds(rows0 + st * 512 + (key0 + rr) * 4);
-                    const bool has = r != AT_NONE;
-                    at_cp16(base + (is_v ? v_at(rr, u) : k_at(rr, u)), src + (has ? (int64_t)r * stride : 0), has);
-                }
-                at_cp_commit();
-                ++pieces;
-                check = (check << 1) | (look ? 1u : 0u);
-                if (pieces - given > (uint32_t)G::DEPTH) {
-                    at_cp_wait<G::DEPTH>();
-                    publish(given, check >> (pieces - 1 - given) & 1);
-                    ++given;
-                }
-            }
-        };
-        // the row numbers (and scales) of key tile kt into stage st
-        auto page_of = [&](uint32_t kt) -> int32_t {
-            const int32_t key = (int32_t)(kt * AT_KEYS + lt);
-            if (!a.pages.k || key < g.t.lo || key >= g.t.hi) return -1;
-            return __ldg(a.table + (uint64_t)g.b * a.table_width + (key >> a.pages.page_shift));
-        };
-        while (walk.next(a, w, g)) {
-            ++seg;
-            int32_t page = g.n ? page_of(g.k0) : -1;
-            uint32_t kst = stage;
-            auto resolve = [&](uint32_t t) {
-                const int32_t key = (int32_t)((g.k0 + t) * AT_KEYS + lt);
-                const bool in = key >= g.t.lo && key < g.t.hi;
-                uint32_t r = AT_NONE;
-                if (in) {
-                    if (a.pages.k) {
+                    for (int i = 0; i < 4; ++i) raw[i] = now[i];
+                    raw_kind = is_v ? 2 : 1;
+                    ++pieces;
+                };
+                auto page_of = [&](uint32_t kt) -> int32_t {
+                    const int32_t key = (int32_t)(kt * AT_KEYS + lt);
+                    return key < lo || key >= hi ? -1 : __ldg(table + (key >> a.pages.page_shift));
+                };
+                int32_t page = n ? page_of(k0) : -1;
+                uint32_t kst = stage;
+                // the row numbers and scales of key tile t into stage kst
+                auto resolve = [&](uint32_t t) {
+                    const int32_t key = (int32_t)((k0 + t) * AT_KEYS + lt);
+                    const bool in = key >= lo && key < hi;
+                    uint32_t r = AT_NONE;
+                    if (in) {
                         const uint64_t slot = ((uint64_t)(uint32_t)page << a.pages.page_shift) +
                                               ((uint32_t)key & ((1u << a.pages.page_shift) - 1));
                         if (page < 0 || slot >= a.pages.slots) atomicOr(err, SERVE_ERR_PAGE);
-                        else r = (uint32_t)page_row(a.pages, slot, g.h);
-                    } else {
-                        r = g.s.q0 + (uint32_t)key;
+                        else r = (uint32_t)page_row(a.pages, slot, head);
                     }
-                }
-                if (t + 1 < g.n) page = page_of(g.k0 + t + 1);
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 512 + lt * 4), "r"(r) : "memory");
-                if constexpr (G::Q8) {
+                    if (t + 1 < n) page = page_of(k0 + t + 1);
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 512 + lt * 4), "r"(r) : "memory");
                     float* sc = reinterpret_cast<float*>(sm + G::sc_off) + kst * 384;
                     float ks = 0.0f, lv = 0.0f, rv = in ? 1.0f : 0.0f;
                     if (r != AT_NONE) {
@@ -883,103 +906,187 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     sc[lt] = ks;
                     sc[128 + lt] = lv;
                     sc[256 + lt] = rv;
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-            };
-            for (uint32_t t = 0; t < (uint32_t)G::LAG && t < g.n; ++t) {
-                resolve(t);
-                for (int c = 0; c < W; ++c) piece(false, c, kst, false);
-                kst = kst + 1 == NSTAGE ? 0 : kst + 1;
-            }
-            for (uint32_t t = 0; t < g.n; ++t) {
-                const bool look = !G::Q8 && at_masked(a, w, g, g.k0 + t);
-                for (int c = 0; c < W; ++c) piece(true, c, stage, look);
-                stage = stage + 1 == NSTAGE ? 0 : stage + 1;
-                if (t + G::LAG < g.n) {
-                    resolve(t + G::LAG);
-                    for (int c = 0; c < W; ++c) piece(false, c, kst, false);
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                };
+                for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) {
+                    resolve(t);
+                    for (int c = 0; c < W; ++c) piece(false, c, kst);
                     kst = kst + 1 == NSTAGE ? 0 : kst + 1;
                 }
-            }
-            // everything in before the next row tile (seg names it in s_bad)
-            if constexpr (G::Q8) {
+                for (uint32_t t = 0; t < n; ++t) {
+                    for (int c = 0; c < W; ++c) piece(true, c, stage);
+                    stage = stage + 1 == NSTAGE ? 0 : stage + 1;
+                    if (t + G::LAG < n) {
+                        resolve(t + G::LAG);
+                        for (int c = 0; c < W; ++c) piece(false, c, kst);
+                        kst = kst + 1 == NSTAGE ? 0 : kst + 1;
+                    }
+                }
                 convert();
-            } else if (g.n) {
-                at_cp_wait<0>();
-                for (; given != pieces; ++given) publish(given, check >> (pieces - 1 - given) & 1);
             }
         }
     } else {
-        if constexpr (NQ == 2) at_regs_down<48>();
+        if constexpr (NQ == 2) at_regs_down<64>();
         else at_regs_down<136>();
-        if (warp == NQ * 4 + 4 && lane == 0) {
+        if (warp == NQ * 4 + 5) {
+            // ------------------------------ the list of row tiles ------------------------------
+            AtWalk walk;
+            walk.start(s_plan);
+            for (bool more = true; more; ++seg) {
+                AtSeg g{};
+                more = walk.next(a, w, g);
+                if (!more) g.kind = AT_END;
+                if (seg >= NSEG) at_wait(b_free + 8 * (seg % NSEG), (seg / NSEG - 1) & 1, &s_dead, err);
+                if (s_dead) break;
+                if (lane == 0) {
+                    small.segs[seg % NSEG] = g;
+                    at_arrive(b_seg + 8 * (seg % NSEG));
+                }
+                __syncwarp();
+            }
+        } else if (!G::Q8 && warp == NQ * 4 + 6) {
+            // ------------------------------ copies ------------------------------
+            uint32_t i = 0, raw = 0, last = 0;  // pieces, those to look over; last: parity of a slot's next phase
+            const uint32_t ps = a.pages.k ? 1u << a.pages.page_shift : 0;
+            const uint32_t nowhere = a.pages.k ? (uint32_t)(a.pages.slots >> a.pages.page_shift) * a.kv_heads : 0;
+            for (;; done()) {
+                const AtSeg& g = take();
+                if (g.kind == AT_END || s_dead) break;
+                const int32_t lo = g.lo, hi = g.hi;
+                const uint32_t n = g.n, k0 = g.k0, head = g.h, q0 = g.s.q0;
+                const int32_t* const table = a.table + (uint64_t)g.b * a.table_width;
+                // keys [key, key + rows) x 64 NB dims from dim d
+                auto piece = [&](const CUtensorMap* map, uint32_t key, uint32_t rows, uint32_t d, uint32_t nb, bool look) {
+                    const uint32_t slot = i % NSLOT, dst = smb + G::ring_off + slot * AT_PIECE;
+                    const uint32_t bar = look ? b_raw + 8 * (raw % NSLOT) : b_full + 8 * slot;
+                    if (look) ++raw;
+                    else last ^= 1u << slot;
+                    if (i >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (i / NSLOT - 1) & 1, &s_dead, err);
+                    ++i;
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(AT_PIECE) : "memory");
+                    __syncwarp();
+                    const uint32_t box = ps ? min(ps, rows) : rows, per = rows / box;  // boxes a block of 64 dims
+                    for (uint32_t j = lane; j < per * nb; j += 32) {
+                        const uint32_t blk = j / per, k = key + (j % per) * box;
+                        uint32_t y, z;
+                        if (ps) {
+                            y = k & (ps - 1);
+                            z = nowhere;
+                            if ((int32_t)(k + box) > lo && (int32_t)k < hi) {
+                                const int32_t page = __ldg(table + (k >> a.pages.page_shift));
+                                if (page >= 0 && ((uint64_t)(uint32_t)page << a.pages.page_shift) < a.pages.slots)
+                                    z = (uint32_t)page * a.kv_heads + head;
+                                else
+                                    atomicOr(err, SERVE_ERR_PAGE);
+                            }
+                        } else {
+                            y = head * w.head_step;
+                            z = q0 + k;
+                        }
+                        asm volatile(
+                            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+                            "[%1, {%2, %3, %4}], [%5];" ::"r"(dst + blk * (rows * 128) + (j % per) * (box * 128)),
+                            "l"(map), "r"(d + blk * 64), "r"(y), "r"(z), "r"(bar)
+                            : "memory");
+                    }
+                    __syncwarp();
+                };
+                auto k_tile = [&](uint32_t t) {
+                    for (int c = 0; c < W; ++c) piece(&kmap, (k0 + t) * AT_KEYS, AT_KEYS, c * 64, 1, false);
+                };
+                for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) k_tile(t);
+                for (uint32_t t = 0; t < n; ++t) {
+                    const bool look = at_look(a, lo, hi, g.p0, k0 + t);
+                    for (int c = 0; c < W; ++c) piece(&vmap, (k0 + t) * AT_KEYS + c * G::VKEYS, G::VKEYS, 0, W, look);
+                    if (t + G::LAG < n) k_tile(t + G::LAG);
+                }
+            }
+            if (s_dead)
+                for (uint32_t j = 0; j < (uint32_t)NSLOT; ++j) {
+                    at_wait_flight(b_full + 8 * j, (last >> j & 1) ^ 1);  // true at once for a barrier never used
+                    if (raw > j) at_wait_flight(b_raw + 8 * ((raw - 1 - j) % NSLOT), ((raw - 1 - j) / NSLOT) & 1);
+                }
+        } else if (warp == NQ * 4 + 4) {
             // ------------------------------ products ------------------------------
             const uint32_t iqk = at_idesc<T>(AT_KEYS, false), ipv = at_idesc<T>(D, true);
             const uint32_t q0 = smb + G::q_off, ring = smb + G::ring_off;
-            uint32_t kp = 0;              // ring index of the next K piece to multiply, by its order of arrival
-            uint32_t np[2] = {0, 0}, nq = 0;
-            while (walk.next(a, w, g)) {
-                if (!g.n) continue;
-                // pieces arrive K(0) .. K(LAG - 1), V(0), K(LAG), V(1), ..
-                const uint32_t base = kp;
-                auto k_piece = [&](uint32_t t) { return base + (t < (uint32_t)G::LAG ? t * W : (2 * t - G::LAG + 1) * W); };
-                auto v_piece = [&](uint32_t t) {
-                    // V(t) comes after K(0 .. min(n, t + LAG) - 1) and V(0 .. t - 1)
-                    return base + (min(g.n, t + G::LAG) + t) * W;
-                };
-                auto qk = [&](uint32_t t, uint32_t qi, uint32_t buf, bool first, bool last) {
-                    for (int c = 0; c < W; ++c) {
-                        const uint32_t i = k_piece(t) + c, slot = i % NSLOT;
-                        if (first) at_wait(b_full + 8 * slot, (i / NSLOT) & 1, &s_dead, err);
-                        at_fence_after();
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            at_mma_ss(tmem + buf * 128, at_desc(q0 + (qi * W + c) * AT_PIECE + k * 32, 16, 1024),
-                                      at_desc(ring + slot * AT_PIECE + k * 32, 16, 1024), iqk, c || k);
-                        if (last) at_commit(b_empty + 8 * slot);
-                    }
-                    at_commit(b_s + 8 * buf);
-                };
-                auto pv = [&](uint32_t t, uint32_t qi, uint32_t buf, bool first, bool last) {
-                    for (int c = 0; c < W; ++c) {
-                        const uint32_t i = v_piece(t) + c, slot = i % NSLOT;
-                        if (first) at_wait(b_full + 8 * slot, (i / NSLOT) & 1, &s_dead, err);
-                        at_fence_after();
-#pragma unroll
-                        for (int k = 0; k < G::VKEYS / 16; ++k)
-                            at_mma_ts(tmem + 256 + qi * D, tmem + buf * 128 + (c * G::VKEYS + k * 16) / 2,
-                                      at_desc(ring + slot * AT_PIECE + k * 2048, G::VKEYS * 128, 1024), ipv, t || c || k);
-                        if (last) at_commit(b_empty + 8 * slot);
-                    }
-                    at_commit(b_o + 8 * qi);
-                };
-                for (int i = 0; i < NQ; ++i) {
-                    at_wait(b_q + 8 * i, nq & 1, &s_dead, err);
-                }
-                ++nq;
+            // One thread. A step multiplies P V of a row tile, then Q K of the
+            // tile that its S buffer takes next; the steps of the two row tiles
+            // (NQ = 2) or S buffers (NQ = 1) alternate. Every call is inlined
+            // once: state that a call kept in memory would cost more than a product.
+            uint32_t base = 0;            // pieces of the row tiles before this one
+            uint32_t cleaned = 0, q_phase = 0, p_phase = 0;
+            uint32_t phase = 0;           // bit: parity of the slot's next phase of b_full
+            for (;; done()) {
+                const AtSeg& g = take();
+                if (g.kind == AT_END || s_dead) break;
+                const uint32_t n = g.n;
+                if (!n || lane != 0) continue;
+                const uint32_t k0 = g.k0;
+                const int32_t lo = g.lo, hi = g.hi, p0 = g.p0;
+                for (int i = 0; i < NQ; ++i) at_wait(b_q + 8 * i, q_phase, &s_dead, err);
+                q_phase ^= 1;
                 at_fence_after();
-                if constexpr (NQ == 2) {
-                    qk(0, 0, 0, true, false);
-                    qk(0, 1, 1, false, true);
-                    for (uint32_t t = 0; t < g.n; ++t)
-                        for (uint32_t i = 0; i < 2; ++i) {
-                            at_wait(b_p + 8 * i, np[i]++ & 1, &s_dead, err);
+                const uint32_t steps = NQ == 2 ? 2 * n + 2 : n + 2;
+#pragma unroll 1
+                for (uint32_t u = 0; u < steps; ++u) {
+                    const uint32_t t = NQ == 2 ? u >> 1 : u, qi = NQ == 2 ? u & 1 : 0, buf = u & 1;
+                    // with two row tiles a piece is waited for by the first and freed by the second
+                    const bool first = NQ == 1 || qi == 0, last = NQ == 1 || qi == 1;
+                    if (t >= (uint32_t)G::LAG) {
+                        // O += P V of key tile t - LAG; pieces arrive K(0) .. K(LAG - 1), V(0), K(LAG), V(1), ..
+                        const uint32_t tv = t - G::LAG;
+                        at_wait(b_p + 8 * buf, p_phase >> buf & 1, &s_dead, err);
+                        p_phase ^= 1u << buf;
+                        const bool look = !G::Q8 && first && at_look(a, lo, hi, p0, k0 + tv);
+                        uint32_t slot = (base + (min(n, t) + tv) * W) % NSLOT;
+#pragma unroll 1
+                        for (int c = 0; c < W; ++c) {
+                            if (look) {
+                                at_wait(b_clean + 8 * (cleaned % NSLOT), (cleaned / NSLOT) & 1, &s_dead, err);
+                                ++cleaned;
+                            } else if (first) {
+                                at_wait(b_full + 8 * slot, phase >> slot & 1, &s_dead, err);
+                                phase ^= 1u << slot;
+                            }
                             at_fence_after();
-                            pv(t, i, i, i == 0, i == 1);
-                            if (t + 1 < g.n) qk(t + 1, i, i, i == 0, i == 1);
+                            const uint64_t bd = at_desc(ring + slot * AT_PIECE, G::VKEYS * 128, 1024);
+#pragma unroll
+                            for (int k = 0; k < G::VKEYS / 16; ++k)
+                                at_mma_ts(tmem + 256 + qi * D, tmem + buf * 128 + (c * G::VKEYS + k * 16) / 2,
+                                          bd + k * (2048 >> 4), ipv, tv || c || k);
+                            if (last) at_commit(b_empty + 8 * slot);
+                            slot = slot + 1 == NSLOT ? 0 : slot + 1;
                         }
-                } else {
-                    qk(0, 0, 0, true, true);
-                    if (g.n > 1) qk(1, 0, 1, true, true);
-                    for (uint32_t t = 0; t < g.n; ++t) {
-                        const uint32_t i = t & 1;
-                        at_wait(b_p + 8 * i, np[i]++ & 1, &s_dead, err);
-                        at_fence_after();
-                        pv(t, 0, i, true, true);
-                        if (t + 2 < g.n) qk(t + 2, 0, i, true, true);
+                        at_commit(b_o + 8 * qi);
+                    }
+                    if (t < n) {
+                        // S = Q K
+                        uint32_t slot = (base + (t < (uint32_t)G::LAG ? t : 2 * t - G::LAG + 1) * W) % NSLOT;
+#pragma unroll 1
+                        for (int c = 0; c < W; ++c) {
+                            if (first) {
+                                at_wait(b_full + 8 * slot, phase >> slot & 1, &s_dead, err);
+                                phase ^= 1u << slot;
+                            }
+                            at_fence_after();
+                            const uint64_t ad = at_desc(q0 + (qi * W + c) * AT_PIECE, 16, 1024);
+                            const uint64_t bd = at_desc(ring + slot * AT_PIECE, 16, 1024);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                at_mma_ss(tmem + buf * 128, ad + k * (32 >> 4), bd + k * (32 >> 4), iqk, c || k);
+                            if (last) at_commit(b_empty + 8 * slot);
+                            slot = slot + 1 == NSLOT ? 0 : slot + 1;
+                        }
+                        at_commit(b_s + 8 * buf);
                     }
                 }
-                kp = base + 2 * g.n * W;
+                base += 2 * n * W;
+            }
+            if (s_dead && lane == 0) {
+                at_commit(b_end);
+                at_wait_flight(b_end, 0);
             }
         }
         __syncwarp();
