@@ -127,7 +127,7 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
     w.sub_tokens = 128 / a.group;
     w.tile_tokens = w.sub_tokens * G::NQ;
     w.least_units = 2;
-    w.split_over = 3;
+    w.split_over = 6;
     CUtensorMap km{}, vm{};
     if constexpr (!G::Q8) {
         const bool b = std::is_same_v<T, bf16>;

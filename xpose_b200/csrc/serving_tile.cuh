@@ -16,9 +16,9 @@
 // of TMEM, so one row tile (NQ = 1) with two S buffers; the products of one
 // key tile run beside the softmax of the next.
 //
-// K and V move in 16 KB pieces through one ring (K: 128 keys x 64 dims, V:
-// 8192 / dim keys x dim), so a ring slot is free again as soon as its piece
-// is multiplied. 16-bit rows come by TMA, a box a page, straight into the
+// K and V move in pieces of a tile (dim 256: of half a tile, K by dims and V by
+// keys) through one ring, so a ring slot is free again as soon as its piece is
+// multiplied. 16-bit rows come by TMA, a box a page, straight into the
 // 128-byte swizzled layouts of the tensor core; a page that a tile must not
 // touch is read past the end of the tensor, which gives zeros. What a tile's
 // last page or the next sequence holds past the tile's keys must not be
@@ -43,7 +43,6 @@
 namespace xp {
 
 constexpr int AT_KEYS = 128;        // keys of a tile
-constexpr int AT_PIECE = 16384;     // bytes of a ring slot
 constexpr uint32_t AT_NONE = 0xFFFFFFFFu;
 constexpr uint32_t AT_SPIN_LIMIT = 1u << 20;
 constexpr uint32_t AT_MAX_CTAS = 180;   // partial slots that the scratch holds
@@ -56,15 +55,17 @@ template <class T, class C, int W> struct AtCfg {
     static constexpr int NB = 2 / NQ;             // S buffers of a row tile
     static constexpr int ROWS = 128 * NQ;
     static constexpr int LAG = NB;                // K runs this many tiles ahead of V
-    static constexpr int NSLOT = (Q8 && W > 1) ? 9 : 10;
-    static constexpr int NPIECE = W;              // pieces of a K (or V) tile
-    static constexpr int VKEYS = AT_KEYS / W;     // keys of a V piece
+    static constexpr int NP = W == 4 ? 2 : 1;     // pieces of a K (or V) tile
+    static constexpr int PIECE = W * 16384 / NP;  // bytes of one, and of a ring slot
+    static constexpr int KB = W / NP;             // blocks of 64 dims of a K piece
+    static constexpr int VKEYS = AT_KEYS / NP;    // keys of a V piece
+    static constexpr int NSLOT = W == 1 ? 10 : Q8 ? 4 : 5;
     static constexpr int NSTAGE = W == 1 ? 8 : 4; // tiles whose row numbers and scales are kept
     static constexpr int THREADS = 128 * NQ + 256;
     // shared memory
     static constexpr int q_off = 0;
-    static constexpr int ring_off = NQ * W * AT_PIECE;
-    static constexpr int row_off = ring_off + NSLOT * AT_PIECE;       // [NSTAGE][128] row numbers, 8-bit pages
+    static constexpr int ring_off = NQ * W * 16384;
+    static constexpr int row_off = ring_off + NSLOT * PIECE;       // [NSTAGE][128] row numbers, 8-bit pages
     static constexpr int sc_off = row_off + (Q8 ? NSTAGE * 512 : 0);  // [NSTAGE][3][128] floats, 8-bit pages
     static constexpr int bar_off = sc_off + (Q8 ? NSTAGE * 1536 : 0);
     static constexpr int smem = bar_off + 1024;                       // barriers, plan, row tiles, flags
@@ -78,15 +79,21 @@ struct AtWork {
     uint32_t tile_tokens;   // tokens of a tile
     uint32_t sub_tokens;    // tokens of one of its NQ row tiles
     uint32_t least_units;   // units of a CTA, at least
-    uint32_t split_over;    // split tiles when the largest has this many units more than an even share
+    uint32_t split_over;    // whole tiles while none has more units, or more than an eighth of a CTA's
 };
 enum : uint32_t { AT_FULL = 0, AT_FIRST = 1, AT_MIDDLE = 2, AT_LAST = 3, AT_END = 4 };
 
 // ---- tcgen05 ------------------------------------------------------------------
-XP_DEV uint64_t at_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    // 128-byte swizzle (layout type 2), descriptor version 1
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
+// Shared-memory operands: 128-byte swizzle (layout type 2), descriptor version
+// 1, 1 KB between groups of 8 rows. Low half: address and leading offset.
+XP_DEV uint32_t at_desc_lo(uint32_t saddr, uint32_t lbo) { return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); }
+XP_DEV uint64_t at_desc(uint32_t lo) {
+    return (uint64_t)lo | ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32);
+}
+XP_DEV bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 template <class T> XP_DEV uint32_t at_idesc(uint32_t n, bool b_mn) {
     const uint32_t f = std::is_same_v<T, bf16> ? 1u : 0u;
@@ -125,6 +132,18 @@ XP_DEV void at_st32(uint32_t addr, const uint32_t* r) {
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
         "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::AT_I8(r, 0),
         AT_I8(r, 8), AT_I8(r, 16), AT_I8(r, 24), "r"(addr)
+        : "memory");
+}
+XP_DEV void at_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : AT_R8(r, 0), AT_R8(r, 8)
+        : "r"(addr));
+}
+XP_DEV void at_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::AT_I8(r, 0),
+        AT_I8(r, 8), "r"(addr)
         : "memory");
 }
 XP_DEV void at_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -329,7 +348,7 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
     const uint64_t g = min((uint64_t)gridDim.x, max(total / w.least_units, (uint64_t)1));
     if (c >= g) return;
     const uint64_t u0 = total * c / g, u1 = total * (c + 1) / g;
-    const bool split = most > (total + g - 1) / g + w.split_over;
+    const bool split = most > max((uint64_t)w.split_over, total / (8 * g));
     if (u0 == u1) return;
     // the first tile of the range: split, the one that holds u0; else the
     // first that starts at or after it
@@ -552,7 +571,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             }
             if (g.n) {
                 // Q into the swizzled layout: 8 values a piece, neighbouring threads along a row
-                const uint32_t qs = smb + G::q_off + wg * W * AT_PIECE;
+                const uint32_t qs = smb + G::q_off + wg * W * 16384;
                 constexpr int PR = D / 8;  // 16-byte pieces of a row
 #pragma unroll 1
                 for (uint32_t i0 = 0; i0 < (uint32_t)PR; i0 += 8) {
@@ -571,7 +590,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const uint32_t id = (i0 + i) * 128 + row, r = id / PR, c = id % PR;
-                        at_sts16(qs + (c >> 3) * AT_PIECE + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[i]);
+                        at_sts16(qs + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[i]);
                     }
                 }
                 fence_proxy_async();
@@ -633,14 +652,14 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         // O so far by the same factor, once the product before this one is in it
                         at_wait(b_o + 8 * wg, (npv - 1) & 1, &s_dead, err);
                         at_fence_after();
-#pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            float o[32];
-                            at_ld32(o_tm + c, reinterpret_cast<uint32_t*>(o));
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {  // few at a time: S fills the registers
+                            float o[16];
+                            at_ld16(o_tm + c, reinterpret_cast<uint32_t*>(o));
                             at_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] *= f;
-                            at_st32(o_tm + c, reinterpret_cast<uint32_t*>(o));
+                            for (int i = 0; i < 16; ++i) o[i] *= f;
+                            at_st16(o_tm + c, reinterpret_cast<uint32_t*>(o));
                         }
                         at_wait_st();
 #pragma unroll
@@ -769,10 +788,10 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
         if constexpr (NQ == 2) at_regs_down<80>();
         else at_regs_down<136>();
         const uint32_t lt = tid - NQ * 128;
-        // where 16 bytes c of row r of a piece go: rows of 128 bytes, swizzled;
-        // a V piece has a block of rows for every 64 dims
-        auto k_at = [&](uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); };
-        auto v_at = [&](uint32_t r, uint32_t c) { return (c >> 3) * (G::VKEYS * 128) + k_at(r, c & 7); };
+        // where 16 bytes c of row r of a piece go: for every 64 dims a block of
+        // rows of 128 bytes, swizzled
+        auto k_at = [&](uint32_t r, uint32_t c) { return (c >> 3) * (AT_KEYS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+        auto v_at = [&](uint32_t r, uint32_t c) { return (c >> 3) * (G::VKEYS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
         if constexpr (!G::Q8) {
             // 16-bit pieces come by TMA: only V tiles that need a look pass here
             uint32_t before = 0, cleaned = 0;  // pieces of the row tiles before this one, pieces looked over
@@ -783,14 +802,14 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const uint32_t n = g.n, k0 = g.k0;
                 for (uint32_t t = 0; t < n; ++t) {
                     if (!at_look(a, lo, hi, p0, k0 + t)) continue;
-                    for (int c = 0; c < W; ++c) {
-                        const uint32_t i = before + (min(n, t + G::LAG) + t) * W + c, slot = i % NSLOT;
+                    for (int c = 0; c < G::NP; ++c) {
+                        const uint32_t i = before + (min(n, t + G::LAG) + t) * G::NP + c, slot = i % NSLOT;
                         at_wait(b_raw + 8 * (cleaned % NSLOT), (cleaned / NSLOT) & 1, &s_dead, err);
-                        const uint32_t base = smb + G::ring_off + slot * AT_PIECE;
+                        const uint32_t base = smb + G::ring_off + slot * G::PIECE;
                         constexpr uint32_t mask = std::is_same_v<T, bf16> ? 0x7F80u : 0x7C00u, VU = 8 * W;
                         bool odd = false;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
+                        for (int j = 0; j < G::PIECE / 2048; ++j) {
                             const uint32_t r = lt / VU + j * (128 / VU), at = base + v_at(r, lt % VU);
                             const int32_t key = (int32_t)((k0 + t) * AT_KEYS + c * G::VKEYS + r);
                             if (key < lo || key >= hi) {
@@ -816,40 +835,48 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         ++cleaned;
                     }
                 }
-                before += 2 * n * W;
+                before += 2 * n * G::NP;
             }
         } else {
-            uint32_t pieces = 0, stage = 0;
-            uint4 raw[4];                 // the codes of the piece issued last
+            // a thread's 4 x 16 codes are 16 KB of a piece: SUB of them make one
+            constexpr uint32_t SUB = G::PIECE / 16384;
+            uint32_t subs = 0, stage = 0;
+            uint4 raw[4];                 // the codes of the part issued last
             uint32_t raw_kind = 0;        // ... 0 none, 1 K, 2 V
             const uint32_t rows0 = smb + G::row_off;
-            // thread -> 16 codes: unit u of rows r0, r0 + step, ..
-            constexpr int KU = 4, VU = 4 * W;
+            // thread -> 16 codes: unit u of rows r0, r0 + step, ..; a K part has
+            // all rows of 64 dims, a V part 128 / W whole rows
+            constexpr uint32_t KU = 4, VU = 4 * W;
             // the codes in `raw` into their slot, as 16-bit values
             auto convert = [&]() {
                 if (raw_kind == 0) return;
-                const uint32_t index = pieces - 1, slot = index % NSLOT, base = smb + G::ring_off + slot * AT_PIECE;
-                if (index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
+                const uint32_t index = (subs - 1) / SUB, sub = (subs - 1) % SUB, slot = index % NSLOT;
+                const uint32_t base = smb + G::ring_off + slot * G::PIECE;
+                if (sub == 0 && index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint2 x0 = at_codes<T>(raw[i].x, C{}), x1 = at_codes<T>(raw[i].y, C{});
                     const uint2 x2 = at_codes<T>(raw[i].z, C{}), x3 = at_codes<T>(raw[i].w, C{});
                     uint32_t d0, d1;
                     if (raw_kind == 1) {
-                        const uint32_t r = lt / KU + i * (128 / KU), c = 2 * (lt % KU);
+                        const uint32_t r = lt / KU + i * (128 / KU), c = sub * 8 + 2 * (lt % KU);
                         d0 = k_at(r, c);
                         d1 = k_at(r, c + 1);
                     } else {
-                        const uint32_t r = lt / VU + i * (128 / VU), c = 2 * (lt % VU);
+                        const uint32_t r = sub * (AT_KEYS / W) + lt / VU + i * (128 / VU), c = 2 * (lt % VU);
                         d0 = v_at(r, c);
                         d1 = v_at(r, c + 1);
                     }
                     at_sts16(base + d0, make_uint4(x0.x, x0.y, x1.x, x1.y));
                     at_sts16(base + d1, make_uint4(x2.x, x2.y, x3.x, x3.y));
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) at_arrive(b_full + 8 * slot);
+                if (sub + 1 == SUB) {
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) at_arrive(b_full + 8 * slot);
+                } else {
+                    fence_proxy_async();
+                }
                 raw_kind = 0;
             };
             for (;; done()) {
@@ -860,7 +887,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const int32_t* const table = a.table + (uint64_t)g.b * a.table_width;
                 auto piece = [&](bool is_v, uint32_t c, uint32_t st) {
                     const uint32_t u = is_v ? lt % VU : lt % KU, r0 = is_v ? lt / VU : lt / KU;
-                    const uint32_t step = is_v ? 128 / VU : 128 / KU, key0 = is_v ? c * G::VKEYS : 0;
+                    const uint32_t step = is_v ? 128 / VU : 128 / KU, key0 = is_v ? c * (AT_KEYS / W) : 0;
                     const uint32_t d = (is_v ? u : c * KU + u) * 16;
                     const C* src = static_cast<const C*>(is_v ? a.pages.v : a.pages.k) + d;
                     uint4 now[4];
@@ -874,7 +901,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 4; ++i) raw[i] = now[i];
                     raw_kind = is_v ? 2 : 1;
-                    ++pieces;
+                    ++subs;
                 };
                 auto page_of = [&](uint32_t kt) -> int32_t {
                     const int32_t key = (int32_t)(kt * AT_KEYS + lt);
@@ -957,14 +984,14 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const int32_t* const table = a.table + (uint64_t)g.b * a.table_width;
                 // keys [key, key + rows) x 64 NB dims from dim d
                 auto piece = [&](const CUtensorMap* map, uint32_t key, uint32_t rows, uint32_t d, uint32_t nb, bool look) {
-                    const uint32_t slot = i % NSLOT, dst = smb + G::ring_off + slot * AT_PIECE;
+                    const uint32_t slot = i % NSLOT, dst = smb + G::ring_off + slot * G::PIECE;
                     const uint32_t bar = look ? b_raw + 8 * (raw % NSLOT) : b_full + 8 * slot;
                     if (look) ++raw;
                     else last ^= 1u << slot;
                     if (i >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (i / NSLOT - 1) & 1, &s_dead, err);
                     ++i;
                     if (lane == 0)
-                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(AT_PIECE) : "memory");
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(G::PIECE) : "memory");
                     __syncwarp();
                     const uint32_t box = ps ? min(ps, rows) : rows, per = rows / box;  // boxes a block of 64 dims
                     for (uint32_t j = lane; j < per * nb; j += 32) {
@@ -993,12 +1020,12 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     __syncwarp();
                 };
                 auto k_tile = [&](uint32_t t) {
-                    for (int c = 0; c < W; ++c) piece(&kmap, (k0 + t) * AT_KEYS, AT_KEYS, c * 64, 1, false);
+                    for (int c = 0; c < G::NP; ++c) piece(&kmap, (k0 + t) * AT_KEYS, AT_KEYS, c * G::KB * 64, G::KB, false);
                 };
                 for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) k_tile(t);
                 for (uint32_t t = 0; t < n; ++t) {
                     const bool look = at_look(a, lo, hi, g.p0, k0 + t);
-                    for (int c = 0; c < W; ++c) piece(&vmap, (k0 + t) * AT_KEYS + c * G::VKEYS, G::VKEYS, 0, W, look);
+                    for (int c = 0; c < G::NP; ++c) piece(&vmap, (k0 + t) * AT_KEYS + c * G::VKEYS, G::VKEYS, 0, W, look);
                     if (t + G::LAG < n) k_tile(t + G::LAG);
                 }
             }
@@ -1011,23 +1038,23 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             // ------------------------------ products ------------------------------
             const uint32_t iqk = at_idesc<T>(AT_KEYS, false), ipv = at_idesc<T>(D, true);
             const uint32_t q0 = smb + G::q_off, ring = smb + G::ring_off;
-            // One thread. A step multiplies P V of a row tile, then Q K of the
-            // tile that its S buffer takes next; the steps of the two row tiles
-            // (NQ = 2) or S buffers (NQ = 1) alternate. Every call is inlined
-            // once: state that a call kept in memory would cost more than a product.
+            // A step multiplies P V of a row tile, then Q K of the tile that its S
+            // buffer takes next; the steps of the two row tiles (NQ = 2) or S
+            // buffers (NQ = 1) alternate. The whole warp runs the loop, so that
+            // addresses and descriptors are uniform, and one lane issues.
+            const bool lead = elect_one();
             uint32_t base = 0;            // pieces of the row tiles before this one
             uint32_t cleaned = 0, q_phase = 0, p_phase = 0;
             uint32_t phase = 0;           // bit: parity of the slot's next phase of b_full
             for (;; done()) {
                 const AtSeg& g = take();
                 if (g.kind == AT_END || s_dead) break;
-                const uint32_t n = g.n;
-                if (!n || lane != 0) continue;
+                const uint32_t n = __shfl_sync(0xffffffffu, g.n, 0);
+                if (!n) continue;
                 const uint32_t k0 = g.k0;
                 const int32_t lo = g.lo, hi = g.hi, p0 = g.p0;
                 for (int i = 0; i < NQ; ++i) at_wait(b_q + 8 * i, q_phase, &s_dead, err);
                 q_phase ^= 1;
-                at_fence_after();
                 const uint32_t steps = NQ == 2 ? 2 * n + 2 : n + 2;
 #pragma unroll 1
                 for (uint32_t u = 0; u < steps; ++u) {
@@ -1037,12 +1064,12 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     if (t >= (uint32_t)G::LAG) {
                         // O += P V of key tile t - LAG; pieces arrive K(0) .. K(LAG - 1), V(0), K(LAG), V(1), ..
                         const uint32_t tv = t - G::LAG;
+                        const bool look = !G::Q8 && first && at_look(a, lo, hi, p0, k0 + tv);
+                        uint32_t slot = (base + (min(n, t) + tv) * G::NP) % NSLOT;
                         at_wait(b_p + 8 * buf, p_phase >> buf & 1, &s_dead, err);
                         p_phase ^= 1u << buf;
-                        const bool look = !G::Q8 && first && at_look(a, lo, hi, p0, k0 + tv);
-                        uint32_t slot = (base + (min(n, t) + tv) * W) % NSLOT;
-#pragma unroll 1
-                        for (int c = 0; c < W; ++c) {
+#pragma unroll
+                        for (int c = 0; c < G::NP; ++c) {
                             if (look) {
                                 at_wait(b_clean + 8 * (cleaned % NSLOT), (cleaned / NSLOT) & 1, &s_dead, err);
                                 ++cleaned;
@@ -1051,40 +1078,48 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                                 phase ^= 1u << slot;
                             }
                             at_fence_after();
-                            const uint64_t bd = at_desc(ring + slot * AT_PIECE, G::VKEYS * 128, 1024);
+                            const uint32_t bd = at_desc_lo(ring + slot * G::PIECE, G::VKEYS * 128);
+                            if (lead) {
 #pragma unroll
-                            for (int k = 0; k < G::VKEYS / 16; ++k)
-                                at_mma_ts(tmem + 256 + qi * D, tmem + buf * 128 + (c * G::VKEYS + k * 16) / 2,
-                                          bd + k * (2048 >> 4), ipv, tv || c || k);
-                            if (last) at_commit(b_empty + 8 * slot);
+                                for (int k = 0; k < G::VKEYS / 16; ++k)
+                                    at_mma_ts(tmem + 256 + qi * D, tmem + buf * 128 + (c * G::VKEYS + k * 16) / 2,
+                                              at_desc(bd + k * (2048 >> 4)), ipv, c || k ? 1u : tv);
+                                if (last) at_commit(b_empty + 8 * slot);
+                                if (c == G::NP - 1) at_commit(b_o + 8 * qi);
+                            }
+                            __syncwarp();
                             slot = slot + 1 == NSLOT ? 0 : slot + 1;
                         }
-                        at_commit(b_o + 8 * qi);
                     }
                     if (t < n) {
                         // S = Q K
-                        uint32_t slot = (base + (t < (uint32_t)G::LAG ? t : 2 * t - G::LAG + 1) * W) % NSLOT;
-#pragma unroll 1
-                        for (int c = 0; c < W; ++c) {
+                        uint32_t slot = (base + (t < (uint32_t)G::LAG ? t : 2 * t - G::LAG + 1) * G::NP) % NSLOT;
+#pragma unroll
+                        for (int c = 0; c < G::NP; ++c) {
                             if (first) {
                                 at_wait(b_full + 8 * slot, phase >> slot & 1, &s_dead, err);
                                 phase ^= 1u << slot;
                             }
                             at_fence_after();
-                            const uint64_t ad = at_desc(q0 + (qi * W + c) * AT_PIECE, 16, 1024);
-                            const uint64_t bd = at_desc(ring + slot * AT_PIECE, 16, 1024);
+                            const uint32_t ad = at_desc_lo(q0 + (qi * W + c * G::KB) * 16384, 16);
+                            const uint32_t bd = at_desc_lo(ring + slot * G::PIECE, 16);
+                            if (lead) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                at_mma_ss(tmem + buf * 128, ad + k * (32 >> 4), bd + k * (32 >> 4), iqk, c || k);
-                            if (last) at_commit(b_empty + 8 * slot);
+                                for (int k = 0; k < 4 * G::KB; ++k) {
+                                    const uint32_t at = (k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4);
+                                    at_mma_ss(tmem + buf * 128, at_desc(ad + at), at_desc(bd + at), iqk, c || k ? 1u : 0u);
+                                }
+                                if (last) at_commit(b_empty + 8 * slot);
+                                if (c == G::NP - 1) at_commit(b_s + 8 * buf);
+                            }
+                            __syncwarp();
                             slot = slot + 1 == NSLOT ? 0 : slot + 1;
                         }
-                        at_commit(b_s + 8 * buf);
                     }
                 }
-                base += 2 * n * W;
+                base += 2 * n * G::NP;
             }
-            if (s_dead && lane == 0) {
+            if (s_dead && lead) {
                 at_commit(b_end);
                 at_wait_flight(b_end, 0);
             }
