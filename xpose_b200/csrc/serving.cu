@@ -126,11 +126,17 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
                   "scratch");
     w.sub_tokens = 128 / a.group;
     w.tile_tokens = w.sub_tokens * G::NQ;
-    w.least_units = 2;
-    w.split_over = 6;
-    CUtensorMap km{}, vm{};
+    w.least_units = AT_COST + 2;
+    w.split_over = AT_COST + 6;
+    CUtensorMap qm{}, km{}, vm{};
+    const bool b = std::is_same_v<T, bf16>;
+    {
+        const uint64_t n[2] = {a.heads, a.tokens};
+        const uint64_t stride[2] = {a.heads > 1 ? (uint64_t)a.q.hs * 2 : G::D * 2, a.tokens > 1 ? (uint64_t)a.q.ts * 2 : G::D * 2};
+        const uint32_t box[2] = {a.group, w.sub_tokens};
+        TRY(row_map(who, &qm, b, a.q.data, G::D, n, stride, box));
+    }
     if constexpr (!G::Q8) {
-        const bool b = std::is_same_v<T, bf16>;
         if (a.pages.k) {
             const uint32_t ps = 1u << a.pages.page_shift;
             const uint64_t n[2] = {ps, (a.pages.slots >> a.pages.page_shift) * a.kv_heads};
@@ -153,7 +159,7 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
             TRY(row_map(who, &vm, b, a.v.data, G::D, n, vs, vbox));
         }
     }
-    cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, false, a, w, km, vm);
+    cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, false, a, w, qm, km, vm);
     if (e == cudaSuccess)
         e = launch_ex(attn_join_kernel<T, W, G::ROWS>, dim3(ctas, G::ROWS / 32), dim3(256), 0, st, 1, true, a, w, ctas);
     if (e != cudaSuccess) return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
@@ -312,6 +318,9 @@ xp_status attention(const char* who, void* stream, const xp_rows* out, const xp_
     TRY(check_rows(who, "q", q, 8));
     TRY(check_rows(who, "out", out, 8));
     REQUIRE(q->dtype != XP_F32, "%s: 'q' must be F16 or BF16", who);
+    REQUIRE((q->token_stride > 0 || q->tokens <= 1) && (q->head_stride > 0 || q->heads <= 1) && q->token_stride >= 0 &&
+                q->head_stride >= 0,
+            "%s: 'q' needs positive strides", who);
     REQUIRE(same_shape(q, out), "%s: 'q' and 'out' differ in shape or type", who);
     REQUIRE(q->dim == 64 || q->dim == 128 || q->dim == 256, "%s: dim must be 64, 128 or 256 (got %u)", who, q->dim);
     uint32_t kv_heads, cache;

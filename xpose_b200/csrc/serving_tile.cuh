@@ -43,6 +43,7 @@
 namespace xp {
 
 constexpr int AT_KEYS = 128;        // keys of a tile
+constexpr uint32_t AT_COST = 2;     // what a row tile costs besides its key tiles, in key tiles
 constexpr uint32_t AT_NONE = 0xFFFFFFFFu;
 constexpr uint32_t AT_SPIN_LIMIT = 1u << 20;
 constexpr uint32_t AT_MAX_CTAS = 180;   // partial slots that the scratch holds
@@ -240,6 +241,12 @@ template <class T> XP_DEV uint2 at_codes(uint32_t w, fp8c) {
     }
     return make_uint2(a, b);
 }
+XP_DEV void at_tma(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
 XP_DEV uint32_t at_lds(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -252,6 +259,22 @@ XP_DEV uint4 at_lds16(uint32_t a) {
 }
 XP_DEV void at_sts16(uint32_t a, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// x[i] of lane l (of four) <-> x[l] of lane i: two rounds, each swaps half
+XP_DEV void at_swap16(uint4& lo, uint4& hi, bool up, int m) {
+    const uint4 s = up ? lo : hi;
+    const uint4 y = make_uint4(__shfl_xor_sync(0xffffffffu, s.x, m), __shfl_xor_sync(0xffffffffu, s.y, m),
+                               __shfl_xor_sync(0xffffffffu, s.z, m), __shfl_xor_sync(0xffffffffu, s.w, m));
+    lo = up ? y : lo;
+    hi = up ? hi : y;
+}
+XP_DEV void at_transpose4(uint4 (&x)[4]) {
+    const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
+    at_swap16(x[0], x[1], b0, 1);
+    at_swap16(x[2], x[3], b0, 1);
+    at_swap16(x[0], x[2], b1, 2);
+    at_swap16(x[1], x[3], b1, 2);
 }
 
 // ---- the split of the work --------------------------------------------------------
@@ -271,9 +294,9 @@ XP_DEV AtTile at_tile(const Seq& s, uint32_t x, uint32_t tt, uint32_t window) {
 }
 
 // Where a CTA starts in the list of units: head h, sequence b, tile x. A tile
-// without keys counts as one unit.
+// counts as its key tiles and AT_COST more, which come first.
 struct AtPlan {
-    uint32_t h, b, x, skip;   // skip: key tiles of the first tile that an earlier CTA has
+    uint32_t h, b, x, skip;   // skip: units of the first tile that earlier CTAs have
     int64_t todo;             // units from there; whole tiles: those that start within them
     bool split;
 };
@@ -324,7 +347,7 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
         }
         b = lo;
         x = i - (lo ? ends[lo - 1] : 0);
-        return max(at_tile(seq_of(a, b), x, w.tile_tokens, a.window).n, 1u);
+        return at_tile(seq_of(a, b), x, w.tile_tokens, a.window).n + AT_COST;
     };
     uint64_t all = 0;
     uint32_t most = 0, b = 0, x = 0;
@@ -397,7 +420,8 @@ struct AtWalk {
     Seq s;
     uint32_t have;      // s is sequence have
     XP_DEV void start(const AtPlan& plan) { p = plan; have = AT_NONE; }
-    XP_DEV bool next(const ServeAttnArgs& a, const AtWork& w, AtSeg& g) {
+    __device__ bool next(const ServeAttnArgs& a, const AtWork& w, AtSeg& g) {
+      for (;;) {
         if (p.todo <= 0) return false;
         for (;;) {
             if (have != p.b) {
@@ -419,15 +443,20 @@ struct AtWalk {
         g.lo = t.lo;
         g.hi = t.hi;
         g.p0 = (int32_t)s.nkv - (int32_t)s.nq + (int32_t)(p.x * w.tile_tokens);
-        const uint32_t n = max(t.n, 1u);
-        const uint32_t take = p.split ? (uint32_t)min((int64_t)(n - p.skip), p.todo) : n;
-        g.kind = p.skip == 0 ? (take == n ? AT_FULL : AT_FIRST) : (p.skip + take == n ? AT_LAST : AT_MIDDLE);
-        g.k0 = t.t0 + p.skip;
-        g.n = t.n ? take : 0;
-        p.todo -= take;
+        // units [skip, skip + step) of the tile are these of its key tiles
+        const uint32_t all = t.n + AT_COST;
+        const uint32_t step = p.split ? (uint32_t)min((int64_t)(all - p.skip), p.todo) : all;
+        const uint32_t from = max(p.skip, AT_COST) - AT_COST, to = max(p.skip + step, AT_COST) - AT_COST;
+        g.kind = from == 0 ? (to == t.n ? AT_FULL : AT_FIRST) : (to == t.n ? AT_LAST : AT_MIDDLE);
+        g.k0 = t.t0 + from;
+        g.n = to - from;
+        // no key tile falls to this CTA: a neighbour has the tile, or it has none
+        const bool none = t.n ? to == from : p.skip != 0;
+        p.todo -= step;
         p.skip = 0;
         ++p.x;
-        return true;
+        if (!none) return true;
+      }
     }
 };
 
@@ -444,14 +473,15 @@ XP_DEV bool at_odd16(uint32_t w, uint32_t exp_mask) {  // an infinity or NaN in 
 template <class T, class C, int W>
 __global__ void __launch_bounds__(AtCfg<T, C, W>::THREADS, 1)
 attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ AtWork w,
-                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+                 const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                 const __grid_constant__ CUtensorMap vmap) {
     using G = AtCfg<T, C, W>;
     constexpr int D = G::D, NQ = G::NQ, NSLOT = G::NSLOT, NSTAGE = G::NSTAGE;
     // no static shared memory: the dynamic part then starts on a 1 KB boundary,
     // which the swizzled layouts need, without a byte lost
     extern __shared__ __align__(1024) unsigned char sm[];
     const uint32_t smb = smem_u32(sm);
-    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 9 + 2 * NSEG;
+    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 11 + 2 * NSEG;
     struct Small {
         AtPlan plan;
         AtSeg segs[NSEG];
@@ -474,7 +504,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     const uint32_t b_s = b_q + 16, b_p = b_s + 16;  // [2] S made, P made (by S buffer)
     const uint32_t b_o = b_p + 16;                  // [NQ] P V added
     const uint32_t b_seg = b_o + 16, b_free = b_seg + NSEG * 8;  // [NSEG] a row tile given, done with
-    const uint32_t b_end = b_free + NSEG * 8;       // products in flight after a failed wait
+    const uint32_t b_qfree = b_free + NSEG * 8;     // [NQ] Q multiplied for the last time
+    const uint32_t b_end = b_qfree + 16;            // products in flight after a failed wait
 
     if (smb & 1023) {  // cannot be multiplied from
         if (tid == 0) atomicOr(a.err, SERVE_ERR_WAIT);
@@ -490,16 +521,16 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
         }
         m += 4 * NSLOT;
         for (int i = 0; i < 2; ++i) {
-            mbar_init(m + i, 4);
+            mbar_init(m + i, 1);
             mbar_init(m + 2 + i, 1);
             mbar_init(m + 4 + i, 4);
             mbar_init(m + 6 + i, 1);
         }
         for (int i = 0; i < NSEG; ++i) {
             mbar_init(m + 8 + i, 1);
-            mbar_init(m + 8 + NSEG + i, NQ * 4 + 4 + 1 + (G::Q8 ? 0 : 1));
+            mbar_init(m + 8 + NSEG + i, NQ * 4 + 4 + 2);
         }
-        mbar_init(m + 8 + 2 * NSEG, 1);
+        for (int i = 0; i < 3; ++i) mbar_init(m + 8 + 2 * NSEG + i, 1);
         fence_mbar_init();
         s_dead = 0;
         for (int i = 0; i < 4; ++i) s_bad[i] = 0;
@@ -568,34 +599,6 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             if (real) {
                 khi = max(pos + 1, 0);
                 klo = a.window ? (int32_t)max((int64_t)pos + 1 - (int64_t)a.window, (int64_t)0) : 0;
-            }
-            if (g.n) {
-                // Q into the swizzled layout: 8 values a piece, neighbouring threads along a row
-                const uint32_t qs = smb + G::q_off + wg * W * 16384;
-                constexpr int PR = D / 8;  // 16-byte pieces of a row
-#pragma unroll 1
-                for (uint32_t i0 = 0; i0 < (uint32_t)PR; i0 += 8) {
-                    uint4 v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t id = (i0 + i) * 128 + row, r = id / PR, c = id % PR;
-                        const uint32_t t1 = r / a.group, g1 = r - t1 * a.group;
-                        const uint32_t tk = g.x * w.tile_tokens + qrow0 + t1;
-                        v[i] = make_uint4(0, 0, 0, 0);
-                        if (t1 < w.sub_tokens && tk < g.s.nq)
-                            v[i] = __ldg(reinterpret_cast<const uint4*>(
-                                static_cast<const T*>(a.q.data) + (int64_t)(g.s.q0 + tk) * a.q.ts +
-                                (int64_t)(g.h * a.group + g1) * a.q.hs + c * 8));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t id = (i0 + i) * 128 + row, r = id / PR, c = id % PR;
-                        at_sts16(qs + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[i]);
-                    }
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) at_arrive(b_q + 8 * wg);
             }
             float m = -INFINITY, ref = 0.0f;
             float2 l2[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
@@ -719,7 +722,12 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             const uint32_t slot = 2 * blockIdx.x + (g.kind == AT_FIRST ? 1 : 0);
             unsigned char* part = w.slots + (size_t)slot * w.slot_bytes;
             const uint64_t orow = (uint64_t)(g.s.q0 + tok), ohead = g.h * a.group + rg;
-            T* op = static_cast<T*>(a.out.data) + (int64_t)orow * a.out.ts + (int64_t)ohead * a.out.hs;
+            T* const op = static_cast<T*>(a.out.data) + (int64_t)orow * a.out.ts + (int64_t)ohead * a.out.hs;
+            // four neighbouring lanes store 64 bytes of one of their rows at a time
+            unsigned long long at4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                at4[i] = __shfl_sync(0xffffffffu, real ? reinterpret_cast<unsigned long long>(op) : 0ull, (lane & ~3u) + i);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float o[32];
@@ -756,17 +764,18 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     }
                 }
                 if (whole) {
-                    if (real) {
+                    uint4 x[4];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint4 r;
-                            r.x = at_pack<T>(o[i] * inv, o[i + 1] * inv);
-                            r.y = at_pack<T>(o[i + 2] * inv, o[i + 3] * inv);
-                            r.z = at_pack<T>(o[i + 4] * inv, o[i + 5] * inv);
-                            r.w = at_pack<T>(o[i + 6] * inv, o[i + 7] * inv);
-                            *reinterpret_cast<uint4*>(op + c + i) = r;
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        x[i].x = at_pack<T>(o[8 * i] * inv, o[8 * i + 1] * inv);
+                        x[i].y = at_pack<T>(o[8 * i + 2] * inv, o[8 * i + 3] * inv);
+                        x[i].z = at_pack<T>(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
+                        x[i].w = at_pack<T>(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
                     }
+                    at_transpose4(x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (at4[i]) reinterpret_cast<uint4*>(reinterpret_cast<T*>(at4[i]) + c)[lane & 3] = x[i];
                 } else if (real) {
                     float4* pp = reinterpret_cast<float4*>(part) + (size_t)(c / 4) * G::ROWS + wg * 128 + row;
 #pragma unroll
@@ -971,9 +980,10 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 }
                 __syncwarp();
             }
-        } else if (!G::Q8 && warp == NQ * 4 + 6) {
+        } else if (warp == NQ * 4 + 6) {
             // ------------------------------ copies ------------------------------
             uint32_t i = 0, raw = 0, last = 0;  // pieces, those to look over; last: parity of a slot's next phase
+            uint32_t tiles = 0;                 // row tiles with keys
             const uint32_t ps = a.pages.k ? 1u << a.pages.page_shift : 0;
             const uint32_t nowhere = a.pages.k ? (uint32_t)(a.pages.slots >> a.pages.page_shift) * a.kv_heads : 0;
             for (;; done()) {
@@ -981,6 +991,25 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 if (g.kind == AT_END || s_dead) break;
                 const int32_t lo = g.lo, hi = g.hi;
                 const uint32_t n = g.n, k0 = g.k0, head = g.h, q0 = g.s.q0;
+                if (!n) continue;
+                // Q: the tile's tokens x the heads of the kv head. Tokens past the
+                // sequence are other rows or zeros: padding rows, which nothing reads.
+                auto q_tile = [&](uint32_t qi) {
+                    if (tiles) at_wait(b_qfree + 8 * qi, (tiles - 1) & 1, &s_dead, err);
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b_q + 8 * qi),
+                                     "r"(W * 128 * w.sub_tokens * a.group) : "memory");
+                    __syncwarp();
+                    if (lane < W)
+                        at_tma(smb + G::q_off + (qi * W + lane) * 16384, &qmap, lane * 64, head * a.group,
+                               q0 + g.x * w.tile_tokens + qi * w.sub_tokens, b_q + 8 * qi);
+                    __syncwarp();
+                };
+                if constexpr (G::Q8) {
+                    for (uint32_t qi = 0; qi < (uint32_t)NQ; ++qi) q_tile(qi);
+                    ++tiles;
+                    continue;
+                }
                 const int32_t* const table = a.table + (uint64_t)g.b * a.table_width;
                 // keys [key, key + rows) x 64 NB dims from dim d
                 auto piece = [&](const CUtensorMap* map, uint32_t key, uint32_t rows, uint32_t d, uint32_t nb, bool look) {
@@ -1011,29 +1040,31 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                             y = head * w.head_step;
                             z = q0 + k;
                         }
-                        asm volatile(
-                            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-                            "[%1, {%2, %3, %4}], [%5];" ::"r"(dst + blk * (rows * 128) + (j % per) * (box * 128)),
-                            "l"(map), "r"(d + blk * 64), "r"(y), "r"(z), "r"(bar)
-                            : "memory");
+                        at_tma(dst + blk * (rows * 128) + (j % per) * (box * 128), map, d + blk * 64, y, z, bar);
                     }
                     __syncwarp();
                 };
                 auto k_tile = [&](uint32_t t) {
                     for (int c = 0; c < G::NP; ++c) piece(&kmap, (k0 + t) * AT_KEYS, AT_KEYS, c * G::KB * 64, G::KB, false);
                 };
-                for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) k_tile(t);
+                q_tile(0);
+                k_tile(0);
+                if (NQ == 2) q_tile(1);
+                ++tiles;
+                for (uint32_t t = 1; t < (uint32_t)G::LAG && t < n; ++t) k_tile(t);
                 for (uint32_t t = 0; t < n; ++t) {
                     const bool look = at_look(a, lo, hi, g.p0, k0 + t);
                     for (int c = 0; c < G::NP; ++c) piece(&vmap, (k0 + t) * AT_KEYS + c * G::VKEYS, G::VKEYS, 0, W, look);
                     if (t + G::LAG < n) k_tile(t + G::LAG);
                 }
             }
-            if (s_dead)
-                for (uint32_t j = 0; j < (uint32_t)NSLOT; ++j) {
+            if (s_dead) {
+                for (uint32_t j = 0; j < (uint32_t)NQ && tiles; ++j) at_wait_flight(b_q + 8 * j, (tiles - 1) & 1);
+                for (uint32_t j = 0; j < (uint32_t)NSLOT && !G::Q8; ++j) {
                     at_wait_flight(b_full + 8 * j, (last >> j & 1) ^ 1);  // true at once for a barrier never used
                     if (raw > j) at_wait_flight(b_raw + 8 * ((raw - 1 - j) % NSLOT), ((raw - 1 - j) / NSLOT) & 1);
                 }
+            }
         } else if (warp == NQ * 4 + 4) {
             // ------------------------------ products ------------------------------
             const uint32_t iqk = at_idesc<T>(AT_KEYS, false), ipv = at_idesc<T>(D, true);
@@ -1111,6 +1142,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                                 }
                                 if (last) at_commit(b_empty + 8 * slot);
                                 if (c == G::NP - 1) at_commit(b_s + 8 * buf);
+                                if (c == G::NP - 1 && t + 1 == n) at_commit(b_qfree + 8 * qi);
                             }
                             __syncwarp();
                             slot = slot + 1 == NSLOT ? 0 : slot + 1;
