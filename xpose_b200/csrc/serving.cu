@@ -7,7 +7,7 @@
 #include <cmath>
 
 #include "host.cuh"
-#include "serving_tile.cuh"
+#include "serving_few.cuh"
 
 using namespace xp;
 
@@ -126,6 +126,8 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
                   "scratch");
     w.sub_tokens = 128 / a.group;
     w.tile_tokens = w.sub_tokens * G::NQ;
+    w.shift = AT_SHIFT;
+    w.cost = AT_COST;
     w.least_units = AT_COST + 2;
     w.split_over = AT_COST + 6;
     CUtensorMap qm{}, km{}, vm{};
@@ -164,6 +166,29 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
         e = launch_ex(attn_join_kernel<T, W, G::ROWS>, dim3(ctas, G::ROWS / 32), dim3(256), 0, st, 1, true, a, w, ctas);
     if (e != cudaSuccess) return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return XP_OK;
+}
+
+template <class T, class C, int W, int NR>
+xp_status launch_few(const char* who, const ServeAttnArgs& a, void* scratch, cudaStream_t st) {
+    using G = FwCfg<T, C, W, NR>;
+    static_assert(G::smem <= 227 * 1024, "shared memory");
+    static std::atomic<bool> attr_set[kMaxDevices];
+    auto kernel = attn_few_kernel<T, C, W, NR>;
+    if (cudaError_t e = smem_attr_once(attr_set, kernel, G::smem); e != cudaSuccess)
+        return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    constexpr uint32_t most = 4 * AT_MAX_CTAS;
+    const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count() * G::CTAS, most);
+    AtWork w{};
+    w.slot_bytes = 8 * NR * (G::D * 4 + 8);
+    w.slots = static_cast<unsigned char*>(scratch) + 16384;
+    static_assert(256 + most * 4 <= 16384 && 16384 + 2ull * most * 8 * NR * (G::D * 4 + 8) <= XP_SERVING_SCRATCH_BYTES, "scratch");
+    w.tile_tokens = 16;  // all of a sequence's
+    w.shift = 6;
+    w.cost = 2;
+    w.least_units = 3;
+    w.split_over = 0;
+    kernel<<<ctas, 128, G::smem, st>>>(a, w, reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(scratch) + 16384 - most * 4));
+    return launched(who);
 }
 
 template <class F> xp_status for_type(uint32_t dtype, F f) {
@@ -385,10 +410,10 @@ xp_status attention(const char* who, void* stream, const xp_rows* out, const xp_
                 using T = decltype(t);
                 using C = decltype(c);
                 if constexpr (sizeof(T) == 2 && (sizeof(C) == 1 || std::is_same_v<C, T>)) {
-                    if (pages && (uint64_t)q_most * a.group <= 16) {
-                        attn_rows_kernel<T, C, d.value><<<dim3(q->tokens, q->heads), 128, 0, (cudaStream_t)stream>>>(a);
-                        return launched(who);
-                    }
+                    // up to 16 rows a kv head: read-bound, one pass of warp products
+                    const uint64_t rows = (uint64_t)q_most * a.group;
+                    if (pages && rows <= 8) return launch_few<T, C, d.value, 1>(who, a, scratch, (cudaStream_t)stream);
+                    if (pages && rows <= 16) return launch_few<T, C, d.value, 2>(who, a, scratch, (cudaStream_t)stream);
                     return launch_tiles<T, C, d.value>(who, a, scratch, (cudaStream_t)stream);
                 } else {
                     return fail(XP_ERR_UNSUPPORTED, "%s: no kernel for these types", who);

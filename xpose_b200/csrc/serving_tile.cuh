@@ -44,10 +44,11 @@ namespace xp {
 
 constexpr int AT_KEYS = 128;        // keys of a tile
 constexpr uint32_t AT_COST = 2;     // what a row tile costs besides its key tiles, in key tiles
+constexpr uint32_t AT_SHIFT = 7;    // log2 AT_KEYS
 constexpr uint32_t AT_NONE = 0xFFFFFFFFu;
 constexpr uint32_t AT_SPIN_LIMIT = 1u << 20;
 constexpr uint32_t AT_MAX_CTAS = 180;   // partial slots that the scratch holds
-constexpr uint32_t AT_MAX_BATCH = 16384;
+constexpr uint32_t AT_MAX_BATCH = 8192;   // sequences whose tile counts fit in shared memory
 
 template <class T, class C, int W> struct AtCfg {
     static constexpr int D = 64 * W;
@@ -79,6 +80,7 @@ struct AtWork {
     uint32_t head_step;     // packed: k and v heads a kv head apart in the tensor maps (0: one for all)
     uint32_t tile_tokens;   // tokens of a tile
     uint32_t sub_tokens;    // tokens of one of its NQ row tiles
+    uint32_t shift, cost;   // log2 of the keys of a key tile; what a tile costs besides them, in key tiles
     uint32_t least_units;   // units of a CTA, at least
     uint32_t split_over;    // whole tiles while none has more units, or more than an eighth of a CTA's
 };
@@ -281,23 +283,40 @@ XP_DEV void at_transpose4(uint4 (&x)[4]) {
 // Tile x of a sequence: tokens [x tt, ..), its key range [lo, hi) and the key
 // tiles that cover it.
 struct AtTile { int32_t lo, hi; uint32_t t0, n; };
-XP_DEV AtTile at_tile(const Seq& s, uint32_t x, uint32_t tt, uint32_t window) {
+XP_DEV AtTile at_tile(const Seq& s, uint32_t x, uint32_t tt, uint32_t window, uint32_t shift) {
     AtTile r;
     const int32_t first = (int32_t)s.nkv - (int32_t)s.nq;
     const uint32_t tok0 = x * tt, tok1 = min(tok0 + tt, s.nq);
     r.hi = max(first + (int32_t)tok1, 0);
     const int64_t lo = window ? (int64_t)first + tok0 + 1 - (int64_t)window : 0;
     r.lo = (int32_t)min(max(lo, (int64_t)0), (int64_t)r.hi);
-    r.t0 = (uint32_t)r.lo / AT_KEYS;
-    r.n = r.hi > r.lo ? ((uint32_t)r.hi + AT_KEYS - 1) / AT_KEYS - r.t0 : 0;
+    r.t0 = (uint32_t)r.lo >> shift;
+    r.n = r.hi > r.lo ? (((uint32_t)r.hi - 1) >> shift) + 1 - r.t0 : 0;
     return r;
 }
 
+// Zeros for the rows of q that are in no sequence.
+template <class T, int D> XP_DEV void at_clear(const ServeAttnArgs& a, uint32_t threads) {
+    const uint32_t lo = (uint32_t)min(max(__ldg(a.starts), 0), (int32_t)a.tokens);
+    const uint32_t hi = max((uint32_t)min(max(__ldg(a.starts + a.batch), 0), (int32_t)a.tokens), lo);
+    const uint64_t n = (uint64_t)(lo + (a.tokens - hi)) * a.heads * (D / 8);
+    for (uint64_t i = (uint64_t)blockIdx.x * threads + threadIdx.x; i < n; i += (uint64_t)gridDim.x * threads) {
+        const uint32_t d = (uint32_t)(i % (D / 8)) * 8, h = (uint32_t)(i / (D / 8) % a.heads);
+        uint32_t tok = (uint32_t)(i / (D / 8) / a.heads);
+        if (tok >= lo) tok += hi - lo;
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out.data) + (int64_t)tok * a.out.ts + (int64_t)h * a.out.hs + d) =
+            make_uint4(0, 0, 0, 0);
+        if (a.lse && d == 0) a.lse[(uint64_t)tok * a.heads + h] = -INFINITY;
+    }
+}
+
 // Where a CTA starts in the list of units: head h, sequence b, tile x. A tile
-// counts as its key tiles and AT_COST more, which come first.
+// counts as its key tiles and `cost` more, which come first.
 struct AtPlan {
     uint32_t h, b, x, skip;   // skip: units of the first tile that earlier CTAs have
     int64_t todo;             // units from there; whole tiles: those that start within them
+    uint64_t at, total;       // unit that the first tile starts at, and of all
+    uint32_t ctas;            // CTAs that have work
     bool split;
 };
 
@@ -347,7 +366,7 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
         }
         b = lo;
         x = i - (lo ? ends[lo - 1] : 0);
-        return at_tile(seq_of(a, b), x, w.tile_tokens, a.window).n + AT_COST;
+        return at_tile(seq_of(a, b), x, w.tile_tokens, a.window, w.shift).n + w.cost;
     };
     uint64_t all = 0;
     uint32_t most = 0, b = 0, x = 0;
@@ -385,7 +404,7 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
             const uint64_t end = at + at_scan(n, sums, THREADS, sum), begin = end - n;
             const bool mine = n && (split ? begin <= u0 && u0 < end : begin >= u0 && begin < u1);
             if (split) {
-                if (mine) *out = AtPlan{h, b, x, (uint32_t)(u0 - begin), (int64_t)(u1 - u0), true};
+                if (mine) *out = AtPlan{h, b, x, (uint32_t)(u0 - begin), (int64_t)(u1 - u0), begin, total, (uint32_t)g, true};
                 found = __syncthreads_or(mine);
             } else {
                 // lowest index among the candidates
@@ -395,7 +414,7 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
                 __syncthreads();
                 uint32_t low = AT_NONE;
                 for (int j = 0; j < THREADS / 32; ++j) low = min(low, sums[j]);
-                if (mine && i == low) *out = AtPlan{h, b, x, 0, (int64_t)(u1 - begin), false};
+                if (mine && i == low) *out = AtPlan{h, b, x, 0, (int64_t)(u1 - begin), begin, total, (uint32_t)g, false};
                 found = low != AT_NONE;
                 __syncthreads();
             }
@@ -413,7 +432,9 @@ struct AtSeg {
     Seq s;
     int32_t lo, hi;     // the tile's keys
     int32_t p0;         // position of its first token
-    uint32_t k0, n;     // first key tile (in keys / 128) and how many
+    uint32_t k0, n;     // first key tile and how many
+    uint64_t at;        // unit that the tile starts at
+    uint32_t all;       // key tiles of the whole tile
 };
 struct AtWalk {
     AtPlan p;
@@ -439,19 +460,22 @@ struct AtWalk {
         g.b = p.b;
         g.x = p.x;
         g.s = s;
-        const AtTile t = at_tile(s, p.x, w.tile_tokens, a.window);
+        const AtTile t = at_tile(s, p.x, w.tile_tokens, a.window, w.shift);
         g.lo = t.lo;
         g.hi = t.hi;
         g.p0 = (int32_t)s.nkv - (int32_t)s.nq + (int32_t)(p.x * w.tile_tokens);
         // units [skip, skip + step) of the tile are these of its key tiles
-        const uint32_t all = t.n + AT_COST;
+        const uint32_t all = t.n + w.cost;
         const uint32_t step = p.split ? (uint32_t)min((int64_t)(all - p.skip), p.todo) : all;
-        const uint32_t from = max(p.skip, AT_COST) - AT_COST, to = max(p.skip + step, AT_COST) - AT_COST;
+        const uint32_t from = max(p.skip, w.cost) - w.cost, to = max(p.skip + step, w.cost) - w.cost;
         g.kind = from == 0 ? (to == t.n ? AT_FULL : AT_FIRST) : (to == t.n ? AT_LAST : AT_MIDDLE);
         g.k0 = t.t0 + from;
         g.n = to - from;
         // no key tile falls to this CTA: a neighbour has the tile, or it has none
         const bool none = t.n ? to == from : p.skip != 0;
+        g.at = p.at;
+        g.all = t.n;
+        p.at += all;
         p.todo -= step;
         p.skip = 0;
         ++p.x;
@@ -539,21 +563,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&small.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    // rows of q in no sequence
-    {
-        const uint32_t lo = (uint32_t)min(max(__ldg(a.starts), 0), (int32_t)a.tokens);
-        const uint32_t hi = (uint32_t)min(max(__ldg(a.starts + a.batch), 0), (int32_t)a.tokens);
-        const uint32_t n = lo + (a.tokens - max(hi, lo));
-        for (uint64_t i = (uint64_t)blockIdx.x * G::THREADS + tid; i < (uint64_t)n * a.heads * (D / 8);
-             i += (uint64_t)gridDim.x * G::THREADS) {
-            const uint32_t d = (uint32_t)(i % (D / 8)) * 8, h = (uint32_t)(i / (D / 8) % a.heads);
-            uint32_t tok = (uint32_t)(i / (D / 8) / a.heads);
-            if (tok >= lo) tok += max(hi, lo) - lo;
-            *reinterpret_cast<uint4*>(static_cast<T*>(a.out.data) + (int64_t)tok * a.out.ts + (int64_t)h * a.out.hs + d) =
-                make_uint4(0, 0, 0, 0);
-            if (a.lse && d == 0) a.lse[(uint64_t)tok * a.heads + h] = -INFINITY;
-        }
-    }
+    at_clear<T, D>(a, G::THREADS);
     at_make_plan<G::THREADS>(a, w, reinterpret_cast<uint32_t*>(sm), s_sums, &s_plan);
     at_fence_before();
     __syncthreads();
