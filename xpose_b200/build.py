@@ -13,6 +13,9 @@ LIB = os.path.join(HERE, "libxp_cuda.so")
 OBJ = os.path.join(HERE, "build")
 # one translation unit each, compiled side by side and linked into the library
 UNITS = [os.path.join(HERE, "csrc", f) for f in ("xp_cuda.cu", "serving.cu")]
+# torch tensors to the serving calls (CPython extension, linked to the library)
+BINDING = os.path.join(HERE, "csrc", "serving_torch.cpp")
+BINDING_LIB = os.path.join(HERE, "_serving.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc" if os.path.exists("/usr/local/cuda/bin/nvcc") else "nvcc")
 
 NVCC_FLAGS = [
@@ -64,6 +67,24 @@ def build_cuda(force=False, verbose=False):
     return LIB
 
 
+def build_binding(force=False, verbose=False):
+    if not force and not _stale(BINDING_LIB, [BINDING, os.path.join(ROOT, "include", "xp_cuda.h")]):
+        return BINDING_LIB
+    import sysconfig
+
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    inc = [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-o", BINDING_LIB, BINDING,
+           *[f"-I{d}" for d in inc], *[x for d in include_paths() for x in ("-isystem", d)],
+           "-L" + HERE, "-lxp_cuda", "-Wl,-rpath,$ORIGIN",
+           *[f"-L{d}" for d in library_paths()], "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    return BINDING_LIB
+
+
 def build_oracle(verbose=False):
     """The CPU checkers (test infrastructure): oracle/liboracle.so always,
     oracle/_ref/libxpref.so when the reference tree is present."""
@@ -76,6 +97,7 @@ def build_oracle(verbose=False):
 
 def main():
     build_cuda(force="--force" in sys.argv, verbose=True)
+    build_binding(force="--force" in sys.argv, verbose=True)
     build_oracle(verbose=True)
     print("built", LIB)
 

@@ -108,6 +108,13 @@ xp_status row_map(const char* who, CUtensorMap* m, bool is_bf16, void* data, uin
     return XP_OK;
 }
 
+// The attentions' scratch: counters and the error word; the row tiles' parts
+// (kinds, then sums); the few-row kernel's tickets and sums. The sums share
+// their room: a call uses one kind.
+constexpr size_t SCRATCH_HEADS = 256, SCRATCH_TICKETS = 8192, SCRATCH_TICKET_COUNT = 4096;
+constexpr size_t SCRATCH_SLOTS = SCRATCH_TICKETS + SCRATCH_TICKET_COUNT * 4;
+static_assert(SCRATCH_HEADS + 2 * AT_MAX_CTAS * 16 <= SCRATCH_TICKETS, "scratch");
+
 template <class T, class C, int W>
 xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, cudaStream_t st) {
     using G = AtCfg<T, C, W>;
@@ -119,15 +126,11 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
     const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count(), AT_MAX_CTAS);
     AtWork w{};
     w.slot_bytes = G::ROWS * (G::D * 4 + 8);
-    w.heads = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(scratch) + 256);
-    w.slots = static_cast<unsigned char*>(scratch) + 16384;
-    static_assert(256 + 2 * AT_MAX_CTAS * 16 <= 16384 &&
-                      16384 + 2ull * AT_MAX_CTAS * G::ROWS * (G::D * 4 + 8) <= XP_SERVING_SCRATCH_BYTES,
-                  "scratch");
+    w.heads = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(scratch) + SCRATCH_HEADS);
+    w.slots = static_cast<unsigned char*>(scratch) + SCRATCH_SLOTS;
+    static_assert(SCRATCH_SLOTS + 2ull * AT_MAX_CTAS * G::ROWS * (G::D * 4 + 8) <= XP_SERVING_SCRATCH_BYTES, "scratch");
     w.sub_tokens = 128 / a.group;
     w.tile_tokens = w.sub_tokens * G::NQ;
-    w.shift = AT_SHIFT;
-    w.cost = AT_COST;
     w.least_units = AT_COST + 2;
     w.split_over = AT_COST + 6;
     CUtensorMap qm{}, km{}, vm{};
@@ -171,23 +174,20 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
 template <class T, class C, int W, int NR>
 xp_status launch_few(const char* who, const ServeAttnArgs& a, void* scratch, cudaStream_t st) {
     using G = FwCfg<T, C, W, NR>;
-    static_assert(G::smem <= 227 * 1024, "shared memory");
+    constexpr size_t slot_bytes = 8 * NR * (G::D * 4 + 8);
+    static_assert(G::RING + AT_MAX_BATCH * 4 <= 227 * 1024, "shared memory");
     static std::atomic<bool> attr_set[kMaxDevices];
     auto kernel = attn_few_kernel<T, C, W, NR>;
-    if (cudaError_t e = smem_attr_once(attr_set, kernel, G::smem); e != cudaSuccess)
+    if (cudaError_t e = smem_attr_once(attr_set, kernel, G::RING + AT_MAX_BATCH * 4); e != cudaSuccess)
         return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
-    constexpr uint32_t most = 4 * AT_MAX_CTAS;
-    const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count() * G::CTAS, most);
-    AtWork w{};
-    w.slot_bytes = 8 * NR * (G::D * 4 + 8);
-    w.slots = static_cast<unsigned char*>(scratch) + 16384;
-    static_assert(256 + most * 4 <= 16384 && 16384 + 2ull * most * 8 * NR * (G::D * 4 + 8) <= XP_SERVING_SCRATCH_BYTES, "scratch");
-    w.tile_tokens = 16;  // all of a sequence's
-    w.shift = 6;
-    w.cost = 2;
-    w.least_units = 3;
-    w.split_over = 0;
-    kernel<<<ctas, 128, G::smem, st>>>(a, w, reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(scratch) + 16384 - most * 4));
+    unsigned char* const s = static_cast<unsigned char*>(scratch);
+    FwWork w{};
+    w.counters = reinterpret_cast<uint32_t*>(s + 128);
+    w.tickets = reinterpret_cast<uint32_t*>(s + SCRATCH_TICKETS);
+    w.slots = s + SCRATCH_SLOTS;
+    w.slot_bytes = slot_bytes;
+    w.most_slots = (uint32_t)std::min<size_t>(SCRATCH_TICKET_COUNT, (XP_SERVING_SCRATCH_BYTES - SCRATCH_SLOTS) / slot_bytes);
+    kernel<<<(uint32_t)sm_count() * G::CTAS, 128, G::RING + a.batch * 4, st>>>(a, w);
     return launched(who);
 }
 

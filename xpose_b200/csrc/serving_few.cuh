@@ -11,10 +11,11 @@
 // transposing register move. Scores of 8-bit caches, the running maximum and
 // non-finite values of v are as in the tile kernel.
 //
-// The four warps of a CTA take the keys of a unit of 64 in turn and add their
-// sums in shared memory; CTAs have equal shares of all units, whatever the
-// lengths, and of a sequence that several share the last to finish adds the
-// parts, in their order.
+// The four warps of a CTA take 16 keys each of a unit of 64 and add their sums
+// in shared memory. Long sequences are cut into chunks of units, about four
+// for every CTA on the GPU, which the CTAs take as they get free: SMs do not
+// read at the same speed, and equal shares left the slow ones a fifth behind.
+// The last CTA of a sequence to finish adds its chunks, in their order.
 #pragma once
 #include "serving_tile.cuh"
 
@@ -25,11 +26,11 @@ template <class T, class C, int W, int NR> struct FwCfg {
     static constexpr bool Q8 = sizeof(C) == 1;
     static constexpr int RB = D * (int)sizeof(C);            // bytes of a row
     static constexpr int STAGE = 2 * 16 * RB + (Q8 ? 128 : 0);  // 16 keys: K, V, scales
-    static constexpr int NST = STAGE > 8500 ? 2 : STAGE > 4300 ? 3 : STAGE > 2200 ? 3 : 6;
+    static constexpr int NST = STAGE > 2200 ? 3 : 6;         // stages of a warp's ring
     static constexpr int MERGE = 4 * 8 * NR * (D + 4) * 4;   // the warps' sums, and their m and l
     static constexpr int RING = 4 * NST * STAGE > MERGE ? 4 * NST * STAGE : MERGE;
-    static constexpr int smem = RING > AT_MAX_BATCH * 4 ? RING : AT_MAX_BATCH * 4;
-    static constexpr int CTAS = smem > 116000 ? 1 : smem > 76000 || W * NR > 4 ? 2 : W == 4 ? 3 : 4;  // of an SM
+    static constexpr int SMEM1 = RING + 512;                 // + a word a sequence
+    static constexpr int CTAS = SMEM1 > 113000 ? 1 : SMEM1 > 75000 || W * NR > 4 ? 2 : W * NR == 4 ? 3 : 4;  // of an SM
 };
 
 XP_DEV void fw_cp16(uint32_t dst, const void* src, bool has) {
@@ -67,64 +68,101 @@ template <int RB> XP_DEV uint32_t fw_at(uint32_t r, uint32_t c) {
     else return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ (r >> 1)) & 7) * 16;
 }
 
+struct FwWork {
+    unsigned char* slots;    // partial sums of the chunks of split sequences, by item
+    uint32_t* tickets;       // by item: chunks of the sequence that starts there that are done
+    uint32_t* counters;      // [0] items taken beyond the first of every CTA, [1] CTAs that ended
+    uint32_t slot_bytes, most_slots;
+};
+
+// An item: chunk c of n of head h of sequence b; items are numbered by head,
+// sequence, chunk. Whatever the lengths, the same on every CTA.
+struct FwPlan {
+    uint32_t per_head, chunk;  // items a head, units a chunk
+};
+// `ends`: a word a sequence, where its items end. A sequence without new
+// tokens has none; one without keys has one.
+XP_DEV FwPlan fw_make_plan(const ServeAttnArgs& a, const FwWork& w, uint32_t* ends, uint32_t* sums) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t n = 0;
+    auto units_of = [&](uint32_t b) -> uint32_t {  // 0: no items
+        if (b >= a.batch) return 0;
+        const Seq s = seq_of(a, b);
+        return s.nq ? max(at_tile(s, 0, 16, a.window, 6).n, 1u) : 0u;
+    };
+    uint64_t all = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 128) {
+        n = units_of(b0 + tid);
+        uint32_t sum;
+        at_scan(n, sums, 128, sum);
+        all += sum;
+    }
+    // one chunk a CTA while there is at most a few units for each, else four
+    all *= a.kv_heads;
+    const uint64_t ctas = gridDim.x;
+    uint64_t chunk = all <= 8 * ctas ? (all + ctas - 1) / ctas : (all + 4 * ctas - 1) / (4 * ctas);
+    chunk = max(chunk, (uint64_t)1);
+    FwPlan p;
+    for (;;) {
+        p.chunk = (uint32_t)min(chunk, (uint64_t)0x7FFFFFFF);
+        uint32_t items = 0;
+        for (uint32_t b0 = 0; b0 < a.batch; b0 += 128) {
+            if (a.batch > 128) n = units_of(b0 + tid);
+            uint32_t sum;
+            const uint32_t end = items + at_scan(n ? (n - 1) / p.chunk + 1 : 0, sums, 128, sum);
+            if (b0 + tid < a.batch) ends[b0 + tid] = end;
+            items += sum;
+        }
+        p.per_head = items;
+        // more items than partial sums have room for: so many sequences need no cut
+        if ((uint64_t)items * a.kv_heads <= w.most_slots || p.chunk == 0x7FFFFFFF) break;
+        chunk = 0x7FFFFFFF;
+        __syncthreads();
+    }
+    __syncthreads();
+    return p;
+}
+
 template <class T, class C, int W, int NR>
 __global__ void __launch_bounds__(128, (FwCfg<T, C, W, NR>::CTAS))
-attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ AtWork w, uint32_t* tickets) {
+attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ FwWork w) {
     using G = FwCfg<T, C, W, NR>;
     constexpr int D = G::D, RB = G::RB, NST = G::NST, KS = D / 16, ROWS = 8 * NR;
     constexpr bool Q8 = G::Q8;
-    extern __shared__ __align__(1024) unsigned char sm[];
-    __shared__ AtPlan s_plan;
-    __shared__ uint32_t s_sums[32], s_last;
+    extern __shared__ __align__(128) unsigned char sm[];
+    __shared__ uint32_t s_sums[32], s_last, s_next;
+    uint32_t* const ends = reinterpret_cast<uint32_t*>(sm + G::RING);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lg = lane >> 2, lq = lane & 3;
     const uint32_t ring = smem_u32(sm) + warp * (NST * G::STAGE);
-    at_clear<T, D>(a, 128);
-    at_make_plan<128>(a, w, reinterpret_cast<uint32_t*>(sm), s_sums, &s_plan);
-    __syncthreads();
-    AtWalk walk;
-    walk.start(s_plan);
-    AtSeg g;
-    while (walk.next(a, w, g)) {
-        // this lane's rows: 8 i + lg as a row of Q, 8 i + 2 lq and the next as columns of S^T and O^T
-        const int32_t first = (int32_t)g.s.nkv - (int32_t)g.s.nq;
-        const uint32_t nrows = g.s.nq * a.group;
-        uint32_t qf[KS][NR][2];
-#pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const uint32_t r = 8 * i + lg, tok = r / a.group, h = g.h * a.group + (r - tok * a.group);
-            const T* qp = static_cast<const T*>(a.q.data) + (int64_t)(g.s.q0 + tok) * a.q.ts + (int64_t)h * a.q.hs;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                // the values that stand where the codes of a key's word stand (8-bit), or in order
-                qf[s][i][0] = qf[s][i][1] = 0;
-                if (r < nrows) {
-                    qf[s][i][0] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + (Q8 ? 4 * lq : 2 * lq)));
-                    qf[s][i][1] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + (Q8 ? 4 * lq + 2 : 2 * lq + 8)));
-                }
+    const FwPlan plan = fw_make_plan(a, w, ends, s_sums);
+    const uint32_t items = plan.per_head * a.kv_heads;
+    struct {
+        uint32_t h, b, k0, n;  // head, sequence, first unit and how many
+        int32_t lo, hi;        // the sequence's keys
+        Seq s;
+    } g;
+    for (uint32_t item = blockIdx.x; item < items; item = s_next) {
+        __syncthreads();
+        if (tid == 0) s_next = gridDim.x + atomicAdd(w.counters, 1u);
+        g.h = item / plan.per_head;
+        const uint32_t in_head = item - g.h * plan.per_head;
+        {
+            uint32_t x = 0, y = a.batch - 1;
+            while (x < y) {
+                const uint32_t mid = (x + y) / 2;
+                if (ends[mid] > in_head) y = mid;
+                else x = mid + 1;
             }
+            g.b = x;
         }
-        int32_t klo[NR][2], khi[NR][2];
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t r = 8 * i + 2 * lq + j;
-                const int32_t pos = first + (int32_t)(r / a.group);
-                khi[i][j] = r < nrows ? max(pos + 1, 0) : 0x7FFFFFFF;
-                klo[i][j] = r < nrows && a.window ? (int32_t)max((int64_t)pos + 1 - (int64_t)a.window, (int64_t)0) : 0;
-            }
-        float o[KS][NR][4], m[NR][2], ref[NR][2], l[NR][2];
-#pragma unroll
-        for (int i = 0; i < NR; ++i) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                m[i][j] = -INFINITY;
-                ref[i][j] = l[i][j] = 0.0f;
-            }
-#pragma unroll
-            for (int d = 0; d < KS; ++d)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[d][i][j] = 0.0f;
+        const uint32_t begin = g.b ? ends[g.b - 1] : 0, nch = ends[g.b] - begin, ch = in_head - begin;
+        g.s = seq_of(a, g.b);
+        {
+            const AtTile t = at_tile(g.s, 0, 16, a.window, 6);
+            g.lo = t.lo;
+            g.hi = t.hi;
+            g.k0 = t.t0 + ch * plan.chunk;
+            g.n = t.n ? min(plan.chunk, t.n - ch * plan.chunk) : 0;
         }
         // ---- the ring ----
         const int32_t lo = g.lo, hi = g.hi;
@@ -167,6 +205,47 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
         };
 #pragma unroll 1
         for (uint32_t u = 0; u < (uint32_t)NST - 1; ++u) issue(u);
+        // this lane's rows: 8 i + lg as a row of Q, 8 i + 2 lq and the next as columns of S^T and O^T
+        const int32_t first = (int32_t)g.s.nkv - (int32_t)g.s.nq;
+        const uint32_t nrows = g.s.nq * a.group;
+        uint32_t qf[KS][NR][2];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const uint32_t r = 8 * i + lg, tok = r / a.group, h = g.h * a.group + (r - tok * a.group);
+            const T* qp = static_cast<const T*>(a.q.data) + (int64_t)(g.s.q0 + tok) * a.q.ts + (int64_t)h * a.q.hs;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                // the values that stand where the codes of a key's word stand (8-bit), or in order
+                qf[s][i][0] = qf[s][i][1] = 0;
+                if (r < nrows) {
+                    qf[s][i][0] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + (Q8 ? 4 * lq : 2 * lq)));
+                    qf[s][i][1] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + (Q8 ? 4 * lq + 2 : 2 * lq + 8)));
+                }
+            }
+        }
+        int32_t klo[NR][2], khi[NR][2];
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t r = 8 * i + 2 * lq + j;
+                const int32_t pos = first + (int32_t)(r / a.group);
+                khi[i][j] = r < nrows ? max(pos + 1, 0) : 0x7FFFFFFF;
+                klo[i][j] = r < nrows && a.window ? (int32_t)max((int64_t)pos + 1 - (int64_t)a.window, (int64_t)0) : 0;
+            }
+        float o[KS][NR][4], m[NR][2], ref[NR][2], l[NR][2];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                m[i][j] = -INFINITY;
+                ref[i][j] = l[i][j] = 0.0f;
+            }
+#pragma unroll
+            for (int d = 0; d < KS; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[d][i][j] = 0.0f;
+        }
 #pragma unroll 1
         for (uint32_t u = 0; u < g.n; ++u) {
             asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
@@ -366,9 +445,8 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 }
             }
         __syncthreads();
-        const bool whole = g.kind == AT_FULL;
-        const uint32_t slot = 2 * blockIdx.x + (g.kind == AT_FIRST ? 1 : 0);
-        unsigned char* const part = w.slots + (size_t)slot * w.slot_bytes;
+        const bool whole = nch == 1;
+        unsigned char* const part = w.slots + (size_t)item * w.slot_bytes;
         auto emit = [&](uint32_t r, uint32_t c, float4 x, float mm, float ll) {
             const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
             const uint32_t tok = r / a.group, h = g.h * a.group + (r - tok * a.group);
@@ -409,45 +487,82 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
             }
         }
         if (!whole) {
-            // the CTAs that have this sequence: those of its first and last unit, and all between
-            const uint64_t u0 = g.at + w.cost, u1 = u0 + g.all - 1, total = s_plan.total, n = s_plan.ctas;
-            const uint32_t c0 = (uint32_t)(((u0 + 1) * n + total - 1) / total - 1);
-            const uint32_t c1 = (uint32_t)(((u1 + 1) * n + total - 1) / total - 1);
+            const uint32_t item0 = item - ch;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                s_last = atomicAdd(tickets + c0, 1u) == c1 - c0;
-                if (s_last) tickets[c0] = 0;
+                s_last = atomicAdd(w.tickets + item0, 1u) == nch - 1;
+                if (s_last) w.tickets[item0] = 0;
             }
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                auto part_of = [&](uint32_t c) { return w.slots + (size_t)(c == c0 ? 2 * c + 1 : 2 * c) * w.slot_bytes; };
-                for (uint32_t id = tid; id < nrows * (D / 4); id += 128) {
-                    const uint32_t r = id / (D / 4), c = id % (D / 4);
-                    float mm = -INFINITY, ll = 0.0f;
-#pragma unroll 8
-                    for (uint32_t i = c0; i <= c1; ++i) {
-                        const float2 v = __ldcg(reinterpret_cast<const float2*>(part_of(i) + (size_t)ROWS * D * 4) + r);
-                        if (v.y != 0.0f) mm = fmaxf(mm, v.x);
+                // 64 parts at a time: their m and l in shared memory, then the sums
+                const unsigned char* const parts = w.slots + (size_t)item0 * w.slot_bytes;
+                float2* const ml = reinterpret_cast<float2*>(sm);  // [64][ROWS]
+                constexpr uint32_t PER = (ROWS * (D / 4) + 127) / 128;  // of a thread
+                float4 x[PER];
+                float mm[PER], ll[PER];
+#pragma unroll
+                for (uint32_t k = 0; k < PER; ++k) {
+                    x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    mm[k] = -INFINITY;
+                    ll[k] = 0.0f;
+                }
+                for (uint32_t i0 = 0; i0 < nch; i0 += 64) {
+                    const uint32_t m = min(nch - i0, 64u);
+                    __syncthreads();
+                    for (uint32_t i = tid; i < m * ROWS; i += 128) {
+                        const uint32_t r = i % ROWS;
+                        ml[i] = r < nrows ? __ldcg(reinterpret_cast<const float2*>(parts + (size_t)(i0 + i / ROWS) * w.slot_bytes +
+                                                                                   (size_t)ROWS * D * 4) + r)
+                                          : make_float2(0.0f, 0.0f);
                     }
-                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    __syncthreads();
+#pragma unroll
+                    for (uint32_t k = 0; k < PER; ++k) {
+                        const uint32_t id = tid + k * 128, r = id / (D / 4);
+                        if (r >= nrows) continue;
+                        float top = mm[k];
+                        for (uint32_t i = 0; i < m; ++i) {
+                            const float2 v = ml[i * ROWS + r];
+                            if (v.y != 0.0f) top = fmaxf(top, v.x);
+                        }
+                        const float f0 = mm[k] == -INFINITY ? 0.0f : at_ex2(mm[k] - top);
+                        mm[k] = top;
+                        ll[k] *= f0;
+                        x[k].x *= f0;
+                        x[k].y *= f0;
+                        x[k].z *= f0;
+                        x[k].w *= f0;
+                        const unsigned char* p = parts + (size_t)i0 * w.slot_bytes + (size_t)id * 16;
 #pragma unroll 8
-                    for (uint32_t i = c0; i <= c1; ++i) {
-                        const float2 v = __ldcg(reinterpret_cast<const float2*>(part_of(i) + (size_t)ROWS * D * 4) + r);
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part_of(i)) + id);
-                        const float f = v.y != 0.0f ? at_ex2(v.x - mm) : 0.0f;
-                        ll += f * v.y;
-                        x.x += f * y.x;
-                        x.y += f * y.y;
-                        x.z += f * y.z;
-                        x.w += f * y.w;
+                        for (uint32_t i = 0; i < m; ++i, p += w.slot_bytes) {
+                            const float4 y = __ldcg(reinterpret_cast<const float4*>(p));
+                            const float2 v = ml[i * ROWS + r];
+                            const float f = v.y != 0.0f ? at_ex2(v.x - top) : 0.0f;
+                            ll[k] = fmaf(f, v.y, ll[k]);
+                            x[k].x = fmaf(f, y.x, x[k].x);
+                            x[k].y = fmaf(f, y.y, x[k].y);
+                            x[k].z = fmaf(f, y.z, x[k].z);
+                            x[k].w = fmaf(f, y.w, x[k].w);
+                        }
                     }
-                    emit(r, c, x, mm, ll);
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < PER; ++k) {
+                    const uint32_t id = tid + k * 128, r = id / (D / 4);
+                    if (r < nrows) emit(r, id % (D / 4), x[k], mm[k], ll[k]);
                 }
             }
         }
         __syncthreads();
+    }
+    at_clear<T, D>(a, 128);
+    // the last CTA leaves the counters as it found them
+    if (tid == 0 && atomicAdd(w.counters + 1, 1u) == gridDim.x - 1) {
+        w.counters[0] = 0;
+        w.counters[1] = 0;
     }
 }
 

@@ -80,7 +80,6 @@ struct AtWork {
     uint32_t head_step;     // packed: k and v heads a kv head apart in the tensor maps (0: one for all)
     uint32_t tile_tokens;   // tokens of a tile
     uint32_t sub_tokens;    // tokens of one of its NQ row tiles
-    uint32_t shift, cost;   // log2 of the keys of a key tile; what a tile costs besides them, in key tiles
     uint32_t least_units;   // units of a CTA, at least
     uint32_t split_over;    // whole tiles while none has more units, or more than an eighth of a CTA's
 };
@@ -311,12 +310,10 @@ template <class T, int D> XP_DEV void at_clear(const ServeAttnArgs& a, uint32_t 
 }
 
 // Where a CTA starts in the list of units: head h, sequence b, tile x. A tile
-// counts as its key tiles and `cost` more, which come first.
+// counts as its key tiles and AT_COST more, which come first.
 struct AtPlan {
     uint32_t h, b, x, skip;   // skip: units of the first tile that earlier CTAs have
     int64_t todo;             // units from there; whole tiles: those that start within them
-    uint64_t at, total;       // unit that the first tile starts at, and of all
-    uint32_t ctas;            // CTAs that have work
     bool split;
 };
 
@@ -366,7 +363,7 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
         }
         b = lo;
         x = i - (lo ? ends[lo - 1] : 0);
-        return at_tile(seq_of(a, b), x, w.tile_tokens, a.window, w.shift).n + w.cost;
+        return at_tile(seq_of(a, b), x, w.tile_tokens, a.window, AT_SHIFT).n + AT_COST;
     };
     uint64_t all = 0;
     uint32_t most = 0, b = 0, x = 0;
@@ -404,7 +401,7 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
             const uint64_t end = at + at_scan(n, sums, THREADS, sum), begin = end - n;
             const bool mine = n && (split ? begin <= u0 && u0 < end : begin >= u0 && begin < u1);
             if (split) {
-                if (mine) *out = AtPlan{h, b, x, (uint32_t)(u0 - begin), (int64_t)(u1 - u0), begin, total, (uint32_t)g, true};
+                if (mine) *out = AtPlan{h, b, x, (uint32_t)(u0 - begin), (int64_t)(u1 - u0), true};
                 found = __syncthreads_or(mine);
             } else {
                 // lowest index among the candidates
@@ -414,7 +411,7 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
                 __syncthreads();
                 uint32_t low = AT_NONE;
                 for (int j = 0; j < THREADS / 32; ++j) low = min(low, sums[j]);
-                if (mine && i == low) *out = AtPlan{h, b, x, 0, (int64_t)(u1 - begin), begin, total, (uint32_t)g, false};
+                if (mine && i == low) *out = AtPlan{h, b, x, 0, (int64_t)(u1 - begin), false};
                 found = low != AT_NONE;
                 __syncthreads();
             }
@@ -433,8 +430,6 @@ struct AtSeg {
     int32_t lo, hi;     // the tile's keys
     int32_t p0;         // position of its first token
     uint32_t k0, n;     // first key tile and how many
-    uint64_t at;        // unit that the tile starts at
-    uint32_t all;       // key tiles of the whole tile
 };
 struct AtWalk {
     AtPlan p;
@@ -460,22 +455,19 @@ struct AtWalk {
         g.b = p.b;
         g.x = p.x;
         g.s = s;
-        const AtTile t = at_tile(s, p.x, w.tile_tokens, a.window, w.shift);
+        const AtTile t = at_tile(s, p.x, w.tile_tokens, a.window, AT_SHIFT);
         g.lo = t.lo;
         g.hi = t.hi;
         g.p0 = (int32_t)s.nkv - (int32_t)s.nq + (int32_t)(p.x * w.tile_tokens);
         // units [skip, skip + step) of the tile are these of its key tiles
-        const uint32_t all = t.n + w.cost;
+        const uint32_t all = t.n + AT_COST;
         const uint32_t step = p.split ? (uint32_t)min((int64_t)(all - p.skip), p.todo) : all;
-        const uint32_t from = max(p.skip, w.cost) - w.cost, to = max(p.skip + step, w.cost) - w.cost;
+        const uint32_t from = max(p.skip, AT_COST) - AT_COST, to = max(p.skip + step, AT_COST) - AT_COST;
         g.kind = from == 0 ? (to == t.n ? AT_FULL : AT_FIRST) : (to == t.n ? AT_LAST : AT_MIDDLE);
         g.k0 = t.t0 + from;
         g.n = to - from;
         // no key tile falls to this CTA: a neighbour has the tile, or it has none
         const bool none = t.n ? to == from : p.skip != 0;
-        g.at = p.at;
-        g.all = t.n;
-        p.at += all;
         p.todo -= step;
         p.skip = 0;
         ++p.x;
