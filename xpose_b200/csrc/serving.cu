@@ -175,10 +175,10 @@ template <class T, class C, int W, int NR>
 xp_status launch_few(const char* who, const ServeAttnArgs& a, void* scratch, cudaStream_t st) {
     using G = FwCfg<T, C, W, NR>;
     constexpr size_t slot_bytes = 8 * NR * (G::D * 4 + 8);
-    static_assert(G::RING + AT_MAX_BATCH * 4 <= 227 * 1024, "shared memory");
+    static_assert(G::ends_off + AT_MAX_BATCH * 4 <= 227 * 1024, "shared memory");
     static std::atomic<bool> attr_set[kMaxDevices];
     auto kernel = attn_few_kernel<T, C, W, NR>;
-    if (cudaError_t e = smem_attr_once(attr_set, kernel, G::RING + AT_MAX_BATCH * 4); e != cudaSuccess)
+    if (cudaError_t e = smem_attr_once(attr_set, kernel, G::ends_off + AT_MAX_BATCH * 4); e != cudaSuccess)
         return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     unsigned char* const s = static_cast<unsigned char*>(scratch);
     FwWork w{};
@@ -187,7 +187,7 @@ xp_status launch_few(const char* who, const ServeAttnArgs& a, void* scratch, cud
     w.slots = s + SCRATCH_SLOTS;
     w.slot_bytes = slot_bytes;
     w.most_slots = (uint32_t)std::min<size_t>(SCRATCH_TICKET_COUNT, (XP_SERVING_SCRATCH_BYTES - SCRATCH_SLOTS) / slot_bytes);
-    kernel<<<(uint32_t)sm_count() * G::CTAS, 128, G::RING + a.batch * 4, st>>>(a, w);
+    kernel<<<(uint32_t)sm_count() * G::CTAS, 128, G::ends_off + a.batch * 4, st>>>(a, w);
     return launched(who);
 }
 
