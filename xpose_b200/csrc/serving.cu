@@ -93,25 +93,25 @@ PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
     }();
     return f;
 }
-// 16-bit rows as boxes of 64 values x `rows` rows, 128-byte swizzled.
-// Packed: [tokens][heads][dim], rows along tokens; paged: [pages * heads][page][dim].
-xp_status row_map(const char* who, CUtensorMap* m, bool is_bf16, void* data, uint64_t dim, const uint64_t (&n)[2],
-                  const uint64_t (&stride)[2], const uint32_t (&box)[2]) {
+// Rows as boxes of `width` bytes x rows, swizzled by that width. Packed:
+// [tokens][heads][dim], rows along tokens; paged: [pages * heads][page][dim].
+xp_status row_map(const char* who, CUtensorMap* m, CUtensorMapDataType type, uint32_t width, uint32_t size, void* data,
+                  uint64_t dim, const uint64_t (&n)[2], const uint64_t (&stride)[2], const uint32_t (&box)[2]) {
     const auto encode = map_encoder();
     if (!encode) return fail(XP_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available", who);
     const cuuint64_t dims[3] = {dim, n[0], n[1]}, strides[2] = {stride[0], stride[1]};
-    const cuuint32_t boxes[3] = {64, box[0], box[1]}, ones[3] = {1, 1, 1};
-    const CUresult r = encode(m, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, data,
-                              dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint32_t boxes[3] = {width / size, box[0], box[1]}, ones[3] = {1, 1, 1};
+    const CUresult r = encode(m, type, 3, data, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(XP_ERR_INVALID, "%s: the rows do not fit a tensor map (%d)", who, (int)r);
     return XP_OK;
 }
 
-// The attentions' scratch: counters and the error word; the row tiles' parts
+// The attentions' scratch: the error word; the row tiles' parts
 // (kinds, then sums); the few-row kernel's tickets and sums. The sums share
 // their room: a call uses one kind.
-constexpr size_t SCRATCH_HEADS = 256, SCRATCH_TICKETS = 8192, SCRATCH_TICKET_COUNT = 4096;
+constexpr size_t SCRATCH_HEADS = 256, SCRATCH_TICKETS = 8192, SCRATCH_TICKET_COUNT = 1024;
 constexpr size_t SCRATCH_SLOTS = SCRATCH_TICKETS + SCRATCH_TICKET_COUNT * 4;
 static_assert(SCRATCH_HEADS + 2 * AT_MAX_CTAS * 16 <= SCRATCH_TICKETS, "scratch");
 
@@ -134,12 +134,13 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
     w.least_units = AT_COST + 2;
     w.split_over = AT_COST + 6;
     CUtensorMap qm{}, km{}, vm{};
-    const bool b = std::is_same_v<T, bf16>;
+    const CUtensorMapDataType type =
+        std::is_same_v<T, bf16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     {
         const uint64_t n[2] = {a.heads, a.tokens};
         const uint64_t stride[2] = {a.heads > 1 ? (uint64_t)a.q.hs * 2 : G::D * 2, a.tokens > 1 ? (uint64_t)a.q.ts * 2 : G::D * 2};
         const uint32_t box[2] = {a.group, w.sub_tokens};
-        TRY(row_map(who, &qm, b, a.q.data, G::D, n, stride, box));
+        TRY(row_map(who, &qm, type, 128, 2, a.q.data, G::D, n, stride, box));
     }
     if constexpr (!G::Q8) {
         if (a.pages.k) {
@@ -147,8 +148,8 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
             const uint64_t n[2] = {ps, (a.pages.slots >> a.pages.page_shift) * a.kv_heads};
             const uint64_t stride[2] = {G::D * 2, (uint64_t)ps * G::D * 2};
             const uint32_t kbox[2] = {std::min<uint32_t>(ps, AT_KEYS), 1}, vbox[2] = {std::min<uint32_t>(ps, G::VKEYS), 1};
-            TRY(row_map(who, &km, b, a.pages.k, G::D, n, stride, kbox));
-            TRY(row_map(who, &vm, b, a.pages.v, G::D, n, stride, vbox));
+            TRY(row_map(who, &km, type, 128, 2, a.pages.k, G::D, n, stride, kbox));
+            TRY(row_map(who, &vm, type, 128, 2, a.pages.v, G::D, n, stride, vbox));
         } else {
             // a lone head or token has no stride of its own; one head for all (stride 0) is a lone head
             w.head_step = 1;
@@ -160,8 +161,8 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
             const uint32_t kbox[2] = {1, AT_KEYS}, vbox[2] = {1, G::VKEYS};
             const uint64_t ks[2] = {mh > 1 ? (uint64_t)a.k.hs * 2 : G::D * 2, a.tokens > 1 ? (uint64_t)a.k.ts * 2 : G::D * 2};
             const uint64_t vs[2] = {mh > 1 ? (uint64_t)a.v.hs * 2 : G::D * 2, a.tokens > 1 ? (uint64_t)a.v.ts * 2 : G::D * 2};
-            TRY(row_map(who, &km, b, a.k.data, G::D, n, ks, kbox));
-            TRY(row_map(who, &vm, b, a.v.data, G::D, n, vs, vbox));
+            TRY(row_map(who, &km, type, 128, 2, a.k.data, G::D, n, ks, kbox));
+            TRY(row_map(who, &vm, type, 128, 2, a.v.data, G::D, n, vs, vbox));
         }
     }
     cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, false, a, w, qm, km, vm);
@@ -175,19 +176,30 @@ template <class T, class C, int W, int NR>
 xp_status launch_few(const char* who, const ServeAttnArgs& a, void* scratch, cudaStream_t st) {
     using G = FwCfg<T, C, W, NR>;
     constexpr size_t slot_bytes = 8 * NR * (G::D * 4 + 8);
-    static_assert(G::ends_off + AT_MAX_BATCH * 4 <= 227 * 1024, "shared memory");
+    static_assert(G::BYTES <= 227 * 1024, "shared memory");
+    constexpr uint32_t most = 4 * AT_MAX_CTAS;
+    static_assert(most <= SCRATCH_TICKET_COUNT && SCRATCH_SLOTS + 2 * most * slot_bytes <= XP_SERVING_SCRATCH_BYTES, "scratch");
     static std::atomic<bool> attr_set[kMaxDevices];
     auto kernel = attn_few_kernel<T, C, W, NR>;
-    if (cudaError_t e = smem_attr_once(attr_set, kernel, G::ends_off + AT_MAX_BATCH * 4); e != cudaSuccess)
+    if (cudaError_t e = smem_attr_once(attr_set, kernel, G::smem); e != cudaSuccess)
         return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     unsigned char* const s = static_cast<unsigned char*>(scratch);
     FwWork w{};
-    w.counters = reinterpret_cast<uint32_t*>(s + 128);
     w.tickets = reinterpret_cast<uint32_t*>(s + SCRATCH_TICKETS);
     w.slots = s + SCRATCH_SLOTS;
     w.slot_bytes = slot_bytes;
-    w.most_slots = (uint32_t)std::min<size_t>(SCRATCH_TICKET_COUNT, (XP_SERVING_SCRATCH_BYTES - SCRATCH_SLOTS) / slot_bytes);
-    kernel<<<(uint32_t)sm_count() * G::CTAS, 128, G::ends_off + a.batch * 4, st>>>(a, w);
+    CUtensorMap km, vm;
+    const uint32_t ps = 1u << a.pages.page_shift;
+    const uint64_t n[2] = {ps, (a.pages.slots >> a.pages.page_shift) * a.kv_heads};
+    const uint64_t stride[2] = {G::RB, (uint64_t)ps * G::RB};
+    const uint32_t box[2] = {std::min<uint32_t>(ps, G::KPS), 1};
+    const CUtensorMapDataType type = G::Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : std::is_same_v<T, bf16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    TRY(row_map(who, &km, type, G::RB < 128 ? 64 : 128, sizeof(C), a.pages.k, G::D, n, stride, box));
+    TRY(row_map(who, &vm, type, G::RB < 128 ? 64 : 128, sizeof(C), a.pages.v, G::D, n, stride, box));
+    const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count() * G::CTAS, most);
+    kernel<<<ctas, 128, G::smem, st>>>(a, w, km, vm);
     return launched(who);
 }
 

@@ -5,17 +5,18 @@
 // of reading the cache. The products are warp-wide mma.sync with the keys as
 // the long side, S^T = K Q^T and O^T = V^T P^T: 8 * NR rows are its narrow
 // side, where the 128-row tiles of tcgen05 would be nearly empty. A warp takes
-// 16 keys at a time from a ring of its own in shared memory (cp.async; keys
-// outside the range are zeros), 8-bit codes become exact 16-bit values in
-// registers, and P moves from one product's layout to the other's by a
-// transposing register move. Scores of 8-bit caches, the running maximum and
-// non-finite values of v are as in the tile kernel.
+// 16 or 32 keys at a time from a ring of its own in shared memory, which TMA
+// fills by pages in the swizzled layout that ldmatrix reads without conflicts;
+// 8-bit codes become exact 16-bit values in registers, and P moves from one
+// product's layout to the other's by a transposing register move. Scores of
+// 8-bit caches, the running maximum and non-finite values of v are as in the
+// tile kernel.
 //
-// The four warps of a CTA take 16 keys each of a unit of 64 and add their sums
-// in shared memory. Long sequences are cut into chunks of units, about four
-// for every CTA on the GPU, which the CTAs take as they get free: SMs do not
-// read at the same speed, and equal shares left the slow ones a fifth behind.
-// The last CTA of a sequence to finish adds its chunks, in their order.
+// The four warps of a CTA take a step each of a unit of four and add their
+// sums in shared memory. CTAs have equal shares of the units of all sequences
+// and heads, laid end to end; of a sequence that several share the last to
+// finish adds the parts, in their order. (Chunks that CTAs take as they get free
+// measured slower: adding the sums of a chunk costs as much as eight units.)
 #pragma once
 #include "serving_tile.cuh"
 
@@ -25,15 +26,19 @@ template <class T, class C, int W, int NR> struct FwCfg {
     static constexpr int D = 64 * W;
     static constexpr bool Q8 = sizeof(C) == 1;
     static constexpr int RB = D * (int)sizeof(C);            // bytes of a row
-    static constexpr int STAGE = 2 * 16 * RB + (Q8 ? 128 : 0);  // 16 keys: K, V, scales
-    static constexpr int NST = STAGE > 4100 ? 2 : STAGE > 2200 ? 3 : 4;  // stages of a warp's ring
+    static constexpr int KPS = RB <= 128 ? 32 : 16;          // keys of a warp's step
+    static constexpr int UNIT = 4 * KPS;                     // keys of a unit
+    static constexpr int SHIFT = KPS == 32 ? 7 : 6;          // log2 UNIT
+    static constexpr int HALF = KPS * RB;                    // K of a step, or V
+    static constexpr int NST = HALF > 4096 ? 2 : HALF > 2048 ? 2 : 3;  // steps of a warp's ring
     // two warps' sums at a time, with their m and l; the queries of two items
-    static constexpr int ring_bytes = 4 * NST * STAGE;
-    static constexpr int sum_off = ring_bytes, sum_bytes = 2 * 8 * NR * (D + 2) * 4;
+    static constexpr int ring_bytes = 4 * NST * 2 * HALF;
+    static constexpr int scale_off = ring_bytes, scale_bytes = Q8 ? 4 * NST * 2 * KPS * 4 : 0;
+    static constexpr int sum_off = scale_off + scale_bytes, sum_bytes = 2 * 8 * NR * (D + 2) * 4;
     static constexpr int q_off = sum_off + sum_bytes, q_bytes = 8 * NR * D * 2;
-    static constexpr int ends_off = q_off + 2 * q_bytes;     // a word a sequence
-    static constexpr int BYTES = ends_off + 1024;            // ... of 128 sequences, and static
-    static constexpr int CTAS = BYTES > 115000 ? 1 : BYTES > 76000 || W * NR > 4 ? 2 : BYTES > 57500 || W * NR == 4 ? 3 : 4;
+    static constexpr int smem = q_off + 2 * q_bytes;
+    static constexpr int BYTES = smem + 2048;                // with static data and what the system keeps
+    static constexpr int CTAS = BYTES > 115000 ? 1 : BYTES > 76000 || W * NR > 4 ? 2 : BYTES > 57000 || W * NR == 4 ? 3 : 4;
 };
 
 XP_DEV void fw_cp16(uint32_t dst, const void* src, bool has) {
@@ -74,157 +79,191 @@ XP_DEV uint2 fw_codes_t(uint32_t w, int8c) {
     return make_uint2(reinterpret_cast<const uint32_t&>(x), reinterpret_cast<const uint32_t&>(y));
 }
 XP_DEV uint2 fw_codes_t(uint32_t w, fp8c) { return at_codes<__half>(__byte_perm(w, 0, 0x3120), fp8c{}); }
-// where 16 bytes c of row r of a stage lie: eight rows' equal chunks in eight bank groups
-template <int RB> XP_DEV uint32_t fw_at(uint32_t r, uint32_t c) {
-    if constexpr (RB >= 128) return r * RB + ((c & ~7u) << 4) + (((c ^ r) & 7) << 4);
-    else return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ (r >> 1)) & 7) * 16;
+// where 16 bytes c of row r of a step's K or V lie: blocks of 128 bytes of every
+// row, in the 128-byte swizzle of the copy (rows of 64 bytes: the 64-byte one),
+// so eight rows' equal chunks are in eight bank groups
+template <int RB, int KPS> XP_DEV uint32_t fw_at(uint32_t r, uint32_t c) {
+    if constexpr (RB >= 128) return (c >> 3) * (KPS * 128) + r * 128 + (((c ^ r) & 7) << 4);
+    else return r * 64 + (((c ^ (r >> 1)) & 3) << 4);
+}
+XP_DEV float fw_lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+XP_DEV float fw_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 struct FwWork {
-    unsigned char* slots;    // partial sums of the chunks of split sequences, by item
-    uint32_t* tickets;       // by item: chunks of the sequence that starts there that are done
-    uint32_t* counters;      // [0] items taken beyond the first of every CTA, [1] CTAs that ended
-    uint32_t slot_bytes, most_slots;
+    unsigned char* slots;    // partial sums, two of slot_bytes a CTA
+    uint32_t* tickets;       // by the CTA with a sequence's first unit: CTAs that are done with it
+    uint32_t slot_bytes;
 };
+constexpr uint32_t FW_COST = 2;  // what a sequence costs besides its units, in units
 
-// An item: chunk c of n of head h of sequence b; items are numbered by head,
-// sequence, chunk. Whatever the lengths, the same on every CTA.
+// The units of all heads and sequences end to end, FW_COST more for each, in
+// equal ranges for `ctas` CTAs. Whatever the lengths, the same on every CTA.
 struct FwPlan {
-    uint32_t per_head, chunk;  // items a head, units a chunk
+    uint64_t total;
+    uint32_t ctas;
+    uint32_t h, b;           // where this CTA's range starts
+    uint32_t skip;           // units of that sequence that earlier CTAs have
+    int64_t todo;            // units of the range
 };
-// `ends`: a word a sequence, where its items end. A sequence without new
-// tokens has none; one without keys has one.
-XP_DEV FwPlan fw_make_plan(const ServeAttnArgs& a, const FwWork& w, uint32_t* ends, uint32_t* sums) {
+template <int SHIFT> XP_DEV void fw_make_plan(const ServeAttnArgs& a, uint32_t* sums, FwPlan* out) {
     const uint32_t tid = threadIdx.x;
-    uint32_t n = 0;
-    auto units_of = [&](uint32_t b) -> uint32_t {  // 0: no items
+    uint32_t n = 0, most = 0;
+    auto units_of = [&](uint32_t b) -> uint32_t {
         if (b >= a.batch) return 0;
         const Seq s = seq_of(a, b);
-        return s.nq ? max(at_tile(s, 0, 16, a.window, 6).n, 1u) : 0u;
+        return s.nq ? at_tile(s, 0, 16, a.window, SHIFT).n + FW_COST : 0u;
     };
     uint64_t all = 0;
-    uint32_t most = 0;
+    uint32_t end = 0;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 128) {
         n = units_of(b0 + tid);
         most = max(most, n);
         uint32_t sum;
-        at_scan(n, sums, 128, sum);
+        end = at_scan(n, sums, 128, sum);
         all += sum;
     }
     most = __reduce_max_sync(0xffffffffu, most);
     __syncthreads();
     if ((tid & 31) == 0) sums[tid >> 5] = most;
+    if (tid == 0) out->todo = 0;
     __syncthreads();
     most = max(max(sums[0], sums[1]), max(sums[2], sums[3]));
-    // One chunk a CTA while there are at most a few units for each, else four.
-    // A chunk of c units takes about c / 2 us, adding the n / c chunks of a
+    __syncthreads();
+    // A range of c units takes about c / 2 us, adding the n / c parts of a
     // sequence about 1 / 24 us each: c near sqrt(n / 12) is the least of both.
-    all *= a.kv_heads;
-    const uint64_t ctas = gridDim.x;
-    uint64_t chunk = all <= 8 * ctas ? (all + ctas - 1) / ctas : (all + 4 * ctas - 1) / (4 * ctas);
-    chunk = max(chunk, (uint64_t)max(sqrtf((float)most / 12.0f) + 0.5f, 1.0f));
-    FwPlan p;
-    for (;;) {
-        p.chunk = (uint32_t)min(chunk, (uint64_t)0x7FFFFFFF);
-        uint32_t items = 0;
-        for (uint32_t b0 = 0; b0 < a.batch; b0 += 128) {
-            if (a.batch > 128) n = units_of(b0 + tid);
-            uint32_t sum;
-            const uint32_t end = items + at_scan(n ? (n - 1) / p.chunk + 1 : 0, sums, 128, sum);
-            if (b0 + tid < a.batch) ends[b0 + tid] = end;
-            items += sum;
+    const uint32_t least = FW_COST + (uint32_t)max(sqrtf((float)most / 12.0f) + 0.5f, 1.0f);
+    const uint64_t total = all * a.kv_heads, c = blockIdx.x;
+    const uint64_t g = min((uint64_t)gridDim.x, max(total / least, (uint64_t)1));
+    const uint64_t u0 = total * c / g, u1 = total * (c + 1) / g;
+    if (all == 0 || c >= g || u0 == u1) return;
+    const uint32_t h = (uint32_t)(u0 / all);
+    uint64_t at = all * h;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 128) {
+        uint32_t sum;
+        if (a.batch > 128) {
+            n = units_of(b0 + tid);
+            end = at_scan(n, sums, 128, sum);
+        } else {
+            sum = 0;
         }
-        p.per_head = items;
-        // more items than partial sums have room for: so many sequences need no cut
-        if ((uint64_t)items * a.kv_heads <= w.most_slots || p.chunk == 0x7FFFFFFF) break;
-        chunk = 0x7FFFFFFF;
-        __syncthreads();
+        const uint64_t e = at + end, s = e - n;
+        if (n && s <= u0 && u0 < e) *out = FwPlan{total, (uint32_t)g, h, b0 + tid, (uint32_t)(u0 - s), (int64_t)(u1 - u0)};
+        at += sum;
     }
     __syncthreads();
-    return p;
 }
 
 // An item as the threads of a CTA see it.
 struct FwItem {
-    uint32_t h, b, ch, nch;  // head, sequence, chunk and of how many
+    uint32_t h, b, kind;     // head, sequence, AT_FULL .. AT_LAST, or AT_END: no more
     uint32_t k0, n;          // first unit, units
     uint32_t q0, nq;
+    uint32_t c0, parts;      // the CTA with the sequence's first unit, CTAs that share it
     int32_t first, lo, hi;   // position of the first new token; the keys that are seen
 };
 
 template <class T, class C, int W, int NR>
 __global__ void __launch_bounds__(128, (FwCfg<T, C, W, NR>::CTAS))
-attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ FwWork w) {
+attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ FwWork w,
+                const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using G = FwCfg<T, C, W, NR>;
     // 8-bit codes are multiplied in fp16 whatever T is: one conversion makes two
     // of them, and bf16 would need four more operations. bf16 queries enter
     // scaled by a power of two a row (exact down to 2^-24 of the row's largest).
     using M = std::conditional_t<G::Q8, __half, T>;
     constexpr bool RESCALE = G::Q8 && std::is_same_v<T, bf16>;
-    constexpr int D = G::D, RB = G::RB, NST = G::NST, KS = D / 16, ROWS = 8 * NR;
+    constexpr int D = G::D, RB = G::RB, NST = G::NST, KS = D / 16, ROWS = 8 * NR, KPS = G::KPS, KG = KPS / 16;
     constexpr bool Q8 = G::Q8;
-    extern __shared__ __align__(128) unsigned char sm[];
-    __shared__ uint32_t s_sums[32], s_last, s_item[2];
+    extern __shared__ __align__(1024) unsigned char sm[];
+    __shared__ FwPlan s_plan;
+    __shared__ uint32_t s_sums[32], s_last;
+    __shared__ uint64_t s_bar[4][NST];
+    __shared__ volatile uint32_t s_dead;
     __shared__ FwItem s_desc[2];
-    uint32_t* const ends = reinterpret_cast<uint32_t*>(sm + G::ends_off);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lg = lane >> 2, lq = lane & 3;
-    const uint32_t ring = smem_u32(sm) + warp * (NST * G::STAGE), qbuf = smem_u32(sm) + G::q_off;
-    const FwPlan plan = fw_make_plan(a, w, ends, s_sums);
-    const uint32_t items = plan.per_head * a.kv_heads;
-    auto describe = [&](uint32_t item) {
+    const uint32_t ring = smem_u32(sm) + warp * (NST * 2 * G::HALF), qbuf = smem_u32(sm) + G::q_off;
+    const uint32_t scales = smem_u32(sm) + G::scale_off + warp * (NST * 2 * KPS * 4), bars = smem_u32(&s_bar[warp][0]);
+    if (tid < 4 * NST) {
+        mbar_init(&s_bar[0][0] + tid, Q8 ? 33 : 1);  // the copies' lane, and every lane's scales
+        fence_mbar_init();
+    }
+    if (tid == 0) s_dead = 0;
+    fw_make_plan<G::SHIFT>(a, s_sums, &s_plan);
+    // The CTA's items. One thread makes them two ahead, so that the ring can
+    // run on into the next item while this one's sums are added.
+    constexpr uint32_t boss = 96;
+    struct {
+        uint64_t at;         // where sequence b of head h starts
+        uint32_t h, b, skip;
+        int64_t todo;
+    } walk = {0, 0, 0, 0, 0};
+    auto describe = [&]() {
         FwItem x;
-        x.h = item / plan.per_head;
-        const uint32_t i = item - x.h * plan.per_head;
-        uint32_t lo = 0, hi = a.batch - 1;
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (ends[mid] > i) hi = mid;
-            else lo = mid + 1;
+        x.kind = AT_END;
+        while (walk.todo > 0) {
+            const Seq s = seq_of(a, walk.b);
+            const AtTile t = at_tile(s, 0, 16, a.window, G::SHIFT);
+            const uint32_t all = s.nq ? t.n + FW_COST : 0;
+            const uint32_t step = (uint32_t)min((int64_t)(all - walk.skip), walk.todo);
+            const uint32_t from = max(walk.skip, FW_COST) - FW_COST, to = max(walk.skip + step, FW_COST) - FW_COST;
+            // no unit falls to this CTA: a neighbour has the sequence, or it has none
+            const bool some = all && (t.n ? to > from : walk.skip == 0);
+            if (some) {
+                x.h = walk.h;
+                x.b = walk.b;
+                x.kind = from == 0 ? (to == t.n ? AT_FULL : AT_FIRST) : (to == t.n ? AT_LAST : AT_MIDDLE);
+                x.k0 = t.t0 + from;
+                x.n = to - from;
+                x.q0 = s.q0;
+                x.nq = s.nq;
+                x.first = (int32_t)s.nkv - (int32_t)s.nq;
+                x.lo = t.lo;
+                x.hi = t.hi;
+                // the CTAs of the first and last unit: ranges end at floor(total c / ctas)
+                const uint64_t total = s_plan.total, g = s_plan.ctas, u0 = walk.at + FW_COST;
+                x.c0 = (uint32_t)(((u0 + 1) * g + total - 1) / total - 1);
+                x.parts = t.n ? (uint32_t)(((u0 + t.n) * g + total - 1) / total - 1) - x.c0 + 1 : 1;
+            }
+            walk.todo -= step;
+            walk.at += all;
+            walk.skip = 0;
+            if (++walk.b == a.batch) {
+                walk.b = 0;
+                if (++walk.h == a.kv_heads) walk.todo = 0;
+            }
+            if (some) break;
         }
-        x.b = lo;
-        const uint32_t begin = lo ? ends[lo - 1] : 0;
-        x.nch = ends[lo] - begin;
-        x.ch = i - begin;
-        const Seq s = seq_of(a, x.b);
-        const AtTile t = at_tile(s, 0, 16, a.window, 6);
-        x.q0 = s.q0;
-        x.nq = s.nq;
-        x.first = (int32_t)s.nkv - (int32_t)s.nq;
-        x.lo = t.lo;
-        x.hi = t.hi;
-        x.k0 = t.t0 + x.ch * plan.chunk;
-        x.n = t.n ? min(plan.chunk, t.n - x.ch * plan.chunk) : 0;
         return x;
     };
-    // The CTA's items: the first by its number, the others from a counter. One
-    // thread fetches them two ahead, so that the ring can run on into the next
-    // item while this one's sums are added.
-    const uint32_t boss = 96;
-    uint32_t fetched = 0;
     if (tid == boss) {
-        s_item[0] = blockIdx.x;
-        s_item[1] = blockIdx.x < items ? gridDim.x + atomicAdd(w.counters, 1u) : items;
-        for (int i = 0; i < 2; ++i)
-            if (s_item[i] < items) s_desc[i] = describe(s_item[i]);
+        walk = {0, s_plan.h, s_plan.b, s_plan.skip, s_plan.todo};
+        // the range starts `skip` units into its sequence
+        if (walk.todo > 0) walk.at = s_plan.total * blockIdx.x / s_plan.ctas - walk.skip;
+        s_desc[0] = describe();
+        s_desc[1] = describe();
     }
     __syncthreads();
 
     // ---- the ring: units of this item, then of the next ----
     uint32_t issued = 0, computed = 0;  // units
+    uint32_t phase = 0;                 // bit: parity of the stage's next phase
     uint32_t iu = 0, ipar = 0;          // unit to issue next, in s_desc[ipar]
     bool ahead = false;                 // ... which is the next item
-    int32_t page = -1;
-    auto page_of = [&](const FwItem& g, uint32_t u) -> int32_t {  // lane & 15: the key
-        const int32_t key = (int32_t)((g.k0 + u) * 64 + warp * 16 + (lane & 15));
-        return u < g.n && key >= g.lo && key < g.hi
-                   ? __ldg(a.table + (uint64_t)g.b * a.table_width + (key >> a.pages.page_shift))
-                   : -1;
-    };
+    const uint32_t ps = 1u << a.pages.page_shift, box = min(ps, (uint32_t)KPS);
+    const uint32_t nowhere = (uint32_t)(a.pages.slots >> a.pages.page_shift) * a.kv_heads;
+    auto step_of = [&](const FwItem& g, uint32_t u) { return (int32_t)((g.k0 + u) * G::UNIT + warp * KPS); };
     auto issue = [&]() {
         const FwItem& g = s_desc[ipar];
         if (iu == 0) {
             // the item's queries, a quarter by each warp: 16-byte pieces, a row's first bits of the piece mixed in
-            page = page_of(g, 0);
             const uint32_t nrows = g.nq * a.group;
             for (uint32_t id = tid; id < (uint32_t)ROWS * (D / 8); id += 128) {
                 const uint32_t r = id / (D / 8), c = id % (D / 8), tok = r / a.group, h = g.h * a.group + (r - tok * a.group);
@@ -234,41 +273,56 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 fw_cp16(qbuf + ipar * G::q_bytes + r * (D * 2) + ((c ^ (r & 7)) << 4), qp, has);
             }
         }
-        const int32_t kb = (int32_t)((g.k0 + iu) * 64 + warp * 16);
-        if (kb < g.hi && kb + 16 > g.lo) {
-            const int32_t key = kb + (int32_t)(lane & 15);
-            uint32_t row = AT_NONE;
-            if (key >= g.lo && key < g.hi) {
-                const uint64_t slot = ((uint64_t)(uint32_t)page << a.pages.page_shift) +
-                                      ((uint32_t)key & ((1u << a.pages.page_shift) - 1));
-                if (page < 0 || slot >= a.pages.slots) atomicOr(a.err, SERVE_ERR_PAGE);
-                else row = (uint32_t)page_row(a.pages, slot, g.h);
-            }
-            const uint32_t st = ring + (issued % NST) * G::STAGE;
-            constexpr uint32_t PR = RB / 16;
-#pragma unroll
-            for (uint32_t i = 0; i < PR / 2; ++i) {
-                const uint32_t id = i * 32 + lane, r = id / PR, c = id % PR;
-                const uint32_t x = __shfl_sync(0xffffffffu, row, r);
-                const bool has = x != AT_NONE;
-                const uint64_t off = has ? (uint64_t)x * RB + c * 16 : 0;
-                fw_cp16(st + fw_at<RB>(r, c), static_cast<const char*>(a.pages.k) + off, has);
-                fw_cp16(st + 16 * RB + fw_at<RB>(r, c), static_cast<const char*>(a.pages.v) + off, has);
+        const int32_t kb = step_of(g, iu), lo = g.lo, hi = g.hi;
+        if (kb < hi && kb + KPS > lo) {
+            const uint32_t stage = issued % NST, st = ring + stage * (2 * G::HALF), bar = bars + stage * 8;
+            const int32_t* const row = a.table + (uint64_t)g.b * a.table_width;
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * G::HALF) : "memory");
+            __syncwarp();
+            // a lane a box: pages of the step x blocks of 128 bytes x K and V
+            constexpr uint32_t NB = RB >= 128 ? RB / 128 : 1;
+            const uint32_t per = KPS / box;
+            for (uint32_t j = lane; j < per * NB * 2; j += 32) {
+                const uint32_t p = j % per, blk = j / per, kv = blk / NB, nb = blk % NB;
+                const int32_t key = kb + (int32_t)(p * box);
+                uint32_t z = nowhere;  // past the end: zeros
+                if (key < hi && key + (int32_t)box > lo) {
+                    const int32_t page = __ldg(row + (key >> a.pages.page_shift));
+                    if (page >= 0 && ((uint64_t)(uint32_t)page << a.pages.page_shift) < a.pages.slots)
+                        z = (uint32_t)page * a.kv_heads + g.h;
+                    else
+                        atomicOr(a.err, SERVE_ERR_PAGE);
+                }
+                at_tma(st + kv * G::HALF + nb * (KPS * 128) + p * box * (RB >= 128 ? 128 : 64), kv ? &vmap : &kmap,
+                       nb * (128 / sizeof(C)), (uint32_t)key & (ps - 1), z, bar);
             }
             if constexpr (Q8) {
-                const bool has = row != AT_NONE;
-                fw_cp4(st + 32 * RB + lane * 4, (lane < 16 ? a.pages.ks : a.pages.vs) + (has ? row : 0), has);
+                const int32_t key = kb + (int32_t)lane;
+                bool has = key >= lo && key < hi;
+                uint64_t at = 0;
+                if (has) {
+                    const int32_t page = __ldg(row + (key >> a.pages.page_shift));
+                    at = ((uint64_t)(uint32_t)page << a.pages.page_shift) + ((uint32_t)key & (ps - 1));
+                    has = page >= 0 && at < a.pages.slots;
+                    at = has ? page_row(a.pages, at, g.h) : 0;
+                }
+                const uint32_t sc = scales + stage * (2 * KPS * 4) + lane * 4;
+                if (lane < KPS) {
+                    fw_cp4(sc, a.pages.ks + at, has);
+                    fw_cp4(sc + KPS * 4, a.pages.vs + at, has);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        page = page_of(g, ++iu);
+        ++iu;
         ++issued;
     };
     // as far as the ring has room and there are units
     auto fill = [&](uint32_t par) {
         while (issued < computed + NST) {
             if (iu >= s_desc[ipar].n) {
-                if (ahead || s_item[par ^ 1] >= items || s_desc[par ^ 1].n == 0) return;
+                if (ahead || s_desc[par ^ 1].kind == AT_END || s_desc[par ^ 1].n == 0) return;
                 ahead = true;
                 ipar = par ^ 1;
                 iu = 0;
@@ -277,10 +331,8 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
         }
     };
 
-    for (uint32_t par = 0; s_item[par] < items; par ^= 1) {
-        const uint32_t item = s_item[par];
+    for (uint32_t par = 0; s_desc[par].kind != AT_END; par ^= 1) {
         const FwItem& g = s_desc[par];
-        if (tid == boss) fetched = s_item[par ^ 1] < items ? gridDim.x + atomicAdd(w.counters, 1u) : items;
         if (!ahead) {
             ipar = par;
             iu = 0;
@@ -291,8 +343,7 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
         uint32_t qf[KS][NR][2];
         if (n) {
             fill(par);
-            if (issued - computed >= (uint32_t)NST - 1) asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
-            else asm volatile("cp.async.wait_group 0;" ::: "memory");
+            asm volatile("cp.async.wait_all;" ::: "memory");
             __syncthreads();  // every warp's part of the queries is in
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
@@ -346,6 +397,17 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 khi[i][j] = r < nrows ? max(pos + 1, 0) : 0x7FFFFFFF;
                 klo[i][j] = r < nrows && a.window ? (int32_t)max((int64_t)pos + 1 - (int64_t)a.window, (int64_t)0) : 0;
             }
+        // the keys that every row sees
+        int32_t flo = g.lo, fhi = g.hi;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                flo = max(flo, klo[i][j]);
+                fhi = min(fhi, khi[i][j]);
+            }
+        flo = __reduce_max_sync(0xffffffffu, flo);
+        fhi = __reduce_min_sync(0xffffffffu, fhi);
         float o[KS][NR][4], m[NR][2], ref[NR][2], l[NR][2];
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
@@ -363,32 +425,35 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
         const uint32_t k0 = g.k0;
 #pragma unroll 1
         for (uint32_t u = 0; u < n; ++u, ++computed) {
-            if (issued - computed >= (uint32_t)NST - 1) asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
-            else asm volatile("cp.async.wait_group 0;" ::: "memory");
-            __syncwarp();
+            __syncwarp();  // the step before is read: its stage can be filled
             fill(par);
-            const int32_t kb = (int32_t)((k0 + u) * 64 + warp * 16);
-            if (kb >= hi || kb + 16 <= lo) continue;
-            const uint32_t st = ring + (computed % NST) * G::STAGE;
-            // ---- S^T = K Q^T ----
-            float s[NR][4], s2[NR][4];
+            const int32_t kb = (int32_t)((k0 + u) * G::UNIT + warp * KPS);
+            if (kb >= hi || kb + KPS <= lo) continue;
+            const uint32_t stage = computed % NST, st = ring + stage * (2 * G::HALF);
+            at_wait(bars + stage * 8, phase >> stage & 1, &s_dead, a.err);
+            phase ^= 1u << stage;
+            const bool partial = kb < flo || kb + KPS > fhi;  // some row does not see some key
+            // ---- S^T = K Q^T: blocks of 16 keys ----
+            float s[KG][NR][4];
 #pragma unroll
-            for (int i = 0; i < NR; ++i)
+            for (int b = 0; b < KG; ++b) {
+                float s2[NR][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j] = 0.0f;
-            {
-                const uint32_t r = lane & 15, c0 = lane >> 4;
+                for (int i = 0; i < NR; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[b][i][j] = s2[i][j] = 0.0f;
+                const uint32_t r = 16 * b + (lane & 15), c0 = lane >> 4;
                 if constexpr (Q8) {
 #pragma unroll
                     for (int k = 0; k < KS; k += 2) {
                         uint32_t x[4];
-                        fw_ldm(st + fw_at<RB>(r, k + c0), x);
+                        fw_ldm(st + fw_at<RB, KPS>(r, k + c0), x);
                         const uint2 y0 = at_codes<M>(x[0], C{}), y1 = at_codes<M>(x[1], C{});
                         const uint2 y2 = at_codes<M>(x[2], C{}), y3 = at_codes<M>(x[3], C{});
                         const uint32_t a0[4] = {y0.x, y1.x, y0.y, y1.y}, a1[4] = {y2.x, y3.x, y2.y, y3.y};
 #pragma unroll
                         for (int i = 0; i < NR; ++i) {
-                            fw_mma<M>(s[i], a0, qf[k][i][0], qf[k][i][1]);
+                            fw_mma<M>(s[b][i], a0, qf[k][i][0], qf[k][i][1]);
                             fw_mma<M>(s2[i], a1, qf[k + 1][i][0], qf[k + 1][i][1]);
                         }
                     }
@@ -396,61 +461,65 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
 #pragma unroll
                     for (int k = 0; k < KS; ++k) {
                         uint32_t x[4];
-                        fw_ldm(st + fw_at<RB>(r, 2 * k + c0), x);
+                        fw_ldm(st + fw_at<RB, KPS>(r, 2 * k + c0), x);
 #pragma unroll
-                        for (int i = 0; i < NR; ++i) fw_mma<M>(k & 1 ? s2[i] : s[i], x, qf[k][i][0], qf[k][i][1]);
+                        for (int i = 0; i < NR; ++i) fw_mma<M>(k & 1 ? s2[i] : s[b][i], x, qf[k][i][0], qf[k][i][1]);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[b][i][j] = (s[b][i][j] + s2[i][j]) * rs[i][j & 1];
             }
-            // ---- weights: keys kb + lg (values 0, 1) and kb + lg + 8 (2, 3), rows 2 lq (0, 2) and 2 lq + 1 ----
-            float rv[2] = {1.0f, 1.0f};
+            // ---- weights: keys 16 b + lg (values 0, 1) and 8 more (2, 3), rows 2 lq (0, 2) and 2 lq + 1 ----
+            float rv[KG][2];
+#pragma unroll
+            for (int b = 0; b < KG; ++b) rv[b][0] = rv[b][1] = 1.0f;
             if constexpr (Q8) {
-                float ks[2], lv[2];
+                // a lane a key: its scale, log2 of v's and its inverse; where there
+                // is no key or no page (codes and scales of zero) the value is zero
+                const uint32_t sc = scales + stage * (2 * KPS * 4) + (lane & (KPS - 1)) * 4;
+                const float ks0 = __uint_as_float(at_lds(sc)), vs0 = __uint_as_float(at_lds(sc + KPS * 4));
+                const float lv0 = vs0 == 0.0f ? 0.0f : fw_lg2(vs0), rv0 = vs0 == 0.0f ? 1.0f : fw_rcp(vs0);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    ks[j] = __uint_as_float(at_lds(st + 32 * RB + (lg + 8 * j) * 4));
-                    const float vs = __uint_as_float(at_lds(st + 32 * RB + 64 + (lg + 8 * j) * 4));
-                    lv[j] = log2f(vs);
-                    rv[j] = 1.0f / vs;
-                    if (kb + (int32_t)lg + 8 * j >= hi || kb + (int32_t)lg + 8 * j < lo || vs == 0.0f) {
-                        // no key, or one whose page is missing: its codes are zeros
-                        lv[j] = 0.0f;
-                        rv[j] = 1.0f;
+                for (int b = 0; b < KG; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t from = 16 * b + 8 * h + lg;
+                        const float ks = __shfl_sync(0xffffffffu, ks0, from), lv = __shfl_sync(0xffffffffu, lv0, from);
+                        rv[b][h] = __shfl_sync(0xffffffffu, rv0, from);
+#pragma unroll
+                        for (int i = 0; i < NR; ++i)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) s[b][i][2 * h + j] = fmaf(s[b][i][2 * h + j], ks, lv);
                     }
-                }
-#pragma unroll
-                for (int i = 0; i < NR; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[i][j] = fmaf((s[i][j] + s2[i][j]) * rs[i][j & 1], ks[j >> 1], lv[j >> 1]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < NR; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[i][j] = (s[i][j] + s2[i][j]) * a.scale_log2;
             }
-            bool partial = false;  // some row does not see some key
+            if (partial) {
 #pragma unroll
-            for (int i = 0; i < NR; ++i)
+                for (int b = 0; b < KG; ++b)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) partial |= kb < klo[i][j] || khi[i][j] - kb < 16;
-            partial = __any_sync(0xffffffffu, partial);
+                    for (int i = 0; i < NR; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int32_t key = kb + 16 * b + (int32_t)lg + 8 * (j >> 1);
+                            if (key < klo[i][j & 1] || key >= khi[i][j & 1] || key >= hi || key < lo) s[b][i][j] = -INFINITY;
+                        }
+            }
             bool up = false;
 #pragma unroll
-            for (int i = 0; i < NR; ++i)
+            for (int b = 0; b < KG; ++b)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (partial) {
-                        const int32_t key = kb + (int32_t)lg + 8 * (j >> 1);
-                        if (key < klo[i][j & 1] || key >= khi[i][j & 1]) s[i][j] = -INFINITY;
-                    }
-                    up |= s[i][j] > m[i][j & 1] + 8.0f;
-                }
+                for (int i = 0; i < NR; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) up |= s[b][i][j] > m[i][j & 1] + 8.0f;
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float x = fmaxf(s[i][j], s[i][j + 2]);
+                        float x = fmaxf(s[0][i][j], s[0][i][j + 2]);
+#pragma unroll
+                        for (int b = 1; b < KG; ++b) x = fmaxf(x, fmaxf(s[b][i][j], s[b][i][j + 2]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                         if (x > m[i][j]) {
@@ -465,33 +534,53 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                         }
                     }
             }
-            uint32_t pb[NR][2];
+            uint32_t pb[KG][NR][2];
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
+            for (int b = 0; b < KG; ++b)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[i][j] = at_ex2(s[i][j] - ref[i][j & 1]);
-                    l[i][j & 1] = fmaf(s[i][j], rv[j >> 1], l[i][j & 1]);
+                for (int i = 0; i < NR; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[b][i][j] = at_ex2(s[b][i][j] - ref[i][j & 1]);
+                        l[i][j & 1] = fmaf(s[b][i][j], rv[b][j >> 1], l[i][j & 1]);
+                    }
+                    pb[b][i][0] = fw_movm(at_pack<M>(s[b][i][0], s[b][i][1]));
+                    pb[b][i][1] = fw_movm(at_pack<M>(s[b][i][2], s[b][i][3]));
                 }
-                pb[i][0] = fw_movm(at_pack<M>(s[i][0], s[i][1]));
-                pb[i][1] = fw_movm(at_pack<M>(s[i][2], s[i][3]));
-            }
             // ---- O^T += V^T P^T ----
-            const uint32_t sv = st + 16 * RB;
+            const uint32_t sv = st + G::HALF;
             if constexpr (Q8) {
                 const uint32_t r = lane & 15, c0 = lane >> 4;
 #pragma unroll
-                for (int d = 0; d < KS; d += 2) {
-                    uint32_t x[4];
-                    fw_ldmt(sv + fw_at<RB>(r, d + c0), x);
-                    // a dim's two keys side by side
-                    const uint2 y0 = fw_codes_t(x[0], C{}), y1 = fw_codes_t(x[1], C{});
-                    const uint2 y2 = fw_codes_t(x[2], C{}), y3 = fw_codes_t(x[3], C{});
-                    const uint32_t a0[4] = {y0.x, y0.y, y1.x, y1.y}, a1[4] = {y2.x, y2.y, y3.x, y3.y};
+                for (int b = 0; b < KG; ++b) {
+                    // rows that are no keys may hold anything, codes of NaN among it
+                    uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+                    if (partial) {
 #pragma unroll
-                    for (int i = 0; i < NR; ++i) {
-                        fw_mma<M>(o[d][i], a0, pb[i][0], pb[i][1]);
-                        fw_mma<M>(o[d + 1][i], a1, pb[i][0], pb[i][1]);
+                        for (int h = 0; h < 2; ++h) {
+                            const int32_t key = kb + 16 * b + 8 * h + 2 * (int32_t)lq;
+                            keep[h] = (key >= lo && key < hi ? 0xFFFFu : 0u) | (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u);
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < KS; d += 2) {
+                        uint32_t x[4];
+                        fw_ldmt(sv + fw_at<RB, KPS>(16 * b + r, d + c0), x);
+                        if (partial) {
+                            x[0] &= keep[0];
+                            x[1] &= keep[1];
+                            x[2] &= keep[0];
+                            x[3] &= keep[1];
+                        }
+                        // a dim's two keys side by side
+                        const uint2 y0 = fw_codes_t(x[0], C{}), y1 = fw_codes_t(x[1], C{});
+                        const uint2 y2 = fw_codes_t(x[2], C{}), y3 = fw_codes_t(x[3], C{});
+                        const uint32_t a0[4] = {y0.x, y0.y, y1.x, y1.y}, a1[4] = {y2.x, y2.y, y3.x, y3.y};
+#pragma unroll
+                        for (int i = 0; i < NR; ++i) {
+                            fw_mma<M>(o[d][i], a0, pb[b][i][0], pb[b][i][1]);
+                            fw_mma<M>(o[d + 1][i], a1, pb[b][i][0], pb[b][i][1]);
+                        }
                     }
                 }
             } else {
@@ -499,29 +588,36 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 constexpr uint32_t mask = std::is_same_v<T, bf16> ? 0x7F80u : 0x7C00u;
                 bool odd = false;
 #pragma unroll
-                for (int d = 0; d < KS; ++d) {
-                    uint32_t x[4];
-                    fw_ldmt(sv + fw_at<RB>(r, 2 * d + c0), x);
-                    if (partial) {  // infinities and NaN only to the rows that see them
+                for (int b = 0; b < KG; ++b)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if ((x[j] & mask) == mask) { x[j] &= 0xFFFF0000u; odd = true; }
-                            if ((x[j] & (mask << 16)) == (mask << 16)) { x[j] &= 0xFFFFu; odd = true; }
+                    for (int d = 0; d < KS; ++d) {
+                        uint32_t x[4];
+                        fw_ldmt(sv + fw_at<RB, KPS>(16 * b + r, 2 * d + c0), x);
+                        if (partial) {  // infinities and NaN only to the rows that see them
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int32_t key = kb + 16 * b + 8 * (j >> 1) + 2 * (int32_t)lq;
+                                if (key < lo || key >= hi) x[j] &= 0xFFFF0000u;
+                                if (key + 1 < lo || key + 1 >= hi) x[j] &= 0xFFFFu;
+                                if ((x[j] & mask) == mask) { x[j] &= 0xFFFF0000u; odd = true; }
+                                if ((x[j] & (mask << 16)) == (mask << 16)) { x[j] &= 0xFFFFu; odd = true; }
+                            }
                         }
-                    }
 #pragma unroll
-                    for (int i = 0; i < NR; ++i) fw_mma<M>(o[d][i], x, pb[i][0], pb[i][1]);
-                }
+                        for (int i = 0; i < NR; ++i) fw_mma<M>(o[d][i], x, pb[b][i][0], pb[b][i][1]);
+                    }
                 if (partial && __any_sync(0xffffffffu, odd)) {
 #pragma unroll
                     for (int d = 0; d < KS; ++d)
-                        for (uint32_t j = 0; j < 16; ++j)
+                        for (uint32_t j = 0; j < (uint32_t)KPS; ++j) {
+                            const int32_t key = kb + (int32_t)j;
+                            if (key < lo || key >= hi) continue;
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
                                 T v;
                                 asm volatile("ld.shared.u16 %0, [%1];"
                                              : "=h"(reinterpret_cast<uint16_t&>(v))
-                                             : "r"(sv + fw_at<RB>(j, 2 * d + half) + lg * 2)
+                                             : "r"(sv + fw_at<RB, KPS>(j, 2 * d + half) + lg * 2)
                                              : "memory");
                                 const float x = to_f32(v);
                                 if (fabsf(x) <= 3.4028235e38f) continue;
@@ -529,8 +625,9 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                                 for (int i = 0; i < NR; ++i)
 #pragma unroll
                                     for (int q = 0; q < 2; ++q)
-                                        if (kb + (int32_t)j >= klo[i][q] && kb + (int32_t)j < khi[i][q]) o[d][i][2 * half + q] += x;
+                                        if (key >= klo[i][q] && key < khi[i][q]) o[d][i][2 * half + q] += x;
                             }
+                        }
                 }
             }
         }
@@ -589,8 +686,8 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
             put();
         }
         __syncthreads();
-        const bool whole = g.nch == 1;
-        unsigned char* const part = w.slots + (size_t)item * w.slot_bytes;
+        const bool whole = g.kind == AT_FULL;
+        unsigned char* const part = w.slots + (size_t)(2 * blockIdx.x + (g.kind == AT_FIRST)) * w.slot_bytes;
         auto emit = [&](uint32_t r, uint32_t c, float4 x, float mm, float ll) {
             const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
             const uint32_t tok = r / a.group, h = g.h * a.group + (r - tok * a.group);
@@ -619,18 +716,18 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
             }
         }
         if (!whole) {
-            const uint32_t item0 = item - g.ch;
+            const uint32_t c0 = g.c0, nparts = g.parts;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                s_last = atomicAdd(w.tickets + item0, 1u) == g.nch - 1;
-                if (s_last) w.tickets[item0] = 0;
+                s_last = atomicAdd(w.tickets + c0, 1u) == nparts - 1;
+                if (s_last) w.tickets[c0] = 0;
             }
             __syncthreads();
             if (s_last) {
                 __threadfence();
                 // 64 parts at a time: their m and l in shared memory, then the sums
-                const unsigned char* const parts = w.slots + (size_t)item0 * w.slot_bytes;
+                auto part_of = [&](uint32_t i) { return w.slots + (size_t)(i ? 2 * (c0 + i) : 2 * c0 + 1) * w.slot_bytes; };
                 float2* const ml = reinterpret_cast<float2*>(sm + G::sum_off);  // [64][ROWS]
                 constexpr uint32_t PER = (ROWS * (D / 4) + 127) / 128;  // of a thread
                 float4 x[PER];
@@ -641,13 +738,12 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                     mm[k] = -INFINITY;
                     ll[k] = 0.0f;
                 }
-                for (uint32_t i0 = 0; i0 < g.nch; i0 += 64) {
-                    const uint32_t m = min(g.nch - i0, 64u);
+                for (uint32_t i0 = 0; i0 < nparts; i0 += 64) {
+                    const uint32_t m = min(nparts - i0, 64u);
                     __syncthreads();
                     for (uint32_t i = tid; i < m * ROWS; i += 128) {
                         const uint32_t r = i % ROWS;
-                        ml[i] = r < nrows ? __ldcg(reinterpret_cast<const float2*>(parts + (size_t)(i0 + i / ROWS) * w.slot_bytes +
-                                                                                   (size_t)ROWS * D * 4) + r)
+                        ml[i] = r < nrows ? __ldcg(reinterpret_cast<const float2*>(part_of(i0 + i / ROWS) + (size_t)ROWS * D * 4) + r)
                                           : make_float2(0.0f, 0.0f);
                     }
                     __syncthreads();
@@ -667,10 +763,9 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                         x[k].y *= f0;
                         x[k].z *= f0;
                         x[k].w *= f0;
-                        const unsigned char* p = parts + (size_t)i0 * w.slot_bytes + (size_t)id * 16;
-#pragma unroll 8
-                        for (uint32_t i = 0; i < m; ++i, p += w.slot_bytes) {
-                            const float4 y = __ldcg(reinterpret_cast<const float4*>(p));
+#pragma unroll 16
+                        for (uint32_t i = 0; i < m; ++i) {
+                            const float4 y = __ldcg(reinterpret_cast<const float4*>(part_of(i0 + i)) + id);
                             const float2 v = ml[i * ROWS + r];
                             const float f = v.y != 0.0f ? at_ex2(v.x - top) : 0.0f;
                             ll[k] = fmaf(f, v.y, ll[k]);
@@ -689,18 +784,16 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
             }
         }
         __syncthreads();  // nobody needs s_desc[par] any more
-        if (tid == boss) {
-            s_item[par] = fetched;
-            if (fetched < items) s_desc[par] = describe(fetched);
-        }
+        if (tid == boss) s_desc[par] = describe();
+        __syncthreads();
+    }
+    if (s_dead) {  // copies may still be on their way into this CTA's memory
+        __syncthreads();
+        if (tid < 4 * NST)
+            for (int i = 0; i < 2; ++i) at_wait_flight(smem_u32(&s_bar[0][0] + tid), i);
         __syncthreads();
     }
     at_clear<T, D>(a, 128);
-    // the last CTA leaves the counters as it found them
-    if (tid == 0 && atomicAdd(w.counters + 1, 1u) == gridDim.x - 1) {
-        w.counters[0] = 0;
-        w.counters[1] = 0;
-    }
 }
 
 }  // namespace xp
