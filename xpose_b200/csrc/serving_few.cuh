@@ -30,7 +30,7 @@ template <class T, class C, int W, int NR> struct FwCfg {
     static constexpr int UNIT = 4 * KPS;                     // keys of a unit
     static constexpr int SHIFT = KPS == 32 ? 7 : 6;          // log2 UNIT
     static constexpr int HALF = KPS * RB;                    // K of a step, or V
-    static constexpr int NST = HALF > 4096 ? 2 : HALF > 2048 ? 2 : 3;  // steps of a warp's ring
+    static constexpr int NST = HALF > 4096 ? (NR == 1 ? 3 : 2) : HALF > 2048 ? 2 : 3;  // steps of a warp's ring
     // two warps' sums at a time, with their m and l; the queries of two items
     static constexpr int ring_bytes = 4 * NST * 2 * HALF;
     static constexpr int scale_off = ring_bytes, scale_bytes = Q8 ? 4 * NST * 2 * KPS * 4 : 0;
@@ -97,6 +97,11 @@ XP_DEV float fw_rcp(float x) {
     return y;
 }
 
+// 64-bit division, in 32 bits where both fit (a tenth of the time)
+XP_DEV uint64_t fw_div(uint64_t x, uint64_t y) {
+    return (x | y) >> 32 ? x / y : (uint64_t)((uint32_t)x / (uint32_t)y);
+}
+
 struct FwWork {
     unsigned char* slots;    // partial sums, two of slot_bytes a CTA
     uint32_t* tickets;       // by the CTA with a sequence's first unit: CTAs that are done with it
@@ -137,14 +142,14 @@ template <int SHIFT> XP_DEV void fw_make_plan(const ServeAttnArgs& a, uint32_t* 
     __syncthreads();
     most = max(max(sums[0], sums[1]), max(sums[2], sums[3]));
     __syncthreads();
-    // A range of c units takes about c / 2 us, adding the n / c parts of a
-    // sequence about 1 / 24 us each: c near sqrt(n / 12) is the least of both.
-    const uint32_t least = FW_COST + (uint32_t)max(sqrtf((float)most / 12.0f) + 0.5f, 1.0f);
+    // A range of c units takes about c us, adding the n / c parts of a sequence
+    // about 1 / 16 us each: c near sqrt(n / 16) is the least of both.
+    const uint32_t least = (uint32_t)max(sqrtf((float)most / 16.0f) + 0.5f, 1.0f);
     const uint64_t total = all * a.kv_heads, c = blockIdx.x;
-    const uint64_t g = min((uint64_t)gridDim.x, max(total / least, (uint64_t)1));
-    const uint64_t u0 = total * c / g, u1 = total * (c + 1) / g;
+    const uint64_t g = min((uint64_t)gridDim.x, max(fw_div(total, least), (uint64_t)1));
+    const uint64_t u0 = fw_div(total * c, g), u1 = fw_div(total * (c + 1), g);
     if (all == 0 || c >= g || u0 == u1) return;
-    const uint32_t h = (uint32_t)(u0 / all);
+    const uint32_t h = (uint32_t)fw_div(u0, all);
     uint64_t at = all * h;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 128) {
         uint32_t sum;
@@ -185,7 +190,7 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
     extern __shared__ __align__(1024) unsigned char sm[];
     __shared__ FwPlan s_plan;
     __shared__ uint32_t s_sums[32], s_last;
-    __shared__ uint64_t s_bar[4][NST];
+    __shared__ uint64_t s_bar[4][NST], s_part;
     __shared__ volatile uint32_t s_dead;
     __shared__ FwItem s_desc[2];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lg = lane >> 2, lq = lane & 3;
@@ -195,7 +200,12 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
         mbar_init(&s_bar[0][0] + tid, Q8 ? 33 : 1);  // the copies' lane, and every lane's scales
         fence_mbar_init();
     }
-    if (tid == 0) s_dead = 0;
+    if (tid == 0) {
+        mbar_init(&s_part, 1);
+        fence_mbar_init();
+        s_dead = 0;
+    }
+    uint32_t part_phase = 0;
     fw_make_plan<G::SHIFT>(a, s_sums, &s_plan);
     // The CTA's items. One thread makes them two ahead, so that the ring can
     // run on into the next item while this one's sums are added.
@@ -229,8 +239,8 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 x.hi = t.hi;
                 // the CTAs of the first and last unit: ranges end at floor(total c / ctas)
                 const uint64_t total = s_plan.total, g = s_plan.ctas, u0 = walk.at + FW_COST;
-                x.c0 = (uint32_t)(((u0 + 1) * g + total - 1) / total - 1);
-                x.parts = t.n ? (uint32_t)(((u0 + t.n) * g + total - 1) / total - 1) - x.c0 + 1 : 1;
+                x.c0 = (uint32_t)fw_div((u0 + 1) * g + total - 1, total) - 1;
+                x.parts = t.n ? (uint32_t)fw_div((u0 + t.n) * g + total - 1, total) - x.c0 : 1;
             }
             walk.todo -= step;
             walk.at += all;
@@ -246,9 +256,9 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
     if (tid == boss) {
         walk = {0, s_plan.h, s_plan.b, s_plan.skip, s_plan.todo};
         // the range starts `skip` units into its sequence
-        if (walk.todo > 0) walk.at = s_plan.total * blockIdx.x / s_plan.ctas - walk.skip;
-        s_desc[0] = describe();
-        s_desc[1] = describe();
+        if (walk.todo > 0) walk.at = fw_div(s_plan.total * blockIdx.x, s_plan.ctas) - walk.skip;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) s_desc[i] = describe();
     }
     __syncthreads();
 
@@ -711,12 +721,13 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
             if (whole) {
                 emit(r, c, x, top, ll);
             } else {
-                __stcg(reinterpret_cast<float4*>(part) + id, x);
-                if (c == 0) __stcg(reinterpret_cast<float2*>(part + (size_t)ROWS * D * 4) + r, make_float2(ll != 0.0f ? top : 0.0f, ll));
+                __stcg(reinterpret_cast<float4*>(part + ROWS * 8) + id, x);
+                if (c == 0) __stcg(reinterpret_cast<float2*>(part) + r, make_float2(ll != 0.0f ? top : 0.0f, ll));
             }
         }
         if (!whole) {
             const uint32_t c0 = g.c0, nparts = g.parts;
+            constexpr uint32_t PER = (ROWS * (D / 4) + 127) / 128;  // float4 of a thread
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -726,10 +737,14 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                // 64 parts at a time: their m and l in shared memory, then the sums
-                auto part_of = [&](uint32_t i) { return w.slots + (size_t)(i ? 2 * (c0 + i) : 2 * c0 + 1) * w.slot_bytes; };
-                float2* const ml = reinterpret_cast<float2*>(sm + G::sum_off);  // [64][ROWS]
-                constexpr uint32_t PER = (ROWS * (D / 4) + 127) / 128;  // of a thread
+                // The parts (m and l of every row, then the sums) come into shared
+                // memory by bulk copies: the ring, if no next item runs on in it,
+                // else the small buffer of the sums. Little code, because it runs
+                // once: what is not in the instruction cache costs more than it does.
+                const bool idle = s_desc[par ^ 1].kind == AT_END;
+                unsigned char* const buf = sm + (idle ? 0 : G::sum_off);
+                const uint32_t bytes = ROWS * 8 + nrows * (D * 4);
+                const uint32_t fit = (idle ? (uint32_t)G::ring_bytes : (uint32_t)G::sum_bytes) / bytes;
                 float4 x[PER];
                 float mm[PER], ll[PER];
 #pragma unroll
@@ -738,35 +753,42 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                     mm[k] = -INFINITY;
                     ll[k] = 0.0f;
                 }
-                for (uint32_t i0 = 0; i0 < nparts; i0 += 64) {
-                    const uint32_t m = min(nparts - i0, 64u);
+#pragma unroll 1
+                for (uint32_t i0 = 0; i0 < nparts; i0 += fit) {
+                    const uint32_t m = min(nparts - i0, fit);
                     __syncthreads();
-                    for (uint32_t i = tid; i < m * ROWS; i += 128) {
-                        const uint32_t r = i % ROWS;
-                        ml[i] = r < nrows ? __ldcg(reinterpret_cast<const float2*>(part_of(i0 + i / ROWS) + (size_t)ROWS * D * 4) + r)
-                                          : make_float2(0.0f, 0.0f);
+                    fence_proxy_async();  // what the threads wrote in the buffer, before the copies write there
+                    if (tid == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&s_part)),
+                                     "r"(m * bytes) : "memory");
+                    __syncthreads();
+                    for (uint32_t i = tid; i < m; i += 128) {
+                        const uint32_t p = i0 + i;
+                        bulk_g2s(buf + i * bytes, w.slots + (size_t)(p ? 2 * (c0 + p) : 2 * c0 + 1) * w.slot_bytes, bytes, &s_part);
                     }
-                    __syncthreads();
+                    at_wait(smem_u32(&s_part), part_phase, &s_dead, a.err);
+                    part_phase ^= 1;
 #pragma unroll
                     for (uint32_t k = 0; k < PER; ++k) {
                         const uint32_t id = tid + k * 128, r = id / (D / 4);
-                        if (r >= nrows) continue;
+                        if (r >= nrows) break;
                         float top = mm[k];
+#pragma unroll 4
                         for (uint32_t i = 0; i < m; ++i) {
-                            const float2 v = ml[i * ROWS + r];
-                            if (v.y != 0.0f) top = fmaxf(top, v.x);
+                            const float2 v = *reinterpret_cast<const float2*>(buf + i * bytes + r * 8);
+                            top = fmaxf(top, v.y != 0.0f ? v.x : -INFINITY);
                         }
-                        const float f0 = mm[k] == -INFINITY ? 0.0f : at_ex2(mm[k] - top);
+                        const float f0 = ll[k] != 0.0f ? at_ex2(mm[k] - top) : 0.0f;
                         mm[k] = top;
                         ll[k] *= f0;
                         x[k].x *= f0;
                         x[k].y *= f0;
                         x[k].z *= f0;
                         x[k].w *= f0;
-#pragma unroll 16
+#pragma unroll 4
                         for (uint32_t i = 0; i < m; ++i) {
-                            const float4 y = __ldcg(reinterpret_cast<const float4*>(part_of(i0 + i)) + id);
-                            const float2 v = ml[i * ROWS + r];
+                            const float2 v = *reinterpret_cast<const float2*>(buf + i * bytes + r * 8);
+                            const float4 y = *reinterpret_cast<const float4*>(buf + i * bytes + ROWS * 8 + id * 16);
                             const float f = v.y != 0.0f ? at_ex2(v.x - top) : 0.0f;
                             ll[k] = fmaf(f, v.y, ll[k]);
                             x[k].x = fmaf(f, y.x, x[k].x);
