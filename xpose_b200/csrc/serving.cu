@@ -167,7 +167,7 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
     }
     cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, false, a, w, qm, km, vm);
     if (e == cudaSuccess)
-        e = launch_ex(attn_join_kernel<T, W, G::ROWS>, dim3(ctas, G::ROWS / 32), dim3(256), 0, st, 1, true, a, w, ctas);
+        e = launch_ex(attn_join_kernel<T, W, G::ROWS>, dim3(ctas, G::ROWS / 32 * W), dim3(256), 0, st, 1, true, a, w, ctas);
     if (e != cudaSuccess) return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return XP_OK;
 }

@@ -97,11 +97,6 @@ XP_DEV float fw_rcp(float x) {
     return y;
 }
 
-// 64-bit division, in 32 bits where both fit (a tenth of the time)
-XP_DEV uint64_t fw_div(uint64_t x, uint64_t y) {
-    return (x | y) >> 32 ? x / y : (uint64_t)((uint32_t)x / (uint32_t)y);
-}
-
 struct FwWork {
     unsigned char* slots;    // partial sums, two of slot_bytes a CTA
     uint32_t* tickets;       // by the CTA with a sequence's first unit: CTAs that are done with it
@@ -146,10 +141,10 @@ template <int SHIFT> XP_DEV void fw_make_plan(const ServeAttnArgs& a, uint32_t* 
     // about 1 / 16 us each: c near sqrt(n / 16) is the least of both.
     const uint32_t least = (uint32_t)max(sqrtf((float)most / 16.0f) + 0.5f, 1.0f);
     const uint64_t total = all * a.kv_heads, c = blockIdx.x;
-    const uint64_t g = min((uint64_t)gridDim.x, max(fw_div(total, least), (uint64_t)1));
-    const uint64_t u0 = fw_div(total * c, g), u1 = fw_div(total * (c + 1), g);
+    const uint64_t g = min((uint64_t)gridDim.x, max(at_div(total, least), (uint64_t)1));
+    const uint64_t u0 = at_div(total * c, g), u1 = at_div(total * (c + 1), g);
     if (all == 0 || c >= g || u0 == u1) return;
-    const uint32_t h = (uint32_t)fw_div(u0, all);
+    const uint32_t h = (uint32_t)at_div(u0, all);
     uint64_t at = all * h;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 128) {
         uint32_t sum;
@@ -239,8 +234,8 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 x.hi = t.hi;
                 // the CTAs of the first and last unit: ranges end at floor(total c / ctas)
                 const uint64_t total = s_plan.total, g = s_plan.ctas, u0 = walk.at + FW_COST;
-                x.c0 = (uint32_t)fw_div((u0 + 1) * g + total - 1, total) - 1;
-                x.parts = t.n ? (uint32_t)fw_div((u0 + t.n) * g + total - 1, total) - x.c0 : 1;
+                x.c0 = (uint32_t)at_div((u0 + 1) * g + total - 1, total) - 1;
+                x.parts = t.n ? (uint32_t)at_div((u0 + t.n) * g + total - 1, total) - x.c0 : 1;
             }
             walk.todo -= step;
             walk.at += all;
@@ -256,7 +251,7 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
     if (tid == boss) {
         walk = {0, s_plan.h, s_plan.b, s_plan.skip, s_plan.todo};
         // the range starts `skip` units into its sequence
-        if (walk.todo > 0) walk.at = fw_div(s_plan.total * blockIdx.x, s_plan.ctas) - walk.skip;
+        if (walk.todo > 0) walk.at = at_div(s_plan.total * blockIdx.x, s_plan.ctas) - walk.skip;
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) s_desc[i] = describe();
     }

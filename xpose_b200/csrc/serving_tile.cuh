@@ -262,20 +262,10 @@ XP_DEV void at_sts16(uint32_t a, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// x[i] of lane l (of four) <-> x[l] of lane i: two rounds, each swaps half
-XP_DEV void at_swap16(uint4& lo, uint4& hi, bool up, int m) {
-    const uint4 s = up ? lo : hi;
-    const uint4 y = make_uint4(__shfl_xor_sync(0xffffffffu, s.x, m), __shfl_xor_sync(0xffffffffu, s.y, m),
-                               __shfl_xor_sync(0xffffffffu, s.z, m), __shfl_xor_sync(0xffffffffu, s.w, m));
-    lo = up ? y : lo;
-    hi = up ? hi : y;
-}
-XP_DEV void at_transpose4(uint4 (&x)[4]) {
-    const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
-    at_swap16(x[0], x[1], b0, 1);
-    at_swap16(x[2], x[3], b0, 1);
-    at_swap16(x[0], x[2], b1, 2);
-    at_swap16(x[1], x[3], b1, 2);
+XP_DEV void at_stg32(void* p, uint4 a, uint4 b) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+                 "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
 }
 
 // ---- the split of the work --------------------------------------------------------
@@ -316,6 +306,11 @@ struct AtPlan {
     int64_t todo;             // units from there; whole tiles: those that start within them
     bool split;
 };
+
+// 64-bit division, in 32 bits where both fit (a tenth of the time)
+XP_DEV uint64_t at_div(uint64_t x, uint64_t y) {
+    return (x | y) >> 32 ? x / y : (uint64_t)((uint32_t)x / (uint32_t)y);
+}
 
 XP_DEV uint32_t at_scan(uint32_t v, uint32_t* warp_sums, uint32_t nthreads, uint32_t& total) {
     // inclusive scan over the CTA; warp_sums: 32 words of shared memory
@@ -366,11 +361,12 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
         return at_tile(seq_of(a, b), x, w.tile_tokens, a.window, AT_SHIFT).n + AT_COST;
     };
     uint64_t all = 0;
-    uint32_t most = 0, b = 0, x = 0;
+    uint32_t most = 0, b = 0, x = 0, n = 0, end = 0;
     for (uint32_t i0 = 0; i0 < tiles; i0 += THREADS) {
-        const uint32_t i = i0 + tid, n = i < tiles ? units(i, b, x) : 0;
+        const uint32_t i = i0 + tid;
+        n = i < tiles ? units(i, b, x) : 0;
         uint32_t sum;
-        at_scan(n, sums, THREADS, sum);
+        end = at_scan(n, sums, THREADS, sum);
         all += sum;
         most = max(most, n);
     }
@@ -384,22 +380,26 @@ XP_DEV void at_make_plan(const ServeAttnArgs& a, const AtWork& w, uint32_t* ends
     if (all == 0) return;
     // no CTA has less than a unit, so the parts of a tile are in consecutive CTAs
     const uint64_t total = all * a.kv_heads, c = blockIdx.x;
-    const uint64_t g = min((uint64_t)gridDim.x, max(total / w.least_units, (uint64_t)1));
+    const uint64_t g = min((uint64_t)gridDim.x, max(at_div(total, w.least_units), (uint64_t)1));
     if (c >= g) return;
-    const uint64_t u0 = total * c / g, u1 = total * (c + 1) / g;
-    const bool split = most > max((uint64_t)w.split_over, total / (8 * g));
+    const uint64_t u0 = at_div(total * c, g), u1 = at_div(total * (c + 1), g);
+    const bool split = most > max((uint64_t)w.split_over, at_div(total, 8 * g));
     if (u0 == u1) return;
     // the first tile of the range: split, the one that holds u0; else the
     // first that starts at or after it
-    const uint32_t h0 = (uint32_t)(u0 / all);
+    const uint32_t h0 = (uint32_t)at_div(u0, all);
     for (uint32_t h = h0; h < a.kv_heads && h <= h0 + 1; ++h) {
         uint64_t at = all * h;
         bool found = false;
         for (uint32_t i0 = 0; i0 < tiles && !found; i0 += THREADS) {
-            const uint32_t i = i0 + tid, n = i < tiles ? units(i, b, x) : 0;
-            uint32_t sum;
-            const uint64_t end = at + at_scan(n, sums, THREADS, sum), begin = end - n;
-            const bool mine = n && (split ? begin <= u0 && u0 < end : begin >= u0 && begin < u1);
+            const uint32_t i = i0 + tid;
+            uint32_t sum = 0;
+            if (tiles > THREADS) {  // else as in the loop above
+                n = i < tiles ? units(i, b, x) : 0;
+                end = at_scan(n, sums, THREADS, sum);
+            }
+            const uint64_t stop = at + end, begin = stop - n;
+            const bool mine = n && (split ? begin <= u0 && u0 < stop : begin >= u0 && begin < u1);
             if (split) {
                 if (mine) *out = AtPlan{h, b, x, (uint32_t)(u0 - begin), (int64_t)(u1 - u0), true};
                 found = __syncthreads_or(mine);
@@ -493,11 +493,15 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                  const __grid_constant__ CUtensorMap vmap) {
     using G = AtCfg<T, C, W>;
     constexpr int D = G::D, NQ = G::NQ, NSLOT = G::NSLOT, NSTAGE = G::NSTAGE;
+    // 8-bit codes are multiplied in fp16 whatever T is (a code costs half as
+    // much to convert as in bf16): bf16 queries become fp16 in place
+    using M = std::conditional_t<G::Q8, __half, T>;
+    constexpr bool RESCALE = G::Q8 && std::is_same_v<T, bf16>;
     // no static shared memory: the dynamic part then starts on a 1 KB boundary,
     // which the swizzled layouts need, without a byte lost
     extern __shared__ __align__(1024) unsigned char sm[];
     const uint32_t smb = smem_u32(sm);
-    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 11 + 2 * NSEG;
+    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 13 + 2 * NSEG;
     struct Small {
         AtPlan plan;
         AtSeg segs[NSEG];
@@ -521,7 +525,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     const uint32_t b_o = b_p + 16;                  // [NQ] P V added
     const uint32_t b_seg = b_o + 16, b_free = b_seg + NSEG * 8;  // [NSEG] a row tile given, done with
     const uint32_t b_qfree = b_free + NSEG * 8;     // [NQ] Q multiplied for the last time
-    const uint32_t b_end = b_qfree + 16;            // products in flight after a failed wait
+    const uint32_t b_qh = b_qfree + 16;             // [NQ] ... made fp16
+    const uint32_t b_end = b_qh + 16;               // products in flight after a failed wait
 
     if (smb & 1023) {  // cannot be multiplied from
         if (tid == 0) atomicOr(a.err, SERVE_ERR_WAIT);
@@ -546,7 +551,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             mbar_init(m + 8 + i, 1);
             mbar_init(m + 8 + NSEG + i, NQ * 4 + 4 + 2);
         }
-        for (int i = 0; i < 3; ++i) mbar_init(m + 8 + 2 * NSEG + i, 1);
+        for (int i = 0; i < 5; ++i) mbar_init(m + 8 + 2 * NSEG + i, i == 2 || i == 3 ? 4 : 1);
         fence_mbar_init();
         s_dead = 0;
         for (int i = 0; i < 4; ++i) s_bad[i] = 0;
@@ -587,7 +592,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             w.heads[(2 * blockIdx.x + 1) * 4] = AT_FULL;
         }
         const uint32_t qrow0 = wg * w.sub_tokens;  // first token of this row tile in its CTA's tile
-        uint32_t stage = 0, s_phase = 0, npv = 0;  // s_phase: a bit for each S buffer
+        uint32_t stage = 0, s_phase = 0, npv = 0, q_phase = 0;  // s_phase: a bit for each S buffer
         for (;; done()) {
             const AtSeg& g = take();
             if (g.kind == AT_END || s_dead) break;
@@ -601,6 +606,42 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             if (real) {
                 khi = max(pos + 1, 0);
                 klo = a.window ? (int32_t)max((int64_t)pos + 1 - (int64_t)a.window, (int64_t)0) : 0;
+            }
+            float rs = 1.0f;  // what this row's scores are multiplied by
+            bool rescaled = false;
+            if constexpr (RESCALE) {
+                if (n) {
+                    // this row as fp16; by a power of two into its range where it is not (the
+                    // row's largest outside 2^-4 .. 2^15), exact down to 2^-24 of the largest
+                    at_wait(b_q + 8 * wg, q_phase, &s_dead, err);
+                    q_phase ^= 1;
+                    const uint32_t base = smb + G::q_off + wg * W * 16384 + row * 128;
+                    uint32_t top = 0;
+#pragma unroll 4
+                    for (int i = 0; i < D / 8; ++i) {
+                        const uint4 v = at_lds16(base + (i >> 3) * 16384 + (i & 7) * 16);
+                        const uint32_t o = max(max(v.x & 0x7F80u, v.y & 0x7F80u), max(v.z & 0x7F80u, v.w & 0x7F80u));
+                        const uint32_t h = max(max(v.x & 0x7F800000u, v.y & 0x7F800000u), max(v.z & 0x7F800000u, v.w & 0x7F800000u));
+                        top = max(top, max(o, h >> 16));
+                    }
+                    const uint32_t e = top >> 7;
+                    float f = 1.0f;
+                    if (e > 20 && e < 250 && (e < 123 || e > 141)) f = __uint_as_float((254u - e) << 23);
+                    rs = 1.0f / f;
+                    rescaled = __any_sync(0xffffffffu, f != 1.0f);
+#pragma unroll 4
+                    for (int i = 0; i < D / 8; ++i) {
+                        const uint32_t at = base + (i >> 3) * 16384 + (i & 7) * 16;
+                        const uint4 v = at_lds16(at);
+                        at_sts16(at, make_uint4(at_pack<__half>(bf16_lo(v.x) * f, bf16_hi(v.x) * f),
+                                                at_pack<__half>(bf16_lo(v.y) * f, bf16_hi(v.y) * f),
+                                                at_pack<__half>(bf16_lo(v.z) * f, bf16_hi(v.z) * f),
+                                                at_pack<__half>(bf16_lo(v.w) * f, bf16_hi(v.w) * f)));
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) at_arrive(b_qh + 8 * wg);
+                }
             }
             float m = -INFINITY, ref = 0.0f;
             float2 l2[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
@@ -621,6 +662,10 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     at_wait_ld();
                 }
                 const float* sc = reinterpret_cast<const float*>(sm + G::sc_off) + stage * 384;
+                if (RESCALE && rescaled) {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j) s[j] *= rs;
+                }
                 if constexpr (G::Q8) {
 #pragma unroll
                     for (int j = 0; j < 128; j += 4) {
@@ -699,8 +744,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                             l2[0] = at_add2(l2[0], e0);
                             l2[1] = at_add2(l2[1], e1);
                         }
-                        p[j / 2] = at_pack<T>(e0.x, e0.y);
-                        p[j / 2 + 1] = at_pack<T>(e1.x, e1.y);
+                        p[j / 2] = at_pack<M>(e0.x, e0.y);
+                        p[j / 2 + 1] = at_pack<M>(e1.x, e1.y);
                     }
                     at_st32(s_tm + half * 32, p);
                 }
@@ -725,11 +770,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             unsigned char* part = w.slots + (size_t)slot * w.slot_bytes;
             const uint64_t orow = (uint64_t)(g.s.q0 + tok), ohead = g.h * a.group + rg;
             T* const op = static_cast<T*>(a.out.data) + (int64_t)orow * a.out.ts + (int64_t)ohead * a.out.hs;
-            // four neighbouring lanes store 64 bytes of one of their rows at a time
-            unsigned long long at4[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                at4[i] = __shfl_sync(0xffffffffu, real ? reinterpret_cast<unsigned long long>(op) : 0ull, (lane & ~3u) + i);
+            // a lane stores its own row, 32 bytes (a sector) at a time where rows allow it
+            const bool wide = ((reinterpret_cast<uintptr_t>(a.out.data) | (uintptr_t)(a.out.ts * 2) | (uintptr_t)(a.out.hs * 2)) & 31) == 0;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float o[32];
@@ -774,10 +816,13 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         x[i].z = at_pack<T>(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
                         x[i].w = at_pack<T>(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
                     }
-                    at_transpose4(x);
+                    if (real && wide) {
+                        at_stg32(op + c, x[0], x[1]);
+                        at_stg32(op + c + 16, x[2], x[3]);
+                    } else if (real) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (at4[i]) reinterpret_cast<uint4*>(reinterpret_cast<T*>(at4[i]) + c)[lane & 3] = x[i];
+                        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(op + c)[i] = x[i];
+                    }
                 } else if (real) {
                     float4* pp = reinterpret_cast<float4*>(part) + (size_t)(c / 4) * G::ROWS + wg * 128 + row;
 #pragma unroll
@@ -866,8 +911,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 if (sub == 0 && index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint2 x0 = at_codes<T>(raw[i].x, C{}), x1 = at_codes<T>(raw[i].y, C{});
-                    const uint2 x2 = at_codes<T>(raw[i].z, C{}), x3 = at_codes<T>(raw[i].w, C{});
+                    const uint2 x0 = at_codes<M>(raw[i].x, C{}), x1 = at_codes<M>(raw[i].y, C{});
+                    const uint2 x2 = at_codes<M>(raw[i].z, C{}), x3 = at_codes<M>(raw[i].w, C{});
                     uint32_t d0, d1;
                     if (raw_kind == 1) {
                         const uint32_t r = lt / KU + i * (128 / KU), c = sub * 8 + 2 * (lt % KU);
@@ -1069,7 +1114,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             }
         } else if (warp == NQ * 4 + 4) {
             // ------------------------------ products ------------------------------
-            const uint32_t iqk = at_idesc<T>(AT_KEYS, false), ipv = at_idesc<T>(D, true);
+            const uint32_t iqk = at_idesc<M>(AT_KEYS, false), ipv = at_idesc<M>(D, true);
             const uint32_t q0 = smb + G::q_off, ring = smb + G::ring_off;
             // A step multiplies P V of a row tile, then Q K of the tile that its S
             // buffer takes next; the steps of the two row tiles (NQ = 2) or S
@@ -1086,7 +1131,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 if (!n) continue;
                 const uint32_t k0 = g.k0;
                 const int32_t lo = g.lo, hi = g.hi, p0 = g.p0;
-                for (int i = 0; i < NQ; ++i) at_wait(b_q + 8 * i, q_phase, &s_dead, err);
+                for (int i = 0; i < NQ; ++i) at_wait((RESCALE ? b_qh : b_q) + 8 * i, q_phase, &s_dead, err);
                 q_phase ^= 1;
                 const uint32_t steps = NQ == 2 ? 2 * n + 2 : n + 2;
 #pragma unroll 1
@@ -1168,50 +1213,68 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     }
 }
 
-// The row tiles that CTAs share: 32 rows of one tile a CTA, the parts added in
-// the order of their keys. blockIdx.x is the CTA that has the tile's first keys.
+// The row tiles that CTAs share: 32 rows x 64 dims of one tile a CTA, the parts
+// added in the order of their keys. blockIdx.x is the CTA that has the tile's
+// first keys; blockIdx.y = rows / 32 + dims / 64 * (ROWS / 32).
 template <class T, int W, int ROWS>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ AtWork w,
                                                         uint32_t ctas) {
-    constexpr int D = 64 * W, NC = D / 32;
+    constexpr int D = 64 * W;
     pdl_wait();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
     const uint4 head = __ldcg(reinterpret_cast<const uint4*>(w.heads) + 2 * c0 + 1);
     if (head.x != AT_FIRST) return;
-    uint32_t parts = 0;  // that follow the first
+    uint32_t parts = 1;
     for (uint32_t j = c0 + 1; j < ctas; j += 32) {
         const uint32_t kind = j + lane < ctas ? __ldcg(w.heads + (size_t)(2 * (j + lane)) * 4) : (uint32_t)AT_LAST;
         const uint32_t last = __ballot_sync(0xffffffffu, kind == AT_LAST);
         parts += last ? __ffs(last) : 32;
         if (last) break;
     }
-    const uint32_t row = blockIdx.y * 32 + lane;
+    const uint32_t row = blockIdx.y % (ROWS / 32) * 32 + lane, col = (blockIdx.y / (ROWS / 32) * 8 + warp) * 2;  // float4 pairs
     auto part = [&](uint32_t i) { return w.slots + (size_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * w.slot_bytes; };
-    float m = -INFINITY;
-    for (uint32_t i = 0; i <= parts; ++i) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(part(i) + (size_t)ROWS * D * 4) + row);
-        if (v.y != 0.0f) m = fmaxf(m, v.x);
-    }
-    float l = 0.0f;
-    float4 o[NC];
+    float m = -INFINITY, l = 0.0f;
+    float4 o[2] = {};
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < parts; i0 += 4) {
+        float2 v[4];
+        float4 x[4][2];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) o[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
-    for (uint32_t i = 0; i <= parts; ++i) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(part(i) + (size_t)ROWS * D * 4) + row);
-        const float4* p = reinterpret_cast<const float4*>(part(i)) + (size_t)warp * NC * ROWS + row;
-        float4 x[NC];
+        for (uint32_t i = 0; i < 4; ++i) {
+            v[i] = make_float2(0.0f, 0.0f);
+            if (i0 + i < parts) {
+                const float4* p = reinterpret_cast<const float4*>(part(i0 + i)) + (size_t)col * ROWS + row;
+                v[i] = __ldcg(reinterpret_cast<const float2*>(part(i0 + i) + (size_t)ROWS * D * 4) + row);
+                x[i][0] = __ldcg(p);
+                x[i][1] = __ldcg(p + ROWS);
+            }
+        }
+        float top = m;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) x[c] = __ldcg(p + (size_t)c * ROWS);
-        if (v.y == 0.0f) continue;
-        const float f = at_ex2(v.x - m);
-        l += f * v.y;
+        for (uint32_t i = 0; i < 4; ++i)
+            if (v[i].y != 0.0f) top = fmaxf(top, v[i].x);
+        const float f0 = l != 0.0f ? at_ex2(m - top) : 0.0f;
+        m = top;
+        l *= f0;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            o[c].x += f * x[c].x;
-            o[c].y += f * x[c].y;
-            o[c].z += f * x[c].z;
-            o[c].w += f * x[c].w;
+        for (int c = 0; c < 2; ++c) {
+            o[c].x *= f0;
+            o[c].y *= f0;
+            o[c].z *= f0;
+            o[c].w *= f0;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (v[i].y == 0.0f) continue;
+            const float f = at_ex2(v[i].x - top);
+            l = fmaf(f, v[i].y, l);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                o[c].x = fmaf(f, x[i][c].x, o[c].x);
+                o[c].y = fmaf(f, x[i][c].y, o[c].y);
+                o[c].z = fmaf(f, x[i][c].z, o[c].z);
+                o[c].w = fmaf(f, x[i][c].w, o[c].w);
+            }
         }
     }
     const Seq s = seq_of(a, head.y);
@@ -1220,17 +1283,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     if (rt >= w.sub_tokens || tok >= s.nq) return;
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     const uint64_t orow = s.q0 + tok, ohead = head.z * a.group + rg;
-    T* op = static_cast<T*>(a.out.data) + (int64_t)orow * a.out.ts + (int64_t)ohead * a.out.hs + warp * NC * 4;
-#pragma unroll
-    for (int c = 0; c < NC; c += 2) {
-        uint4 y;
-        y.x = at_pack<T>(o[c].x * inv, o[c].y * inv);
-        y.y = at_pack<T>(o[c].z * inv, o[c].w * inv);
-        y.z = at_pack<T>(o[c + 1].x * inv, o[c + 1].y * inv);
-        y.w = at_pack<T>(o[c + 1].z * inv, o[c + 1].w * inv);
-        *reinterpret_cast<uint4*>(op + c * 4) = y;
-    }
-    if (a.lse && warp == 0)
+    uint4 y;
+    y.x = at_pack<T>(o[0].x * inv, o[0].y * inv);
+    y.y = at_pack<T>(o[0].z * inv, o[0].w * inv);
+    y.z = at_pack<T>(o[1].x * inv, o[1].y * inv);
+    y.w = at_pack<T>(o[1].z * inv, o[1].w * inv);
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.out.data) + (int64_t)orow * a.out.ts + (int64_t)ohead * a.out.hs + col * 4) = y;
+    if (a.lse && col == 0)
         a.lse[orow * a.heads + ohead] = l != 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
