@@ -63,7 +63,13 @@ template <class T, class C, int W> struct AtCfg {
     static constexpr int VKEYS = AT_KEYS / NP;    // keys of a V piece
     static constexpr int NSLOT = W == 1 ? 10 : Q8 ? 4 : 5;
     static constexpr int NSTAGE = W == 1 ? 8 : 4; // tiles whose row numbers and scales are kept
-    static constexpr int THREADS = 128 * NQ + 256;
+    static constexpr int NLD = Q8 && W == 4 ? 2 : 1;  // loader warpgroups
+    static constexpr int THREADS = 128 * NQ + 128 * NLD + 128;
+    // registers of a softmax, a loader and the last warpgroup: THREADS / 128 shares of the launch's
+    static constexpr int R_SOFT = NQ == 2 ? 184 : NLD == 2 ? 208 : 232;
+    static constexpr int R_LOAD = NQ == 2 ? 80 : NLD == 2 ? 104 : 136;
+    static constexpr int R_REST = NQ == 2 ? 64 : NLD == 2 ? 96 : 136;
+    static_assert(NQ * R_SOFT + NLD * R_LOAD + R_REST <= THREADS / 128 * (65536 / THREADS / 8 * 8), "registers");
     // shared memory
     static constexpr int q_off = 0;
     static constexpr int ring_off = NQ * W * 16384;
@@ -476,14 +482,17 @@ struct AtWalk {
     }
 };
 
-// V of key tile kt needs a look: a loaded row lies outside the tile's keys, or
-// some row of the tile does not see some key.
-XP_DEV bool at_look(const ServeAttnArgs& a, int32_t lo, int32_t hi, int32_t p0, uint32_t kt) {
-    const int64_t k0 = (int64_t)kt * AT_KEYS, k1 = k0 + AT_KEYS;
+// The V rows of keys [k0, k0 + n) need a look: one lies outside the tile's
+// keys, or some row of the tile does not see some of them.
+XP_DEV bool at_look(const ServeAttnArgs& a, int32_t lo, int32_t hi, int32_t p0, uint32_t key, uint32_t n) {
+    const int64_t k0 = (int64_t)key, k1 = k0 + n;
     return k0 < lo || k1 > hi || k1 > (int64_t)p0 + 1 || (a.window && k0 < (int64_t)hi - (int64_t)a.window);
 }
-XP_DEV bool at_odd16(uint32_t w, uint32_t exp_mask) {  // an infinity or NaN in either half
-    return (w & exp_mask) == exp_mask || (w & (exp_mask << 16)) == (exp_mask << 16);
+// Bits 15 and 31: an infinity or NaN in either half (all exponent bits set, so
+// one more carries out of them)
+template <class T> XP_DEV uint32_t at_odd16(uint32_t w) {
+    if constexpr (std::is_same_v<T, bf16>) return (w & 0x7F807F80u) + 0x00800080u;
+    else return (w & 0x7C007C00u) + 0x04000400u;
 }
 
 template <class T, class C, int W>
@@ -495,6 +504,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     constexpr int D = G::D, NQ = G::NQ, NSLOT = G::NSLOT, NSTAGE = G::NSTAGE;
     // 8-bit codes are multiplied in fp16 whatever T is (a code costs half as
     // much to convert as in bf16): bf16 queries become fp16 in place
+    constexpr uint32_t LAST = NQ * 4 + G::NLD * 4;  // first warp of the last warpgroup
     using M = std::conditional_t<G::Q8, __half, T>;
     constexpr bool RESCALE = G::Q8 && std::is_same_v<T, bf16>;
     // no static shared memory: the dynamic part then starts on a 1 KB boundary,
@@ -535,7 +545,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     if (tid == 0) {
         uint64_t* m = reinterpret_cast<uint64_t*>(sm + G::bar_off);
         for (int i = 0; i < NSLOT; ++i) {
-            mbar_init(m + i, G::Q8 ? 4 : 1);
+            mbar_init(m + i, G::Q8 ? 4 * G::NLD : 1);
             mbar_init(m + NSLOT + i, 1);
             mbar_init(m + 2 * NSLOT + i, 1);
             mbar_init(m + 3 * NSLOT + i, 4);
@@ -549,14 +559,14 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
         }
         for (int i = 0; i < NSEG; ++i) {
             mbar_init(m + 8 + i, 1);
-            mbar_init(m + 8 + NSEG + i, NQ * 4 + 4 + 2);
+            mbar_init(m + 8 + NSEG + i, NQ * 4 + G::NLD * 4 + 2);
         }
         for (int i = 0; i < 5; ++i) mbar_init(m + 8 + 2 * NSEG + i, i == 2 || i == 3 ? 4 : 1);
         fence_mbar_init();
         s_dead = 0;
         for (int i = 0; i < 4; ++i) s_bad[i] = 0;
     }
-    if (warp == NQ * 4 + 4) {
+    if (warp == LAST) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&small.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -582,8 +592,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
 
     if (warp < NQ * 4) {
         // ------------------------------ softmax ------------------------------
-        if constexpr (NQ == 2) at_regs_up<184>();
-        else at_regs_up<232>();
+        at_regs_up<G::R_SOFT>();
         const uint32_t wg = warp >> 2, row = tid & 127;
         const uint32_t lanes = (warp & 3) * 32 << 16;
         const uint32_t o_tm = tmem + lanes + 256 + wg * D;
@@ -619,7 +628,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     uint32_t top = 0;
 #pragma unroll 4
                     for (int i = 0; i < D / 8; ++i) {
-                        const uint4 v = at_lds16(base + (i >> 3) * 16384 + (i & 7) * 16);
+                        const uint4 v = at_lds16(base + (i >> 3) * 16384 + ((i ^ row) & 7) * 16);
                         const uint32_t o = max(max(v.x & 0x7F80u, v.y & 0x7F80u), max(v.z & 0x7F80u, v.w & 0x7F80u));
                         const uint32_t h = max(max(v.x & 0x7F800000u, v.y & 0x7F800000u), max(v.z & 0x7F800000u, v.w & 0x7F800000u));
                         top = max(top, max(o, h >> 16));
@@ -631,7 +640,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     rescaled = __any_sync(0xffffffffu, f != 1.0f);
 #pragma unroll 4
                     for (int i = 0; i < D / 8; ++i) {
-                        const uint32_t at = base + (i >> 3) * 16384 + (i & 7) * 16;
+                        const uint32_t at = base + (i >> 3) * 16384 + ((i ^ row) & 7) * 16;
                         const uint4 v = at_lds16(at);
                         at_sts16(at, make_uint4(at_pack<__half>(bf16_lo(v.x) * f, bf16_hi(v.x) * f),
                                                 at_pack<__half>(bf16_lo(v.y) * f, bf16_hi(v.y) * f),
@@ -785,10 +794,11 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 if (bad && real) {
                     // infinities and NaN of v were left out of the products of tiles
                     // where not every row sees every key: they go to the rows that do
-                    for (uint32_t t = 0; t < g.n; ++t) {
-                        if (!at_look(a, g.lo, g.hi, g.p0, g.k0 + t)) continue;
-                        const int32_t j0 = max((int32_t)((g.k0 + t) * AT_KEYS), klo);
-                        const int32_t j1 = min(min((int32_t)((g.k0 + t + 1) * AT_KEYS), khi), g.hi);
+                    for (uint32_t t = 0; t < g.n * G::NP; ++t) {
+                        const uint32_t key0 = g.k0 * AT_KEYS + t * G::VKEYS;
+                        if (!at_look(a, g.lo, g.hi, g.p0, key0, G::VKEYS)) continue;
+                        const int32_t j0 = max((int32_t)key0, klo);
+                        const int32_t j1 = min(min((int32_t)(key0 + G::VKEYS), khi), g.hi);
                         for (int32_t j = j0; j < j1; ++j) {
                             const T* vp;
                             if (a.pages.k) {
@@ -839,11 +849,10 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 if (tid == 0) *reinterpret_cast<uint4*>(w.heads + slot * 4) = make_uint4(g.kind, g.b, g.h, g.x);
             }
         }
-    } else if (warp < NQ * 4 + 4) {
+    } else if (warp < LAST) {
         // ------------------------------ loader ------------------------------
-        if constexpr (NQ == 2) at_regs_down<80>();
-        else at_regs_down<136>();
-        const uint32_t lt = tid - NQ * 128;
+        at_regs_down<G::R_LOAD>();
+        const uint32_t lt = (tid - NQ * 128) & 127, lw = (tid - NQ * 128) >> 7;  // lw: which loader warpgroup
         // where 16 bytes c of row r of a piece go: for every 64 dims a block of
         // rows of 128 bytes, swizzled
         auto k_at = [&](uint32_t r, uint32_t c) { return (c >> 3) * (AT_KEYS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
@@ -856,46 +865,55 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 if (g.kind == AT_END || s_dead) break;
                 const int32_t lo = g.lo, hi = g.hi, p0 = g.p0;
                 const uint32_t n = g.n, k0 = g.k0;
-                for (uint32_t t = 0; t < n; ++t) {
-                    if (!at_look(a, lo, hi, p0, k0 + t)) continue;
-                    for (int c = 0; c < G::NP; ++c) {
-                        const uint32_t i = before + (min(n, t + G::LAG) + t) * G::NP + c, slot = i % NSLOT;
-                        at_wait(b_raw + 8 * (cleaned % NSLOT), (cleaned / NSLOT) & 1, &s_dead, err);
-                        const uint32_t base = smb + G::ring_off + slot * G::PIECE;
-                        constexpr uint32_t mask = std::is_same_v<T, bf16> ? 0x7F80u : 0x7C00u, VU = 8 * W;
-                        bool odd = false;
-#pragma unroll
-                        for (int j = 0; j < G::PIECE / 2048; ++j) {
-                            const uint32_t r = lt / VU + j * (128 / VU), at = base + v_at(r, lt % VU);
-                            const int32_t key = (int32_t)((k0 + t) * AT_KEYS + c * G::VKEYS + r);
-                            if (key < lo || key >= hi) {
-                                at_sts16(at, make_uint4(0, 0, 0, 0));
-                                continue;
-                            }
-                            uint4 v = at_lds16(at);
-                            if (at_odd16(v.x, mask) || at_odd16(v.y, mask) || at_odd16(v.z, mask) || at_odd16(v.w, mask)) {
-                                odd = true;
-                                uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    if ((x[q] & mask) == mask) x[q] &= 0xFFFF0000u;
-                                    if ((x[q] & (mask << 16)) == (mask << 16)) x[q] &= 0xFFFFu;
-                                }
-                                at_sts16(at, make_uint4(x[0], x[1], x[2], x[3]));
-                            }
+                for (uint32_t u = 0; u < n * G::NP; ++u) {
+                    const uint32_t t = u / G::NP, c = u % G::NP, key0 = (k0 + t) * AT_KEYS + c * G::VKEYS;
+                    if (!at_look(a, lo, hi, p0, key0, G::VKEYS)) continue;
+                    const uint32_t i = before + (min(n, t + G::LAG) + t) * G::NP + c, slot = i % NSLOT;
+                    at_wait(b_raw + 8 * (cleaned % NSLOT), (cleaned / NSLOT) & 1, &s_dead, err);
+                    const uint32_t base = smb + G::ring_off + slot * G::PIECE;
+                    constexpr uint32_t VU = 8 * W, N = G::PIECE / 2048;
+                    const uint32_t r0 = lt / VU, u0 = lt % VU;
+                    if ((int32_t)key0 < lo || (int32_t)(key0 + G::VKEYS) > hi) {
+#pragma unroll 4
+                        for (uint32_t j = 0; j < N; ++j) {
+                            const uint32_t r = r0 + j * (128 / VU);
+                            const int32_t key = (int32_t)(key0 + r);
+                            if (key < lo || key >= hi) at_sts16(base + v_at(r, u0), make_uint4(0, 0, 0, 0));
                         }
-                        if (odd) s_bad[seg & 3] = seg + 1;
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) at_arrive(b_clean + 8 * (cleaned % NSLOT));
-                        ++cleaned;
                     }
+                    uint32_t odd = 0;
+#pragma unroll 8
+                    for (uint32_t j = 0; j < N; ++j) {
+                        const uint4 v = at_lds16(base + v_at(r0 + j * (128 / VU), u0));
+                        odd |= at_odd16<T>(v.x) | at_odd16<T>(v.y) | at_odd16<T>(v.z) | at_odd16<T>(v.w);
+                    }
+                    if (odd & 0x80008000u) {
+                        for (uint32_t j = 0; j < N; ++j) {
+                            const uint32_t at = base + v_at(r0 + j * (128 / VU), u0);
+                            const uint4 v = at_lds16(at);
+                            uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const uint32_t m = at_odd16<T>(x[q]);
+                                if (m & 0x8000u) x[q] &= 0xFFFF0000u;
+                                if (m & 0x80000000u) x[q] &= 0xFFFFu;
+                            }
+                            at_sts16(at, make_uint4(x[0], x[1], x[2], x[3]));
+                        }
+                        s_bad[seg & 3] = seg + 1;
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) at_arrive(b_clean + 8 * (cleaned % NSLOT));
+                    ++cleaned;
                 }
                 before += 2 * n * G::NP;
             }
         } else {
-            // a thread's 4 x 16 codes are 16 KB of a piece: SUB of them make one
-            constexpr uint32_t SUB = G::PIECE / 16384;
+            // a warpgroup's 4 x 16 codes a thread are 16 KB of a piece: SUB of them
+            // make one, one after the other or by a warpgroup each
+            constexpr uint32_t SUB = G::PIECE / 16384 / G::NLD;
+            static_assert(G::NLD == 1 || SUB == 1, "loaders");
             uint32_t subs = 0, stage = 0;
             uint4 raw[4];                 // the codes of the part issued last
             uint32_t raw_kind = 0;        // ... 0 none, 1 K, 2 V
@@ -906,9 +924,10 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             // the codes in `raw` into their slot, as 16-bit values
             auto convert = [&]() {
                 if (raw_kind == 0) return;
-                const uint32_t index = (subs - 1) / SUB, sub = (subs - 1) % SUB, slot = index % NSLOT;
+                const uint32_t index = (subs - 1) / SUB, turn = (subs - 1) % SUB, slot = index % NSLOT;
+                const uint32_t sub = G::NLD == 2 ? lw : turn;
                 const uint32_t base = smb + G::ring_off + slot * G::PIECE;
-                if (sub == 0 && index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
+                if (turn == 0 && index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint2 x0 = at_codes<M>(raw[i].x, C{}), x1 = at_codes<M>(raw[i].y, C{});
@@ -926,13 +945,9 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     at_sts16(base + d0, make_uint4(x0.x, x0.y, x1.x, x1.y));
                     at_sts16(base + d1, make_uint4(x2.x, x2.y, x3.x, x3.y));
                 }
-                if (sub + 1 == SUB) {
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) at_arrive(b_full + 8 * slot);
-                } else {
-                    fence_proxy_async();
-                }
+                fence_proxy_async();
+                __syncwarp();
+                if (turn + 1 == SUB && lane == 0) at_arrive(b_full + 8 * slot);
                 raw_kind = 0;
             };
             for (;; done()) {
@@ -977,6 +992,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         else r = (uint32_t)page_row(a.pages, slot, head);
                     }
                     if (t + 1 < n) page = page_of(k0 + t + 1);
+                    if (lw == 0) {
                     asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 512 + lt * 4), "r"(r) : "memory");
                     float* sc = reinterpret_cast<float*>(sm + G::sc_off) + kst * 384;
                     float ks = 0.0f, lv = 0.0f, rv = in ? 1.0f : 0.0f;
@@ -989,19 +1005,20 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     sc[lt] = ks;
                     sc[128 + lt] = lv;
                     sc[256 + lt] = rv;
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    }
+                    asm volatile("bar.sync 1, %0;" ::"n"(128 * G::NLD) : "memory");
                 };
                 for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) {
                     resolve(t);
-                    for (int c = 0; c < W; ++c) piece(false, c, kst);
+                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, kst);
                     kst = kst + 1 == NSTAGE ? 0 : kst + 1;
                 }
                 for (uint32_t t = 0; t < n; ++t) {
-                    for (int c = 0; c < W; ++c) piece(true, c, stage);
+                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(true, c, stage);
                     stage = stage + 1 == NSTAGE ? 0 : stage + 1;
                     if (t + G::LAG < n) {
                         resolve(t + G::LAG);
-                        for (int c = 0; c < W; ++c) piece(false, c, kst);
+                        for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, kst);
                         kst = kst + 1 == NSTAGE ? 0 : kst + 1;
                     }
                 }
@@ -1009,9 +1026,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             }
         }
     } else {
-        if constexpr (NQ == 2) at_regs_down<64>();
-        else at_regs_down<136>();
-        if (warp == NQ * 4 + 5) {
+        at_regs_down<G::R_REST>();
+        if (warp == LAST + 1) {
             // ------------------------------ the list of row tiles ------------------------------
             AtWalk walk;
             walk.start(s_plan);
@@ -1027,7 +1043,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 }
                 __syncwarp();
             }
-        } else if (warp == NQ * 4 + 6) {
+        } else if (warp == LAST + 2) {
             // ------------------------------ copies ------------------------------
             uint32_t i = 0, raw = 0, last = 0;  // pieces, those to look over; last: parity of a slot's next phase
             uint32_t tiles = 0;                 // row tiles with keys
@@ -1100,8 +1116,10 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 ++tiles;
                 for (uint32_t t = 1; t < (uint32_t)G::LAG && t < n; ++t) k_tile(t);
                 for (uint32_t t = 0; t < n; ++t) {
-                    const bool look = at_look(a, lo, hi, g.p0, k0 + t);
-                    for (int c = 0; c < G::NP; ++c) piece(&vmap, (k0 + t) * AT_KEYS + c * G::VKEYS, G::VKEYS, 0, W, look);
+                    for (int c = 0; c < G::NP; ++c) {
+                        const uint32_t key = (k0 + t) * AT_KEYS + c * G::VKEYS;
+                        piece(&vmap, key, G::VKEYS, 0, W, at_look(a, lo, hi, g.p0, key, G::VKEYS));
+                    }
                     if (t + G::LAG < n) k_tile(t + G::LAG);
                 }
             }
@@ -1112,7 +1130,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     if (raw > j) at_wait_flight(b_raw + 8 * ((raw - 1 - j) % NSLOT), ((raw - 1 - j) / NSLOT) & 1);
                 }
             }
-        } else if (warp == NQ * 4 + 4) {
+        } else if (warp == LAST) {
             // ------------------------------ products ------------------------------
             const uint32_t iqk = at_idesc<M>(AT_KEYS, false), ipv = at_idesc<M>(D, true);
             const uint32_t q0 = smb + G::q_off, ring = smb + G::ring_off;
@@ -1142,12 +1160,12 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     if (t >= (uint32_t)G::LAG) {
                         // O += P V of key tile t - LAG; pieces arrive K(0) .. K(LAG - 1), V(0), K(LAG), V(1), ..
                         const uint32_t tv = t - G::LAG;
-                        const bool look = !G::Q8 && first && at_look(a, lo, hi, p0, k0 + tv);
                         uint32_t slot = (base + (min(n, t) + tv) * G::NP) % NSLOT;
                         at_wait(b_p + 8 * buf, p_phase >> buf & 1, &s_dead, err);
                         p_phase ^= 1u << buf;
 #pragma unroll
                         for (int c = 0; c < G::NP; ++c) {
+                            const bool look = !G::Q8 && first && at_look(a, lo, hi, p0, (k0 + tv) * AT_KEYS + c * G::VKEYS, G::VKEYS);
                             if (look) {
                                 at_wait(b_clean + 8 * (cleaned % NSLOT), (cleaned / NSLOT) & 1, &s_dead, err);
                                 ++cleaned;
@@ -1207,7 +1225,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     }
     at_fence_before();
     __syncthreads();
-    if (warp == NQ * 4 + 4) {
+    if (warp == LAST) {
         at_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
