@@ -69,7 +69,10 @@ xp_status check_rope_data(const char* who, const xp_rotary* r) {
 #define TRY(expr) \
     if (xp_status s_ = (expr); s_ != XP_OK) return s_
 
-RowsArg rows_arg(const xp_rows* r) { return RowsArg{r->data, r->token_stride, r->head_stride}; }
+RowsArg rows_arg(const xp_rows* r, uint64_t t0 = 0) {
+    return RowsArg{static_cast<char*>(r->data) + (int64_t)t0 * r->token_stride * (int64_t)bytes_of(r->dtype), r->token_stride,
+                   r->head_stride};
+}
 RopeArg rope_arg(const xp_rotary* r) {
     if (!r) return RopeArg{};
     return RopeArg{reinterpret_cast<const unsigned long long*>(r->turns), r->positions, r->rot_dim,
@@ -131,8 +134,8 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
     static_assert(SCRATCH_SLOTS + 2ull * AT_MAX_CTAS * G::ROWS * (G::D * 4 + 8) <= XP_SERVING_SCRATCH_BYTES, "scratch");
     w.sub_tokens = 128 / a.group;
     w.tile_tokens = w.sub_tokens * G::NQ;
-    w.least_units = AT_COST + 2;
-    w.split_over = AT_COST + 6;
+    w.least_units = 2;
+    w.split_over = AT_COST + 1;
     CUtensorMap qm{}, km{}, vm{};
     const CUtensorMapDataType type =
         std::is_same_v<T, bf16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -226,9 +229,15 @@ template <class F> xp_status for_dim(uint32_t dim, F f) {
     }
 }
 
-xp_status grid_of(const char* who, uint64_t blocks, unsigned* grid) {
-    REQUIRE(blocks <= 0x7FFFFFFFull, "%s: too many rows for one launch", who);
-    *grid = (unsigned)blocks;
+// f(first token, tokens, grid) for as many tokens at a time as keep a launch's
+// thread numbers in 32 bits.
+template <class F> xp_status in_parts(const char* who, uint64_t tokens, uint64_t per_token, uint32_t block, F f) {
+    REQUIRE(per_token < (1ull << 31), "%s: too many values in a token", who);
+    const uint64_t most = std::max<uint64_t>((1ull << 31) / per_token, 1);
+    for (uint64_t t0 = 0; t0 < tokens; t0 += most) {
+        const uint64_t n = std::min(tokens - t0, most);
+        TRY(f(t0, (uint32_t)n, (unsigned)((n * per_token + block - 1) / block)));
+    }
     return XP_OK;
 }
 
@@ -281,15 +290,22 @@ xp_status xp_rope_rows(void* stream, const xp_rows* out, const xp_rows* in, cons
     uint32_t hpt = 1;
     while (hpt < 8 && hpt < in->heads && (uint64_t)in->tokens * units * in->heads / (2 * hpt) >= (uint64_t)sm_count() * 2048)
         hpt *= 2;
-    unsigned grid;
-    TRY(grid_of(who, ((uint64_t)in->tokens * ((in->heads + hpt - 1) / hpt) * units + 255) / 256, &grid));
+    // 32-byte accesses where a unit's values lie side by side and every row allows it
+    bool side = wide && in->dim % (2 * vec) == 0;
+    for (const xp_rows* r : {out, in})
+        side = side && r->token_stride % (2 * vec) == 0 && r->head_stride % (2 * vec) == 0 && (uintptr_t)r->data % 32 == 0;
     const bool copy = out->data != in->data;
-    return for_type(in->dtype, [&](auto t) {
-        using T = decltype(t);
-        auto k = wide ? rope_rows_kernel<T, 16 / sizeof(T)> : rope_rows_kernel<T, 1>;
-        k<<<grid, 256, 0, (cudaStream_t)stream>>>(rows_arg(out), rows_arg(in), rope_arg(rope), in->tokens, in->heads,
-                                                  in->dim, hpt, units, copy);
-        return launched(who);
+    const uint64_t per_token = (uint64_t)((in->heads + hpt - 1) / hpt) * units;
+    return in_parts(who, in->tokens, per_token, 256, [&](uint64_t t0, uint32_t n, unsigned grid) {
+        return for_type(in->dtype, [&](auto t) {
+            using T = decltype(t);
+            auto k = wide ? rope_rows_kernel<T, 16 / sizeof(T)> : rope_rows_kernel<T, 1>;
+            RopeArg r = rope_arg(rope);
+            r.positions += t0;
+            k<<<grid, 256, 0, (cudaStream_t)stream>>>(rows_arg(out, t0), rows_arg(in, t0), r, n, in->heads, in->dim, hpt,
+                                                      units, copy, side);
+            return launched(who);
+        });
     });
 }
 
@@ -297,23 +313,24 @@ xp_status xp_kv_write(void* stream, const xp_pages* pages, const xp_rows* k, con
                       const xp_rotary* rope) {
     const char* who = "kv_write";
     TRY(check_pages(who, pages));
-    const uint32_t w = pages->head_dim / 64;
-    TRY(check_rows(who, "k", k, w));
-    TRY(check_rows(who, "v", v, w));
+    TRY(check_rows(who, "k", k, 8));
+    TRY(check_rows(who, "v", v, 8));
     REQUIRE(same_shape(k, v) && k->heads == pages->kv_heads && k->dim == pages->head_dim,
             "%s: 'k', 'v' and the pages differ in shape or type", who);
-    if (rope) TRY(check_rope(who, rope, k->dim, 2 * w));
+    if (rope) TRY(check_rope(who, rope, k->dim, 8));
     if (k->tokens == 0) return XP_OK;
     if (rope) TRY(check_rope_data(who, rope));
     REQUIRE(slots, "%s: argument 'slots' is null", who);
-    unsigned grid;
-    TRY(grid_of(who, ((uint64_t)k->tokens * k->heads + 7) / 8, &grid));
-    return for_type(k->dtype, [&](auto t) {
-        return for_cache(pages->dtype, [&](auto c) {
-            return for_dim(k->dim, [&](auto d) {
-                kv_write_kernel<decltype(t), decltype(c), d.value><<<grid, 256, 0, (cudaStream_t)stream>>>(
-                    pages_arg(pages), rows_arg(k), rows_arg(v), slots, k->tokens, rope_arg(rope), rope != nullptr);
-                return launched(who);
+    return in_parts(who, k->tokens, (uint64_t)k->heads * (k->dim / 8), 256, [&](uint64_t t0, uint32_t n, unsigned grid) {
+        return for_type(k->dtype, [&](auto t) {
+            return for_cache(pages->dtype, [&](auto c) {
+                return for_dim(k->dim, [&](auto d) {
+                    RopeArg r = rope_arg(rope);
+                    if (rope) r.positions += t0;
+                    kv_write_kernel<decltype(t), decltype(c), d.value><<<grid, 256, 0, (cudaStream_t)stream>>>(
+                        pages_arg(pages), rows_arg(k, t0), rows_arg(v, t0), slots + t0, n, r, rope != nullptr);
+                    return launched(who);
+                });
             });
         });
     });
@@ -331,14 +348,14 @@ xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, cons
             "%s: 'k', 'v' and the pages differ in shape or type", who);
     if (k->tokens == 0) return XP_OK;
     REQUIRE(slots, "%s: argument 'slots' is null", who);
-    unsigned grid;
-    TRY(grid_of(who, ((uint64_t)k->tokens * k->heads * (k->dim / 16) + 255) / 256, &grid));
-    return for_type(k->dtype, [&](auto t) {
-        return for_cache(pages->dtype, [&](auto c) {
-            return for_dim(k->dim, [&](auto d) {
-                kv_read_kernel<decltype(t), decltype(c), d.value><<<grid, 256, 0, (cudaStream_t)stream>>>(
-                    pages_arg(pages), rows_arg(k), rows_arg(v), slots, k->tokens);
-                return launched(who);
+    return in_parts(who, k->tokens, (uint64_t)k->heads * (k->dim / 16), 256, [&](uint64_t t0, uint32_t n, unsigned grid) {
+        return for_type(k->dtype, [&](auto t) {
+            return for_cache(pages->dtype, [&](auto c) {
+                return for_dim(k->dim, [&](auto d) {
+                    kv_read_kernel<decltype(t), decltype(c), d.value><<<grid, 256, 0, (cudaStream_t)stream>>>(
+                        pages_arg(pages), rows_arg(k, t0), rows_arg(v, t0), slots + t0, n);
+                    return launched(who);
+                });
             });
         });
     });

@@ -7,9 +7,9 @@
 // bits of a turn, so position 10^6 is as exact as position 1. A thread makes
 // the cosines and sines of its pairs once and applies them to all its heads.
 //
-// Cache rows. One warp per (token, kv head) holds the k row and the v row in
-// registers, two vectors of W = dim / 64 values a lane, so the row's maximum
-// is one warp reduction and the codes leave in the same pass.
+// Cache rows. dim / 8 lanes hold a row of k and one of v in registers, two
+// vectors of four values a lane, so a row's maximum is a few shuffles and the
+// codes leave in the same pass.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -43,6 +43,48 @@ template <int N, class T> XP_DEV void store_f32(T* p, const float* x) {
     *reinterpret_cast<Pack<T, N>*>(p) = r;
 }
 
+// 32 bytes of values as one access (`side`: they lie side by side, aligned to
+// 32) or as two vectors
+struct Raw32 { uint32_t w[8]; };
+XP_DEV Raw32 load_raw32(const void* a, const void* b, bool side) {
+    Raw32 r;
+    if (side) {
+        asm("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+            : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+            : "l"(a));
+    } else {
+        const uint4 x = *static_cast<const uint4*>(a), y = *static_cast<const uint4*>(b);
+        r = Raw32{{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}};
+    }
+    return r;
+}
+XP_DEV void store_raw32(void* a, void* b, const Raw32& r, bool side) {
+    if (side) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(a), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]),
+                     "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7])
+                     : "memory");
+    } else {
+        *static_cast<uint4*>(a) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+        *static_cast<uint4*>(b) = make_uint4(r.w[4], r.w[5], r.w[6], r.w[7]);
+    }
+}
+// its 32 / sizeof(T) values
+template <class T> XP_DEV float raw_get(const Raw32& r, int i) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[i]);
+    else if constexpr (std::is_same_v<T, bf16>) return i & 1 ? bf16_hi(r.w[i / 2]) : bf16_lo(r.w[i / 2]);
+    else return __half2float(__ushort_as_half((unsigned short)(r.w[i / 2] >> (16 * (i & 1)))));
+}
+template <class T> XP_DEV void raw_put2(Raw32& r, int i, float x, float y) {  // values i and i + 1, i even
+    if constexpr (sizeof(T) == 4) {
+        r.w[i] = __float_as_uint(x);
+        r.w[i + 1] = __float_as_uint(y);
+    } else if constexpr (std::is_same_v<T, bf16>) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.w[i / 2]) : "f"(y), "f"(x));
+    } else {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r.w[i / 2]) : "f"(y), "f"(x));
+    }
+}
+
 struct RowsArg {
     void* data;
     int64_t ts, hs;  // token and head strides, elements
@@ -69,18 +111,18 @@ XP_DEV void rope_angle(const RopeArg& r, int32_t pos, uint32_t i, float& c, floa
 // A unit is VP pairs: two vectors of VP values of the head (half layout) or 2
 // VP consecutive ones (interleaved); units past the rotated part copy 2 VP
 // values. Thread = (token, unit) of `hpt` consecutive heads.
-// VP > 1 needs rot / 2 and dim to be multiples of VP and 2 VP, and every row
-// to be aligned to VP values; VP = 1 takes any strides and alignment.
+// VP > 1 needs rot / 2 and dim to be multiples of VP, and every row to be
+// aligned to VP values; VP = 1 takes any strides and alignment. `side`: rows
+// are aligned to 2 VP values, so that values side by side move in one access
+// of 32 bytes (a whole sector; two of 16 took 75 us where this takes 53, 16381
+// tokens x 32 heads of 128 in bf16).
 template <class T, int VP>
 __global__ void __launch_bounds__(256) rope_rows_kernel(RowsArg out, RowsArg in, RopeArg r, uint32_t tokens,
                                                         uint32_t heads, uint32_t dim, uint32_t hpt, uint32_t nunits,
-                                                        bool copy_tail) {
+                                                        bool copy_tail, bool side) {
     const uint32_t chunks = (heads + hpt - 1) / hpt;
-    const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint32_t unit = (uint32_t)(id % nunits);
-    const uint64_t rest = id / nunits;
-    const uint32_t h0 = (uint32_t)(rest % chunks) * hpt;
-    const uint64_t t = rest / chunks;
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, rest = id / nunits, unit = id - rest * nunits;
+    const uint32_t t = rest / chunks, h0 = (rest - t * chunks) * hpt;
     if (t >= tokens) return;
     const uint32_t n = r.rot / 2, rot_units = n / VP;
     const T* src = static_cast<const T*>(in.data) + (int64_t)t * in.ts + (int64_t)h0 * in.hs;
@@ -93,37 +135,69 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(RowsArg out, RowsArg in,
         for (int i = 0; i < VP; ++i) rope_angle(r, pos, unit * VP + i, c[i], s[i]);
         const uint32_t a0 = r.interleaved ? 2 * unit * VP : unit * VP;
         const uint32_t b0 = r.interleaved ? a0 + VP : n + unit * VP;
-#pragma unroll 4
-        for (uint32_t h = 0; h < nh; ++h, src += in.hs, dst += out.hs) {
-            float x[2 * VP], y[2 * VP];
-            load_f32<VP>(src + a0, x);
-            load_f32<VP>(src + b0, x + VP);
-            if (r.interleaved) {
+        if constexpr (VP > 1) {
+            const bool both = side && r.interleaved;
+            constexpr uint32_t B = 4;  // heads whose loads are under way together
+            for (uint32_t h = 0; h < nh; h += B) {
+                Raw32 x[B];
 #pragma unroll
-                for (int i = 0; i < VP; ++i) {
-                    y[2 * i] = x[2 * i] * c[i] - x[2 * i + 1] * s[i];
-                    y[2 * i + 1] = x[2 * i] * s[i] + x[2 * i + 1] * c[i];
-                }
-            } else {
+                for (uint32_t j = 0; j < B; ++j)
+                    if (h + j < nh) x[j] = load_raw32(src + (h + j) * in.hs + a0, src + (h + j) * in.hs + b0, both);
 #pragma unroll
-                for (int i = 0; i < VP; ++i) {
-                    y[i] = x[i] * c[i] - x[VP + i] * s[i];
-                    y[VP + i] = x[i] * s[i] + x[VP + i] * c[i];
+                for (uint32_t j = 0; j < B; ++j) {
+                    if (h + j >= nh) break;
+                    Raw32 y;
+                    if (r.interleaved) {
+#pragma unroll
+                        for (int i = 0; i < VP; ++i) {
+                            const float p = raw_get<T>(x[j], 2 * i), q = raw_get<T>(x[j], 2 * i + 1);
+                            raw_put2<T>(y, 2 * i, p * c[i] - q * s[i], p * s[i] + q * c[i]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < VP; i += 2) {
+                            const float p0 = raw_get<T>(x[j], i), q0 = raw_get<T>(x[j], VP + i);
+                            const float p1 = raw_get<T>(x[j], i + 1), q1 = raw_get<T>(x[j], VP + i + 1);
+                            raw_put2<T>(y, i, p0 * c[i] - q0 * s[i], p1 * c[i + 1] - q1 * s[i + 1]);
+                            raw_put2<T>(y, VP + i, p0 * s[i] + q0 * c[i], p1 * s[i + 1] + q1 * c[i + 1]);
+                        }
+                    }
+                    store_raw32(dst + (h + j) * out.hs + a0, dst + (h + j) * out.hs + b0, y, both);
                 }
             }
-            store_f32<VP>(dst + a0, y);
-            store_f32<VP>(dst + b0, y + VP);
+        } else {
+            for (uint32_t h = 0; h < nh; ++h, src += in.hs, dst += out.hs) {
+                const float p = to_f32(src[a0]), q = to_f32(src[b0]);
+                dst[a0] = from_f32<T>(p * c[0] - q * s[0]);
+                dst[b0] = from_f32<T>(p * s[0] + q * c[0]);
+            }
         }
     } else if (copy_tail) {
         const uint32_t d = r.rot + (unit - rot_units) * 2 * VP;
         const bool second = d + VP < dim;
-#pragma unroll 4
-        for (uint32_t h = 0; h < nh; ++h, src += in.hs, dst += out.hs) {
-            const Pack<T, VP> a = *reinterpret_cast<const Pack<T, VP>*>(src + d);
-            Pack<T, VP> b{};
-            if (second) b = *reinterpret_cast<const Pack<T, VP>*>(src + d + VP);
-            *reinterpret_cast<Pack<T, VP>*>(dst + d) = a;
-            if (second) *reinterpret_cast<Pack<T, VP>*>(dst + d + VP) = b;
+        if constexpr (VP > 1) {
+            constexpr uint32_t B = 4;
+            for (uint32_t h = 0; h < nh; h += B) {
+                Raw32 x[B];
+#pragma unroll
+                for (uint32_t j = 0; j < B; ++j)
+                    if (h + j < nh) {
+                        const T* p = src + (h + j) * in.hs + d;
+                        x[j] = load_raw32(p, second ? p + VP : p, side && second);
+                    }
+#pragma unroll
+                for (uint32_t j = 0; j < B; ++j) {
+                    if (h + j >= nh) break;
+                    T* p = dst + (h + j) * out.hs + d;
+                    if (second) store_raw32(p, p + VP, x[j], side);
+                    else *reinterpret_cast<uint4*>(p) = make_uint4(x[j].w[0], x[j].w[1], x[j].w[2], x[j].w[3]);
+                }
+            }
+        } else {
+            for (uint32_t h = 0; h < nh; ++h, src += in.hs, dst += out.hs) {
+                dst[d] = src[d];
+                if (second) dst[d + 1] = src[d + 1];
+            }
         }
     }
 }
@@ -144,88 +218,111 @@ XP_DEV uint64_t page_row(const PagesArg& p, uint64_t slot, uint32_t head) {
 
 constexpr float CACHE_FLOOR = 0x1p-100f;  // smallest row maximum told from zero
 
-// A row's 2 W values a lane (at lane_d[0] and lane_d[1]) into its place.
-template <class C, int W>
-XP_DEV void cache_row_store(C* row, float* scale, const float* x, const uint32_t* d) {
+// A lane's 8 values of a row, four at d[0] and four at d[1], into its place;
+// LANES lanes hold the row.
+template <class C, int LANES>
+XP_DEV void cache_row_store(C* row, float* scale, const float* x, const uint32_t* d, bool live) {
     if constexpr (sizeof(C) > 1) {
-        store_f32<W>(row + d[0], x);
-        store_f32<W>(row + d[1], x + W);
+        if (!live) return;
+        if (d[1] == d[0] + 4) {
+            store_f32<8>(row + d[0], x);
+        } else {
+            store_f32<4>(row + d[0], x);
+            store_f32<4>(row + d[1], x + 4);
+        }
     } else {
         constexpr float Q = std::is_same_v<C, int8c> ? 127.0f : 448.0f;
         // the maximum as an integer: for |x| the order of the bits is the
         // order of the values, and an infinity or NaN is above them all
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 2 * W; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-        top = __reduce_max_sync(0xffffffffu, top);
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (!live) return;
         const bool finite = top < 0x7F800000u;
         const float m = fmaxf(__uint_as_float(top), CACHE_FLOOR);
         const float inv = finite ? __fdiv_rn(Q, m) : 0.0f;
-        if ((threadIdx.x & 31) == 0) *scale = finite ? __fdiv_rn(m, Q) : __uint_as_float(0x7FC00000u);
+        if (threadIdx.x % LANES == 0) *scale = finite ? __fdiv_rn(m, Q) : __uint_as_float(0x7FC00000u);
+        uint32_t w[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            Pack<uint8_t, W> r;
+            uint32_t b[4];
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float y = finite ? x[j * W + i] * inv : 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const float y = finite ? x[j * 4 + i] * inv : 0.0f;
                 if constexpr (std::is_same_v<C, int8c>) {
-                    r.v[i] = (uint8_t)(int8_t)__float2int_rn(fminf(fmaxf(y, -127.0f), 127.0f));
+                    b[i] = (uint32_t)__float2int_rn(fminf(fmaxf(y, -127.0f), 127.0f)) & 0xFFu;
                 } else {
                     uint16_t two;
                     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.0f), "f"(y));
-                    r.v[i] = (uint8_t)two;
+                    b[i] = two & 0xFFu;
                 }
             }
-            *reinterpret_cast<Pack<uint8_t, W>*>(reinterpret_cast<uint8_t*>(row) + d[j]) = r;
+            w[j] = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+        }
+        uint8_t* const p = reinterpret_cast<uint8_t*>(row);
+        if (d[1] == d[0] + 4) {
+            *reinterpret_cast<uint2*>(p + d[0]) = make_uint2(w[0], w[1]);
+        } else {
+            *reinterpret_cast<uint32_t*>(p + d[0]) = w[0];
+            *reinterpret_cast<uint32_t*>(p + d[1]) = w[1];
         }
     }
 }
 
-// One warp per (token, kv head). W = dim / 64 values in each of a lane's two
-// vectors; with a rotation a lane's vectors are the two ends of its pairs.
+// dim / 8 lanes per (token, kv head). A lane's two vectors of four lie side by
+// side, except that a half-layout rotation pairs four of the first half with
+// the four that turn with them.
 template <class T, class C, int W>
 __global__ void __launch_bounds__(256) kv_write_kernel(PagesArg p, RowsArg k, RowsArg v, const int64_t* slots,
                                                        uint32_t tokens, RopeArg r, bool rotate) {
-    constexpr uint32_t DIM = 64 * W;
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t id = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const uint64_t t = id / p.kv_heads;
-    const uint32_t h = (uint32_t)(id % p.kv_heads);
-    if (t >= tokens) return;
-    const int64_t slot = __ldg(slots + t);
-    if (slot < 0 || (uint64_t)slot >= p.slots) return;
-    const T* kp = static_cast<const T*>(k.data) + (int64_t)t * k.ts + (int64_t)h * k.hs;
-    const T* vp = static_cast<const T*>(v.data) + (int64_t)t * v.ts + (int64_t)h * v.hs;
-    // the lane's vectors: contiguous pairs of vectors, except that a half-
-    // layout rotation pairs vector j of the first half with j of the second
-    uint32_t d[2] = {lane * 2 * W, lane * 2 * W + W};
+    constexpr uint32_t DIM = 64 * W, LANES = DIM / 8;
+    const uint32_t part = threadIdx.x % LANES, id = (blockIdx.x * 256 + threadIdx.x) / LANES;
+    const uint32_t t = id / p.kv_heads, h = id - t * p.kv_heads;
+    const int64_t slot = t < tokens ? __ldg(slots + t) : -1;
+    const bool live = slot >= 0 && (uint64_t)slot < p.slots;  // others only take part in the shuffles
+    uint32_t d[2] = {part * 8, part * 8 + 4};
     const uint32_t n = r.rot / 2;
-    const bool turns = rotate && lane * W < n;
+    const bool turns = rotate && part * 4 < n;
     if (turns && !r.interleaved) {
-        d[0] = lane * W;
-        d[1] = n + lane * W;
+        d[0] = part * 4;
+        d[1] = n + part * 4;
     }
-    float kx[2 * W], vx[2 * W];
-    load_f32<W>(kp + d[0], kx);
-    load_f32<W>(kp + d[1], kx + W);
-    load_f32<W>(vp + d[0], vx);
-    load_f32<W>(vp + d[1], vx + W);
-    if (turns) {
-        const int32_t pos = __ldg(r.positions + t);
+    float kx[8] = {}, vx[8] = {};
+    if (live) {
+        const T* kp = static_cast<const T*>(k.data) + (int64_t)t * k.ts + (int64_t)h * k.hs;
+        const T* vp = static_cast<const T*>(v.data) + (int64_t)t * v.ts + (int64_t)h * v.hs;
+        if (sizeof(T) == 2 && d[1] == d[0] + 4) {
+            load_f32<8>(kp + d[0], kx);
+            load_f32<8>(vp + d[0], vx);
+        } else {
+            load_f32<4>(kp + d[0], kx);
+            load_f32<4>(kp + d[1], kx + 4);
+            load_f32<4>(vp + d[0], vx);
+            load_f32<4>(vp + d[1], vx + 4);
+        }
+        if (turns) {
+            const int32_t pos = __ldg(r.positions + t);
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            float c, s;
-            rope_angle(r, pos, lane * W + i, c, s);
-            float& a = r.interleaved ? kx[2 * i] : kx[i];
-            float& b = r.interleaved ? kx[2 * i + 1] : kx[W + i];
-            const float a1 = a * c - b * s, b1 = a * s + b * c;
-            a = a1;
-            b = b1;
+            for (int i = 0; i < 4; ++i) {
+                float c, s;
+                rope_angle(r, pos, part * 4 + i, c, s);
+                const float a = r.interleaved ? kx[2 * i] : kx[i], b = r.interleaved ? kx[2 * i + 1] : kx[4 + i];
+                const float a1 = a * c - b * s, b1 = a * s + b * c;
+                if (r.interleaved) {
+                    kx[2 * i] = a1;
+                    kx[2 * i + 1] = b1;
+                } else {
+                    kx[i] = a1;
+                    kx[4 + i] = b1;
+                }
+            }
         }
     }
-    const uint64_t row = page_row(p, (uint64_t)slot, h);
-    cache_row_store<C, W>(static_cast<C*>(p.k) + row * DIM, p.ks + row, kx, d);
-    cache_row_store<C, W>(static_cast<C*>(p.v) + row * DIM, p.vs + row, vx, d);
+    const uint64_t row = live ? page_row(p, (uint64_t)slot, h) : 0;
+    cache_row_store<C, LANES>(static_cast<C*>(p.k) + row * DIM, p.ks + row, kx, d, live);
+    cache_row_store<C, LANES>(static_cast<C*>(p.v) + row * DIM, p.vs + row, vx, d, live);
 }
 
 // 4 codes of a word as fp32
@@ -249,18 +346,30 @@ template <class T, class C, int W>
 __global__ void __launch_bounds__(256) kv_read_kernel(PagesArg p, RowsArg k, RowsArg v, const int64_t* slots,
                                                       uint32_t rows) {
     constexpr uint32_t DIM = 64 * W, PER = DIM / 16;
-    const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint32_t part = (uint32_t)(id % PER) * 16;
-    const uint64_t th = id / PER;
-    const uint64_t t = th / p.kv_heads;
-    const uint32_t h = (uint32_t)(th % p.kv_heads);
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, part = id % PER * 16, th = id / PER;
+    const uint32_t t = th / p.kv_heads, h = th - t * p.kv_heads;
     if (t >= rows) return;
     const int64_t slot = __ldg(slots + t);
     const bool has = slot >= 0 && (uint64_t)slot < p.slots;
     const uint64_t row = page_row(p, has ? (uint64_t)slot : 0, h);
+    // both sides' codes and scales under way together
+    Pack<C, 16> c[2];
+    float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
         const C* src = static_cast<const C*>(side ? p.v : p.k) + row * DIM + part;
+        if (has) {
+            if constexpr (sizeof(C) > 1) {
+                reinterpret_cast<uint4*>(&c[side])[0] = reinterpret_cast<const uint4*>(src)[0];
+                reinterpret_cast<uint4*>(&c[side])[1] = reinterpret_cast<const uint4*>(src)[1];
+            } else {
+                *reinterpret_cast<uint4*>(&c[side]) = *reinterpret_cast<const uint4*>(src);
+                s[side] = (side ? p.vs : p.ks)[row];
+            }
+        }
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
         const RowsArg& o = side ? v : k;
         T* dst = static_cast<T*>(o.data) + (int64_t)t * o.ts + (int64_t)h * o.hs + part;
         float x[16];
@@ -268,21 +377,32 @@ __global__ void __launch_bounds__(256) kv_read_kernel(PagesArg p, RowsArg k, Row
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = 0.0f;
         } else if constexpr (sizeof(C) > 1) {
-            load_f32<8>(src, x);
-            load_f32<8>(src + 8, x + 8);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = to_f32(c[side].v[i]);
         } else {
-            const uint4 w = *reinterpret_cast<const uint4*>(src);
-            const float s = (side ? p.vs : p.ks)[row];
+            const uint4 w = *reinterpret_cast<const uint4*>(&c[side]);
             codes4(w.x, C{}, x);
             codes4(w.y, C{}, x + 4);
             codes4(w.z, C{}, x + 8);
             codes4(w.w, C{}, x + 12);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] *= s;
+            for (int i = 0; i < 16; ++i) x[i] *= s[side];
         }
         constexpr int V = 16 / sizeof(T);
+        // a lane's 32 bytes as whole sectors, where the rows allow it
+        const bool wide = ((reinterpret_cast<uintptr_t>(o.data) | (uintptr_t)(o.ts * sizeof(T)) | (uintptr_t)(o.hs * sizeof(T))) & 31) == 0;
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < 16; i += V) store_f32<V>(dst + i, x + i);
+            for (int i = 0; i < 16; i += 2 * V) {
+                Raw32 r;
+#pragma unroll
+                for (int j = 0; j < 2 * V; j += 2) raw_put2<T>(r, j, x[i + j], x[i + j + 1]);
+                store_raw32(dst + i, nullptr, r, true);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += V) store_f32<V>(dst + i, x + i);
+        }
     }
 }
 

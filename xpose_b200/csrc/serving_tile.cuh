@@ -914,26 +914,26 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             // make one, one after the other or by a warpgroup each
             constexpr uint32_t SUB = G::PIECE / 16384 / G::NLD;
             static_assert(G::NLD == 1 || SUB == 1, "loaders");
-            uint32_t subs = 0, stage = 0;
-            uint4 raw[4];                 // the codes of the part issued last
-            uint32_t raw_kind = 0;        // ... 0 none, 1 K, 2 V
+            uint32_t given = 0, stage = 0;   // parts given to the tensor core
+            // the codes of the two parts issued last (0 older), and what they are: 0 none, 1 K, 2 V
+            uint4 raw[2][4];
+            uint32_t kind[2] = {0, 0};
             const uint32_t rows0 = smb + G::row_off;
             // thread -> 16 codes: unit u of rows r0, r0 + step, ..; a K part has
             // all rows of 64 dims, a V part 128 / W whole rows
             constexpr uint32_t KU = 4, VU = 4 * W;
-            // the codes in `raw` into their slot, as 16-bit values
+            // the older part into its slot, as 16-bit values; the other takes its place
             auto convert = [&]() {
-                if (raw_kind == 0) return;
-                const uint32_t index = (subs - 1) / SUB, turn = (subs - 1) % SUB, slot = index % NSLOT;
+                const uint32_t index = given / SUB, turn = given % SUB, slot = index % NSLOT;
                 const uint32_t sub = G::NLD == 2 ? lw : turn;
                 const uint32_t base = smb + G::ring_off + slot * G::PIECE;
                 if (turn == 0 && index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint2 x0 = at_codes<M>(raw[i].x, C{}), x1 = at_codes<M>(raw[i].y, C{});
-                    const uint2 x2 = at_codes<M>(raw[i].z, C{}), x3 = at_codes<M>(raw[i].w, C{});
+                    const uint2 x0 = at_codes<M>(raw[0][i].x, C{}), x1 = at_codes<M>(raw[0][i].y, C{});
+                    const uint2 x2 = at_codes<M>(raw[0][i].z, C{}), x3 = at_codes<M>(raw[0][i].w, C{});
                     uint32_t d0, d1;
-                    if (raw_kind == 1) {
+                    if (kind[0] == 1) {
                         const uint32_t r = lt / KU + i * (128 / KU), c = sub * 8 + 2 * (lt % KU);
                         d0 = k_at(r, c);
                         d1 = k_at(r, c + 1);
@@ -948,7 +948,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 fence_proxy_async();
                 __syncwarp();
                 if (turn + 1 == SUB && lane == 0) at_arrive(b_full + 8 * slot);
-                raw_kind = 0;
+                ++given;
             };
             for (;; done()) {
                 const AtSeg& g = take();
@@ -968,45 +968,60 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         now[i] = make_uint4(0, 0, 0, 0);
                         if (r != AT_NONE) now[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
                     }
-                    convert();
+                    if (kind[0]) convert();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) raw[i] = now[i];
-                    raw_kind = is_v ? 2 : 1;
-                    ++subs;
+                    for (int i = 0; i < 4; ++i) {
+                        raw[0][i] = raw[1][i];
+                        raw[1][i] = now[i];
+                    }
+                    kind[0] = kind[1];
+                    kind[1] = is_v ? 2 : 1;
                 };
                 auto page_of = [&](uint32_t kt) -> int32_t {
                     const int32_t key = (int32_t)(kt * AT_KEYS + lt);
                     return key < lo || key >= hi ? -1 : __ldg(table + (key >> a.pages.page_shift));
                 };
-                int32_t page = n ? page_of(k0) : -1;
                 uint32_t kst = stage;
-                // the row numbers and scales of key tile t into stage kst
-                auto resolve = [&](uint32_t t) {
-                    const int32_t key = (int32_t)((k0 + t) * AT_KEYS + lt);
-                    const bool in = key >= lo && key < hi;
-                    uint32_t r = AT_NONE;
-                    if (in) {
-                        const uint64_t slot = ((uint64_t)(uint32_t)page << a.pages.page_shift) +
-                                              ((uint32_t)key & ((1u << a.pages.page_shift) - 1));
-                        if (page < 0 || slot >= a.pages.slots) atomicOr(err, SERVE_ERR_PAGE);
-                        else r = (uint32_t)page_row(a.pages, slot, head);
+                // A thread a key, each step a tile ahead of the next: its page, then its
+                // row's number and scales, then what the others need of them.
+                auto row_of = [&](uint32_t kt, int32_t page) -> uint32_t {
+                    const int32_t key = (int32_t)(kt * AT_KEYS + lt);
+                    if (key < lo || key >= hi) return AT_NONE;
+                    const uint64_t slot = ((uint64_t)(uint32_t)page << a.pages.page_shift) +
+                                          ((uint32_t)key & ((1u << a.pages.page_shift) - 1));
+                    if (page < 0 || slot >= a.pages.slots) {
+                        atomicOr(err, SERVE_ERR_PAGE);
+                        return AT_NONE;
+                    }
+                    return (uint32_t)page_row(a.pages, slot, head);
+                };
+                int32_t page = -1;
+                uint32_t r = AT_NONE;
+                float ks = 0.0f, vs = 0.0f;
+                auto fetch = [&](uint32_t t) {  // row and scales of tile t, page of the one after
+                    r = t < n ? row_of(k0 + t, page) : AT_NONE;
+                    if (lw == 0 && r != AT_NONE) {
+                        ks = a.pages.ks[r];
+                        vs = a.pages.vs[r];
                     }
                     if (t + 1 < n) page = page_of(k0 + t + 1);
+                };
+                if (n) {
+                    page = page_of(k0);
+                    fetch(0);
+                }
+                // the row numbers and scales of key tile t into stage kst
+                auto resolve = [&](uint32_t t) {
                     if (lw == 0) {
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 512 + lt * 4), "r"(r) : "memory");
-                    float* sc = reinterpret_cast<float*>(sm + G::sc_off) + kst * 384;
-                    float ks = 0.0f, lv = 0.0f, rv = in ? 1.0f : 0.0f;
-                    if (r != AT_NONE) {
-                        ks = a.pages.ks[r] * a.scale_log2;
-                        const float vs = a.pages.vs[r];
-                        lv = log2f(vs);
-                        rv = 1.0f / vs;
-                    }
-                    sc[lt] = ks;
-                    sc[128 + lt] = lv;
-                    sc[256 + lt] = rv;
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 512 + lt * 4), "r"(r) : "memory");
+                        float* sc = reinterpret_cast<float*>(sm + G::sc_off) + kst * 384;
+                        const bool has = r != AT_NONE;  // a missing page: scores and values of zero
+                        sc[lt] = has ? ks * a.scale_log2 : 0.0f;
+                        sc[128 + lt] = has ? log2f(vs) : 0.0f;
+                        sc[256 + lt] = has ? 1.0f / vs : 1.0f;
                     }
                     asm volatile("bar.sync 1, %0;" ::"n"(128 * G::NLD) : "memory");
+                    fetch(t + 1);
                 };
                 for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) {
                     resolve(t);
@@ -1022,7 +1037,14 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         kst = kst + 1 == NSTAGE ? 0 : kst + 1;
                     }
                 }
-                convert();
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (kind[0]) convert();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) raw[0][i] = raw[1][i];
+                    kind[0] = kind[1];
+                    kind[1] = 0;
+                }
             }
         }
     } else {
