@@ -168,7 +168,7 @@ xp_status launch_tiles(const char* who, const ServeAttnArgs& a, void* scratch, c
             TRY(row_map(who, &vm, type, 128, 2, a.v.data, G::D, n, vs, vbox));
         }
     }
-    cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, false, a, w, qm, km, vm);
+    cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(G::THREADS), G::smem, st, 1, true, a, w, qm, km, vm);
     if (e == cudaSuccess)
         e = launch_ex(attn_join_kernel<T, W, G::ROWS>, dim3(ctas, G::ROWS / 32 * W), dim3(256), 0, st, 1, true, a, w, ctas);
     if (e != cudaSuccess) return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
@@ -202,8 +202,9 @@ xp_status launch_few(const char* who, const ServeAttnArgs& a, void* scratch, cud
     TRY(row_map(who, &km, type, G::RB < 128 ? 64 : 128, sizeof(C), a.pages.k, G::D, n, stride, box));
     TRY(row_map(who, &vm, type, G::RB < 128 ? 64 : 128, sizeof(C), a.pages.v, G::D, n, stride, box));
     const uint32_t ctas = std::min<uint32_t>((uint32_t)sm_count() * G::CTAS, most);
-    kernel<<<ctas, 128, G::smem, st>>>(a, w, km, vm);
-    return launched(who);
+    if (cudaError_t e = launch_ex(kernel, dim3(ctas), dim3(128), G::smem, st, 1, true, a, w, km, vm); e != cudaSuccess)
+        return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    return XP_OK;
 }
 
 template <class F> xp_status for_type(uint32_t dtype, F f) {

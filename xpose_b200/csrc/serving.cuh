@@ -117,7 +117,7 @@ XP_DEV void rope_angle(const RopeArg& r, int32_t pos, uint32_t i, float& c, floa
 // of 32 bytes (a whole sector; two of 16 took 75 us where this takes 53, 16381
 // tokens x 32 heads of 128 in bf16).
 template <class T, int VP>
-__global__ void __launch_bounds__(256) rope_rows_kernel(RowsArg out, RowsArg in, RopeArg r, uint32_t tokens,
+__global__ void __launch_bounds__(256, 3) rope_rows_kernel(RowsArg out, RowsArg in, RopeArg r, uint32_t tokens,
                                                         uint32_t heads, uint32_t dim, uint32_t hpt, uint32_t nunits,
                                                         bool copy_tail, bool side) {
     const uint32_t chunks = (heads + hpt - 1) / hpt;

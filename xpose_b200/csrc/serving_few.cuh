@@ -201,6 +201,8 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
         s_dead = 0;
     }
     uint32_t part_phase = 0;
+    pdl_launch_dependents();
+    pdl_wait();  // everything above may run under the kernel before this one
     fw_make_plan<G::SHIFT>(a, s_sums, &s_plan);
     // The CTA's items. One thread makes them two ahead, so that the ring can
     // run on into the next item while this one's sums are added.

@@ -511,7 +511,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     // which the swizzled layouts need, without a byte lost
     extern __shared__ __align__(1024) unsigned char sm[];
     const uint32_t smb = smem_u32(sm);
-    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 13 + 2 * NSEG;
+    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 15 + 2 * NSEG;
     struct Small {
         AtPlan plan;
         AtSeg segs[NSEG];
@@ -536,7 +536,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     const uint32_t b_seg = b_o + 16, b_free = b_seg + NSEG * 8;  // [NSEG] a row tile given, done with
     const uint32_t b_qfree = b_free + NSEG * 8;     // [NQ] Q multiplied for the last time
     const uint32_t b_qh = b_qfree + 16;             // [NQ] ... made fp16
-    const uint32_t b_end = b_qh + 16;               // products in flight after a failed wait
+    const uint32_t b_ph = b_qh + 16;                // [2] P's first 64 keys made (b_p: all), by S buffer
+    const uint32_t b_end = b_ph + 16;               // products in flight after a failed wait
 
     if (smb & 1023) {  // cannot be multiplied from
         if (tid == 0) atomicOr(a.err, SERVE_ERR_WAIT);
@@ -561,7 +562,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             mbar_init(m + 8 + i, 1);
             mbar_init(m + 8 + NSEG + i, NQ * 4 + G::NLD * 4 + 2);
         }
-        for (int i = 0; i < 5; ++i) mbar_init(m + 8 + 2 * NSEG + i, i == 2 || i == 3 ? 4 : 1);
+        for (int i = 0; i < 7; ++i) mbar_init(m + 8 + 2 * NSEG + i, i >= 2 && i < 6 ? 4 : 1);
         fence_mbar_init();
         s_dead = 0;
         for (int i = 0; i < 4; ++i) s_bad[i] = 0;
@@ -570,6 +571,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&small.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    pdl_wait();  // everything above may run under the kernel before this one
     at_clear<T, D>(a, G::THREADS);
     at_make_plan<G::THREADS>(a, w, reinterpret_cast<uint32_t*>(sm), s_sums, &s_plan);
     at_fence_before();
@@ -757,11 +759,11 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         p[j / 2 + 1] = at_pack<M>(e1.x, e1.y);
                     }
                     at_st32(s_tm + half * 32, p);
+                    at_wait_st();
+                    at_fence_before();
+                    __syncwarp();
+                    if (lane == 0) at_arrive((half ? b_p : b_ph) + 8 * buf);  // a half is multiplied while the other is made
                 }
-                at_wait_st();
-                at_fence_before();
-                __syncwarp();
-                if (lane == 0) at_arrive(b_p + 8 * buf);
                 ++npv;
                 stage = stage + 1 == NSTAGE ? 0 : stage + 1;
             }
@@ -1183,8 +1185,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         // O += P V of key tile t - LAG; pieces arrive K(0) .. K(LAG - 1), V(0), K(LAG), V(1), ..
                         const uint32_t tv = t - G::LAG;
                         uint32_t slot = (base + (min(n, t) + tv) * G::NP) % NSLOT;
-                        at_wait(b_p + 8 * buf, p_phase >> buf & 1, &s_dead, err);
-                        p_phase ^= 1u << buf;
+                        at_wait(b_ph + 8 * buf, p_phase >> buf & 1, &s_dead, err);
 #pragma unroll
                         for (int c = 0; c < G::NP; ++c) {
                             const bool look = !G::Q8 && first && at_look(a, lo, hi, p0, (k0 + tv) * AT_KEYS + c * G::VKEYS, G::VKEYS);
@@ -1195,13 +1196,26 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                                 at_wait(b_full + 8 * slot, phase >> slot & 1, &s_dead, err);
                                 phase ^= 1u << slot;
                             }
-                            at_fence_after();
                             const uint32_t bd = at_desc_lo(ring + slot * G::PIECE, G::VKEYS * 128);
-                            if (lead) {
+                            // P's first 64 keys, then the others (with two pieces: the second)
+                            auto pv = [&](int k0, int k1) {
 #pragma unroll
-                                for (int k = 0; k < G::VKEYS / 16; ++k)
+                                for (int k = k0; k < k1; ++k)
                                     at_mma_ts(tmem + 256 + qi * D, tmem + buf * 128 + (c * G::VKEYS + k * 16) / 2,
                                               at_desc(bd + k * (2048 >> 4)), ipv, c || k ? 1u : tv);
+                            };
+                            if (c == 0) {
+                                at_fence_after();
+                                if (lead) pv(0, 4);
+                                __syncwarp();
+                            }
+                            if (c == G::NP - 1) {
+                                at_wait(b_p + 8 * buf, p_phase >> buf & 1, &s_dead, err);
+                                p_phase ^= 1u << buf;
+                                at_fence_after();
+                                if (lead) pv(G::NP == 1 ? 4 : 0, G::VKEYS / 16);
+                            }
+                            if (lead) {
                                 if (last) at_commit(b_empty + 8 * slot);
                                 if (c == G::NP - 1) at_commit(b_o + 8 * qi);
                             }
@@ -1260,6 +1274,7 @@ template <class T, int W, int ROWS>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__ AtWork w,
                                                         uint32_t ctas) {
     constexpr int D = 64 * W;
+    pdl_launch_dependents();
     pdl_wait();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
     const uint4 head = __ldcg(reinterpret_cast<const uint4*>(w.heads) + 2 * c0 + 1);
