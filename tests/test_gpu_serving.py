@@ -584,3 +584,119 @@ def test_no_tokens_is_no_work(scratch):
     S.kv_read(kp, vp, ks, vs, x[1], x[2], ints([], torch.int64))
     S.attention_paged(x[0], x[0], kp, vp, ks, vs, ints([[0], [0]]), ints([3, 0]), ints([0, 0, 0]), 1, scratch)
     torch.cuda.synchronize()
+
+
+# ---- layouts, and what only some kernels meet ------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_packed_layouts_and_shared_heads(scratch, dim):
+    """Heads before tokens, one k and v head broadcast to several, and rows far apart."""
+    g = gen(31)
+    n, lens = 333, [200, 133]
+    q = randn(g, 6, n, dim, dtype=BF16).transpose(0, 1)
+    k, v = (randn(g, n, 1, dim, dtype=BF16).expand(n, 3, dim) for _ in range(2))
+    assert k.stride(1) == 0
+    far = torch.zeros(n, 9, dim, dtype=BF16, device="cuda")
+    out, lse = far[:, 2:8], torch.empty(n, 6, device="cuda")
+    S.attention_packed(out, q, k, v, starts_of(lens), scratch, lse=lse)
+    at = 0
+    for m in lens:
+        s = slice(at, at + m)
+        want, mag, wlse = R.attend(q[s], k[s], v[s], 0, 0, dim ** -0.5)
+        check_attention(out[s], lse[s], want, mag, wlse, BF16, m, 5.0)
+        at += m
+    assert not far[:, :2].any() and not far[:, 8:].any()
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads", [(1, 128, 1), (3, 100, 2), (40, 64, 1), (200, 33, 33)])
+def test_paged_unusual_groups(scratch, rows, heads, kv_heads):
+    run_paged(scratch, [rows, 1], [rows + 300, 77], heads, kv_heads, 64, 16, I8, BF16, seed=rows)
+    run_paged(scratch, [rows], [rows + 140], heads, kv_heads, 128, 32, F16, F16, window=50, seed=rows + 1)
+
+
+@pytest.mark.parametrize("cache", [I8, FP8])
+@pytest.mark.parametrize("size", [1e-30, 1e-3, 3e4, 1e30])
+@pytest.mark.parametrize("n", [1, 50])
+def test_paged_queries_of_any_size(scratch, cache, size, n):
+    """bf16 queries far outside fp16's range over 8-bit pages: the scale of the scores makes up for it."""
+    g = gen(33)
+    kp, vp, ks, vs = make_cache(g, 40, 16, 1, 256, cache)
+    table = torch.randperm(40, generator=g, device="cuda", dtype=torch.int32)[None].contiguous()
+    q = (torch.randn(n, 4, 256, generator=g, device="cuda") * size).to(BF16)
+    q[0, 1] = 0
+    out, lse = torch.empty_like(q), torch.empty(n, 4, device="cuda")
+    scale = 0.0625 / size
+    S.attention_paged(out, q, kp, vp, ks, vs, table, ints([600]), ints([0, n]), n, scratch, scale=scale, lse=lse)
+    i = torch.arange(600, device="cuda")
+    slots = table[0, i // 16].long() * 16 + i % 16
+    want, mag, wlse = R.attend(q, R.rows_of(kp, ks, slots), R.rows_of(vp, vs, slots), 600 - n, 0,
+                               float(torch.tensor(scale, dtype=F32)))
+    check_attention(out, lse, want, mag, wlse, BF16, 600, float(vs.max()) * TOPS[cache])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,window", [(4, 0), (4, 100), (60, 0), (60, 100), (1, 100)])
+def test_paged_what_is_masked_does_not_matter(scratch, dtype, dim, n, window):
+    """Infinities and NaN in 16-bit pages reach exactly the new tokens that see them."""
+    g = gen(35)
+    kv, page = 700, 16
+    kp, vp, ks, vs = make_cache(g, 44, page, 1, dim, dtype)
+    table = torch.arange(44, dtype=torch.int32, device="cuda")[None].contiguous()
+    at = lambda j: (j // page, 0, j % page)  # noqa: E731
+    vp[at(698)][3], vp[at(699)][dim - 1] = math.nan, math.inf
+    kp[at(697)][1] = math.nan
+    vp[at(kv - n - window + 2 if window else 5)][0] = -math.inf
+    q = randn(g, n, 2, dim, dtype=dtype)
+    out = torch.empty_like(q)
+    S.attention_paged(out, q, kp, vp, ks, vs, table, ints([kv]), ints([0, n]), n, scratch, window=window)
+    slots = torch.arange(kv, device="cuda")
+    want, mag, _ = R.attend(q, R.rows_of(kp, ks, slots), R.rows_of(vp, vs, slots), kv - n, window, dim ** -0.5)
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), fine)
+    assert ((out.double() - want).abs() <= R.attention_bound(want, mag, dtype, kv, 6.0))[fine].all()
+
+
+@pytest.mark.parametrize("n", [1, 4, 30])
+def test_paged_rows_written_as_nan(scratch, n):
+    """A token whose values were not finite makes those who see it NaN, and nobody else."""
+    g = gen(37)
+    kp, vp, ks, vs = S.new_pages(20, 16, 1, 64, I8)
+    k, v = randn(g, 300, 1, 64), randn(g, 300, 1, 64)
+    v[290, 0, 9] = math.inf
+    S.kv_write(kp, vp, ks, vs, k, v, torch.arange(300, device="cuda"))
+    q = randn(g, n, 2, 64, dtype=F16)
+    out = torch.empty_like(q)
+    for length in (290, 292, 300):
+        S.attention_paged(out, q, kp, vp, ks, vs, torch.arange(20, dtype=torch.int32, device="cuda")[None].contiguous(),
+                          ints([length]), ints([0, n]), n, scratch)
+        sees = torch.arange(length - n, length, device="cuda") >= 290
+        assert torch.equal(torch.isnan(out).all(-1).all(-1), sees) and torch.isfinite(out[~sees]).all()
+
+
+def test_many_sequences_at_once(scratch):
+    r = random.Random(9)
+    kv = [r.choice([0, 1, 3, 20, 150]) for _ in range(1200)]
+    run_paged(scratch, [min(1, n) for n in kv], kv, 2, 1, 64, 8, F16, F16, seed=10)
+    run_paged(scratch, [min(n, r.choice([1, 9, 20])) for n in kv], kv, 2, 1, 64, 8, F16, F16, seed=11)
+
+
+def test_python_refusals():
+    x = torch.zeros(4, 2, 64, dtype=F16)
+    c = x.cuda()
+    kp, vp, ks, vs = S.new_pages(4, 16, 2, 64, I8)
+    turns, _ = S.rope_turns(64, 1e4)
+    pos, slots = ints([0, 1, 2, 3]), ints([0, 1, 2, 3], torch.int64)
+    bad = [lambda: S.rope_rows(x, x, pos, turns), lambda: S.rope_rows(c, c, pos.long(), turns),
+           lambda: S.rope_rows(c, c, pos[:3], turns), lambda: S.rope_rows(c, c, pos, turns, layout="other"),
+           lambda: S.rope_rows(c[:, :, ::2], c[:, :, ::2], pos, turns), lambda: S.rope_rows(c[0], c[0], pos, turns),
+           lambda: S.rope_rows(c.double(), c.double(), pos, turns), lambda: S.rope_rows(None, c, pos, turns),
+           lambda: S.kv_write(kp, vp, None, None, c, c, slots), lambda: S.kv_write(kp, vp[:2], ks, vs, c, c, slots),
+           lambda: S.kv_write(kp, vp, ks, vs, c, c, pos), lambda: S.kv_read(kp, vp, ks[:2], vs, c, c, slots),
+           lambda: S.kv_write(kp, vp, ks, vs, c, c, slots, positions=None, turns=turns),
+           lambda: S.attention_packed(c, c, c, c, ints([0, 4]), torch.zeros(100, dtype=torch.uint8, device="cuda")),
+           lambda: S.attention_paged(c, c, kp, vp, ks, vs, ints([0, 1]), ints([4]), ints([0, 4]), 4, S.new_scratch()),
+           lambda: S.attention_paged(c, c, kp, vp, ks, vs, ints([[0, 1]]), ints([4]), ints([0, 2, 4]), 4, S.new_scratch()),
+           lambda: S.attention_paged(c, c, kp, vp, ks, vs, ints([[0, 1]]), ints([4]), ints([0, 4]), -1, S.new_scratch())]
+    for f in bad:
+        with pytest.raises(S.XpError):
+            f()

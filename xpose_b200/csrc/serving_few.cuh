@@ -484,10 +484,12 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
             for (int b = 0; b < KG; ++b) rv[b][0] = rv[b][1] = 1.0f;
             if constexpr (Q8) {
                 // a lane a key: its scale, log2 of v's and its inverse; where there
-                // is no key or no page (codes and scales of zero) the value is zero
+                // is no key or no page (codes and scales of zero) the value is zero. A scale
+                // of NaN makes the weights of those who see the key NaN; the others' weight
+                // of 0 must not meet it
                 const uint32_t sc = scales + stage * (2 * KPS * 4) + (lane & (KPS - 1)) * 4;
                 const float ks0 = __uint_as_float(at_lds(sc)), vs0 = __uint_as_float(at_lds(sc + KPS * 4));
-                const float lv0 = vs0 == 0.0f ? 0.0f : fw_lg2(vs0), rv0 = vs0 == 0.0f ? 1.0f : fw_rcp(vs0);
+                const float lv0 = vs0 == 0.0f ? 0.0f : fw_lg2(vs0), rv0 = vs0 == 0.0f ? 1.0f : vs0 == vs0 ? fw_rcp(vs0) : 0.0f;
 #pragma unroll
                 for (int b = 0; b < KG; ++b)
 #pragma unroll

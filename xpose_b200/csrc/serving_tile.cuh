@@ -1020,7 +1020,9 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         const bool has = r != AT_NONE;  // a missing page: scores and values of zero
                         sc[lt] = has ? ks * a.scale_log2 : 0.0f;
                         sc[128 + lt] = has ? log2f(vs) : 0.0f;
-                        sc[256 + lt] = has ? 1.0f / vs : 1.0f;
+                        // a scale of NaN makes the weights of those who see the key NaN; the others'
+                        // weight of 0 must not meet it
+                        sc[256 + lt] = !has ? 1.0f : vs == vs ? 1.0f / vs : 0.0f;
                     }
                     asm volatile("bar.sync 1, %0;" ::"n"(128 * G::NLD) : "memory");
                     fetch(t + 1);
