@@ -522,7 +522,8 @@ xp_status xp_rope_rows(void* stream, const xp_rows* out, const xp_rows* in, cons
  * is skipped, so -1 marks padding; no slot twice), k rotated first when `rope`
  * is not NULL. 8-bit pages: top = max |x| of the row (at least 2^-100), code =
  * x * (Q / top) rounded to nearest even, scale = top / Q, Q = 127 or 448; a
- * row with an infinity or NaN gets a NaN scale and reads back as NaN. */
+ * row with an infinity or NaN gets a NaN scale and reads back as NaN. Rows are
+ * aligned to 8 values; rot_dim is a multiple of 8. */
 xp_status xp_kv_write(void* stream, const xp_pages* pages, const xp_rows* k, const xp_rows* v, const int64_t* slots,
                       const xp_rotary* rope);
 /* The rows in slots[0 .. tokens - 1] as values; a slot outside the cache gives
@@ -531,17 +532,19 @@ xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, cons
 /* Scratch of the two attentions: 16-byte aligned, zeroed once, one call at a
  * time. Its uint32 at byte 4 is a sticky error word: 1 = a length past its
  * table row (clamped), 2 = a page outside the cache (its rows read as zeros),
- * 4 = a wait ran out, 8 = a sequence had more than q_most new tokens (the
- * rest were left out). */
+ * 4 = a wait ran out (the output is unspecified; zero the scratch again), 8 = a
+ * sequence had more than q_most new tokens (the rest were left out). */
 #define XP_SERVING_SCRATCH_BYTES (48u << 20)
 /* Causal attention over whole prompts packed one after the other: sequence b
  * is tokens starts[b] .. starts[b + 1] - 1 (device, [batch + 1]), and a token
  * attends to those of its own sequence up to itself, the last `window` of them
  * when window is not 0. Head h uses k and v head h / (heads / kv_heads).
  * scale 0 = 1 / sqrt(dim). q, k, v and out of one type, F16 or BF16; dim 64,
- * 128 or 256. Data and strides of 16 bytes. lse (may be NULL): [tokens][heads]
+ * 128 or 256; at most 128 heads a kv head and 8192 sequences. Data and strides
+ * are multiples of 16 bytes; q, k and v have positive ones, but k and v may
+ * have a head stride of 0 (one head for all). lse (may be NULL): [tokens][heads]
  * natural log of the sum of the exponentiated scores, -inf for a token in no
- * sequence, whose output is zero. What other sequences and later tokens hold,
+ * sequence (before starts[0], or from starts[batch] on), whose output is zero. What other sequences and later tokens hold,
  * NaN included, does not matter. */
 xp_status xp_attention_packed(void* stream, const xp_rows* out, const xp_rows* q, const xp_rows* k, const xp_rows* v,
                               const int32_t* starts, uint32_t batch, uint32_t window, float scale, float* lse,
