@@ -214,6 +214,13 @@ XP_DEV float2 at_add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
 }
+XP_DEV float2 at_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
 template <class T> XP_DEV uint32_t at_pack(float lo, float hi) {
     uint32_t r;
     if constexpr (std::is_same_v<T, bf16>) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -789,22 +796,17 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             T* const op = static_cast<T*>(a.out.data) + (int64_t)orow * a.out.ts + (int64_t)ohead * a.out.hs;
             // a lane stores its own row, 32 bytes (a sector) at a time where rows allow it
             const bool wide = ((reinterpret_cast<uintptr_t>(a.out.data) | (uintptr_t)(a.out.ts * 2) | (uintptr_t)(a.out.hs * 2)) & 31) == 0;
+            if (bad) {
+                // infinities and NaN of v were left out of the products of pieces
+                // where not every row sees every key: they go to the rows that do
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                float o[32];
-                if (g.n) {
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
                     at_ld32(o_tm + c, reinterpret_cast<uint32_t*>(o));
                     at_wait_ld();
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0.0f;
-                }
-                if (bad && real) {
-                    // infinities and NaN of v were left out of the products of tiles
-                    // where not every row sees every key: they go to the rows that do
                     for (uint32_t t = 0; t < g.n * G::NP; ++t) {
                         const uint32_t key0 = g.k0 * AT_KEYS + t * G::VKEYS;
-                        if (!at_look(a, g.lo, g.hi, g.p0, key0, G::VKEYS)) continue;
+                        if (!real || !at_look(a, g.lo, g.hi, g.p0, key0, G::VKEYS)) continue;
                         const int32_t j0 = max((int32_t)key0, klo);
                         const int32_t j1 = min(min((int32_t)(key0 + G::VKEYS), khi), g.hi);
                         for (int32_t j = j0; j < j1; ++j) {
@@ -824,27 +826,50 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                             }
                         }
                     }
+                    __syncwarp();
+                    at_st32(o_tm + c, reinterpret_cast<uint32_t*>(o));
+                    at_wait_st();
                 }
-                if (whole) {
-                    uint4 x[4];
+            }
+            // few instructions: they run once a row tile, cold
+            if (whole) {
+                const float2 inv2 = {inv, inv};
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    if (g.n) {
+                        at_ld32(o_tm + c, reinterpret_cast<uint32_t*>(o));
+                        at_wait_ld();
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[i].x = at_pack<T>(o[8 * i] * inv, o[8 * i + 1] * inv);
-                        x[i].y = at_pack<T>(o[8 * i + 2] * inv, o[8 * i + 3] * inv);
-                        x[i].z = at_pack<T>(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
-                        x[i].w = at_pack<T>(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
+                        for (int i = 0; i < 32; ++i) o[i] = 0.0f;
                     }
+                    uint32_t x[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 y = at_mul2({o[2 * i], o[2 * i + 1]}, inv2);
+                        x[i] = at_pack<T>(y.x, y.y);
+                    }
+                    uint4* const p = reinterpret_cast<uint4*>(op + c);
                     if (real && wide) {
-                        at_stg32(op + c, x[0], x[1]);
-                        at_stg32(op + c + 16, x[2], x[3]);
+                        at_stg32(p, make_uint4(x[0], x[1], x[2], x[3]), make_uint4(x[4], x[5], x[6], x[7]));
+                        at_stg32(p + 2, make_uint4(x[8], x[9], x[10], x[11]), make_uint4(x[12], x[13], x[14], x[15]));
                     } else if (real) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(op + c)[i] = x[i];
+                        for (int i = 0; i < 4; ++i) p[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
                     }
-                } else if (real) {
+                }
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    at_ld32(o_tm + c, reinterpret_cast<uint32_t*>(o));
+                    at_wait_ld();
                     float4* pp = reinterpret_cast<float4*>(part) + (size_t)(c / 4) * G::ROWS + wg * 128 + row;
+                    if (real) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) pp[(size_t)(i / 4) * G::ROWS] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 32; i += 4) pp[(size_t)(i / 4) * G::ROWS] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
                 }
             }
             at_fence_before();
