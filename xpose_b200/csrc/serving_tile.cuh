@@ -35,9 +35,10 @@
 // two or more CTAs share leaves partial sums (O, m, l) that a second, small
 // launch joins in a fixed order.
 //
-// Measured: 2048 tokens over 32768 keys, 16 / 2 heads of 128, bf16: 489 us, 1.09
-// PFLOP/s, bound by the softmax of a row tile, which its own products wait for;
-// a prompt of 8192, 4 / 1 heads of 256: 138 us, 0.99 PFLOP/s, bound by shared
+// Measured: 2048 tokens over 32768 keys, 16 / 2 heads of 128, bf16: 484 us, 1.10
+// PFLOP/s (440 to 505 us as the power limit has it), bound by the softmax of a
+// row tile, which its own products wait for;
+// a prompt of 8192, 4 / 1 heads of 256: 141 us, 0.97 PFLOP/s, bound by shared
 // memory (320 KB of operands and copies for 2048 cycles of products); 12 prompts
 // of 33 to 2048, 32 / 8 heads of 128, fp16: 115 us, 0.62 PFLOP/s.
 #pragma once
