@@ -18,8 +18,7 @@ namespace {
         if (!(cond)) return fail(XP_ERR_INVALID, __VA_ARGS__);  \
     } while (0)
 
-xp_status launched(const char* who) {
-    const cudaError_t e = cudaGetLastError();
+xp_status launched(const char* who, cudaError_t e) {
     if (e == cudaSuccess) return XP_OK;
     return fail(XP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }
@@ -303,9 +302,8 @@ xp_status xp_rope_rows(void* stream, const xp_rows* out, const xp_rows* in, cons
             auto k = wide ? rope_rows_kernel<T, 16 / sizeof(T)> : rope_rows_kernel<T, 1>;
             RopeArg r = rope_arg(rope);
             r.positions += t0;
-            k<<<grid, 256, 0, (cudaStream_t)stream>>>(rows_arg(out, t0), rows_arg(in, t0), r, n, in->heads, in->dim, hpt,
-                                                      units, copy, side);
-            return launched(who);
+            return launched(who, launch_ex(k, dim3(grid), dim3(256), 0, (cudaStream_t)stream, 1, true, rows_arg(out, t0),
+                                           rows_arg(in, t0), r, n, in->heads, in->dim, hpt, units, copy, side));
         });
     });
 }
@@ -328,9 +326,9 @@ xp_status xp_kv_write(void* stream, const xp_pages* pages, const xp_rows* k, con
                 return for_dim(k->dim, [&](auto d) {
                     RopeArg r = rope_arg(rope);
                     if (rope) r.positions += t0;
-                    kv_write_kernel<decltype(t), decltype(c), d.value><<<grid, 256, 0, (cudaStream_t)stream>>>(
-                        pages_arg(pages), rows_arg(k, t0), rows_arg(v, t0), slots + t0, n, r, rope != nullptr);
-                    return launched(who);
+                    return launched(who, launch_ex(kv_write_kernel<decltype(t), decltype(c), d.value>, dim3(grid), dim3(256),
+                                                   0, (cudaStream_t)stream, 1, true, pages_arg(pages), rows_arg(k, t0),
+                                                   rows_arg(v, t0), slots + t0, n, r, rope != nullptr));
                 });
             });
         });
@@ -353,9 +351,9 @@ xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, cons
         return for_type(k->dtype, [&](auto t) {
             return for_cache(pages->dtype, [&](auto c) {
                 return for_dim(k->dim, [&](auto d) {
-                    kv_read_kernel<decltype(t), decltype(c), d.value><<<grid, 256, 0, (cudaStream_t)stream>>>(
-                        pages_arg(pages), rows_arg(k, t0), rows_arg(v, t0), slots + t0, n);
-                    return launched(who);
+                    return launched(who, launch_ex(kv_read_kernel<decltype(t), decltype(c), d.value>, dim3(grid), dim3(256),
+                                                   0, (cudaStream_t)stream, 1, true, pages_arg(pages), rows_arg(k, t0),
+                                                   rows_arg(v, t0), slots + t0, n));
                 });
             });
         });

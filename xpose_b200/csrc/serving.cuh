@@ -89,6 +89,22 @@ template <class T> XP_DEV void raw_put2(Raw32& r, int i, float x, float y) {  //
     }
 }
 
+// Words that other kernels write, positions and lengths and the like. Not by
+// the read-only path: a grid that starts under the kernel before it is not
+// alone with them, even if it reads them only once that one has ended. In order
+// with pdl_wait(), as volatile.
+XP_DEV int32_t ld_now(const int32_t* p) {
+    int32_t x;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(x) : "l"(p));
+    return x;
+}
+template <class T> XP_DEV T ld_now(const T* p) {
+    static_assert(sizeof(T) == 8);
+    T x;
+    asm volatile("ld.global.b64 %0, [%1];" : "=l"(x) : "l"(p));
+    return x;
+}
+
 struct RowsArg {
     void* data;
     int64_t ts, hs;  // token and head strides, elements
@@ -104,7 +120,7 @@ struct RopeArg {
 
 // cos and sin of pair i at position `pos`, times the magnitude
 XP_DEV void rope_angle(const RopeArg& r, int32_t pos, uint32_t i, float& c, float& s) {
-    const long long part = (long long)((unsigned long long)(long long)pos * __ldg(r.turns + i));
+    const long long part = (long long)((unsigned long long)(long long)pos * ld_now(r.turns + i));
     const float half_turns = (float)(int32_t)(part >> 32) * 0x1p-31f;
     sincospif(half_turns, &s, &c);
     c *= r.magnitude;
@@ -124,6 +140,8 @@ template <class T, int VP>
 __global__ void __launch_bounds__(256, 3) rope_rows_kernel(RowsArg out, RowsArg in, RopeArg r, uint32_t tokens,
                                                         uint32_t heads, uint32_t dim, uint32_t hpt, uint32_t nunits,
                                                         bool copy_tail, bool side) {
+    pdl_launch_dependents();
+    pdl_wait();
     const uint32_t chunks = (heads + hpt - 1) / hpt;
     const uint32_t id = blockIdx.x * 256 + threadIdx.x, rest = id / nunits, unit = id - rest * nunits;
     const uint32_t t = rest / chunks, h0 = (rest - t * chunks) * hpt;
@@ -133,7 +151,7 @@ __global__ void __launch_bounds__(256, 3) rope_rows_kernel(RowsArg out, RowsArg 
     T* dst = static_cast<T*>(out.data) + (int64_t)t * out.ts + (int64_t)h0 * out.hs;
     const uint32_t nh = min(hpt, heads - h0);
     if (unit < rot_units) {
-        const int32_t pos = __ldg(r.positions + t);
+        const int32_t pos = ld_now(r.positions + t);
         float c[VP], s[VP];
 #pragma unroll
         for (int i = 0; i < VP; ++i) rope_angle(r, pos, unit * VP + i, c[i], s[i]);
@@ -282,9 +300,11 @@ template <class T, class C, int W>
 __global__ void __launch_bounds__(256) kv_write_kernel(PagesArg p, RowsArg k, RowsArg v, const int64_t* slots,
                                                        uint32_t tokens, RopeArg r, bool rotate) {
     constexpr uint32_t DIM = 64 * W, LANES = DIM / 8;
+    pdl_launch_dependents();
+    pdl_wait();
     const uint32_t part = threadIdx.x % LANES, id = (blockIdx.x * 256 + threadIdx.x) / LANES;
     const uint32_t t = id / p.kv_heads, h = id - t * p.kv_heads;
-    const int64_t slot = t < tokens ? __ldg(slots + t) : -1;
+    const int64_t slot = t < tokens ? ld_now(slots + t) : -1;
     const bool live = slot >= 0 && (uint64_t)slot < p.slots;  // others only take part in the shuffles
     uint32_t d[2] = {part * 8, part * 8 + 4};
     const uint32_t n = r.rot / 2;
@@ -307,7 +327,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(PagesArg p, RowsArg k, Ro
             load_f32<4>(vp + d[1], vx + 4);
         }
         if (turns) {
-            const int32_t pos = __ldg(r.positions + t);
+            const int32_t pos = ld_now(r.positions + t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float c, s;
@@ -350,10 +370,12 @@ template <class T, class C, int W>
 __global__ void __launch_bounds__(256) kv_read_kernel(PagesArg p, RowsArg k, RowsArg v, const int64_t* slots,
                                                       uint32_t rows) {
     constexpr uint32_t DIM = 64 * W, PER = DIM / 16;
+    pdl_launch_dependents();
+    pdl_wait();
     const uint32_t id = blockIdx.x * 256 + threadIdx.x, part = id % PER * 16, th = id / PER;
     const uint32_t t = th / p.kv_heads, h = th - t * p.kv_heads;
     if (t >= rows) return;
-    const int64_t slot = __ldg(slots + t);
+    const int64_t slot = ld_now(slots + t);
     const bool has = slot >= 0 && (uint64_t)slot < p.slots;
     const uint64_t row = page_row(p, has ? (uint64_t)slot : 0, h);
     // both sides' codes and scales under way together

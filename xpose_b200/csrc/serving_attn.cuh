@@ -30,12 +30,12 @@ struct ServeAttnArgs {
 struct Seq { uint32_t q0, nq, nkv; };
 XP_DEV Seq seq_of(const ServeAttnArgs& a, uint32_t b) {
     Seq s;
-    const int32_t lo = __ldg(a.starts + b), hi = __ldg(a.starts + b + 1);
+    const int32_t lo = ld_now(a.starts + b), hi = ld_now(a.starts + b + 1);
     s.q0 = (uint32_t)min(max(lo, 0), (int32_t)a.tokens);
     s.nq = (uint32_t)max(min(max(hi, 0), (int32_t)a.tokens) - (int32_t)s.q0, 0);
     if (a.pages.k) {
         const uint64_t most = (uint64_t)a.table_width << a.pages.page_shift;
-        const int32_t n = max(__ldg(a.kv_lens + b), 0);
+        const int32_t n = max(ld_now(a.kv_lens + b), 0);
         s.nkv = (uint32_t)min((uint64_t)n, most);
         if ((uint64_t)n > most) atomicOr(a.err, SERVE_ERR_LENGTH);
         if (s.nq > a.q_most) {

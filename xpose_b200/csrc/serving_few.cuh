@@ -299,7 +299,7 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 const int32_t key = kb + (int32_t)(p * box);
                 uint32_t z = nowhere;  // past the end: zeros
                 if (key < hi && key + (int32_t)box > lo) {
-                    const int32_t page = __ldg(row + (key >> a.pages.page_shift));
+                    const int32_t page = ld_now(row + (key >> a.pages.page_shift));
                     if (page >= 0 && ((uint64_t)(uint32_t)page << a.pages.page_shift) < a.pages.slots)
                         z = (uint32_t)page * a.kv_heads + g.h;
                     else
@@ -313,7 +313,7 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 bool has = key >= lo && key < hi;
                 uint64_t at = 0;
                 if (has) {
-                    const int32_t page = __ldg(row + (key >> a.pages.page_shift));
+                    const int32_t page = ld_now(row + (key >> a.pages.page_shift));
                     at = ((uint64_t)(uint32_t)page << a.pages.page_shift) + ((uint32_t)key & (ps - 1));
                     has = page >= 0 && at < a.pages.slots;
                     at = has ? page_row(a.pages, at, g.h) : 0;

@@ -306,8 +306,8 @@ XP_DEV AtTile at_tile(const Seq& s, uint32_t x, uint32_t tt, uint32_t window, ui
 
 // Zeros for the rows of q that are in no sequence.
 template <class T, int D> XP_DEV void at_clear(const ServeAttnArgs& a, uint32_t threads) {
-    const uint32_t lo = (uint32_t)min(max(__ldg(a.starts), 0), (int32_t)a.tokens);
-    const uint32_t hi = max((uint32_t)min(max(__ldg(a.starts + a.batch), 0), (int32_t)a.tokens), lo);
+    const uint32_t lo = (uint32_t)min(max(ld_now(a.starts), 0), (int32_t)a.tokens);
+    const uint32_t hi = max((uint32_t)min(max(ld_now(a.starts + a.batch), 0), (int32_t)a.tokens), lo);
     const uint64_t n = (uint64_t)(lo + (a.tokens - hi)) * a.heads * (D / 8);
     for (uint64_t i = (uint64_t)blockIdx.x * threads + threadIdx.x; i < n; i += (uint64_t)gridDim.x * threads) {
         const uint32_t d = (uint32_t)(i % (D / 8)) * 8, h = (uint32_t)(i / (D / 8) % a.heads);
@@ -813,7 +813,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         for (int32_t j = j0; j < j1; ++j) {
                             const T* vp;
                             if (a.pages.k) {
-                                const int32_t page = __ldg(a.table + (uint64_t)g.b * a.table_width + (j >> a.pages.page_shift));
+                                const int32_t page = ld_now(a.table + (uint64_t)g.b * a.table_width + (j >> a.pages.page_shift));
                                 const uint64_t sl = ((uint64_t)(uint32_t)page << a.pages.page_shift) + (j & ((1u << a.pages.page_shift) - 1));
                                 if (page < 0 || sl >= a.pages.slots) continue;
                                 vp = static_cast<const T*>(a.pages.v) + page_row(a.pages, sl, g.h) * D + c;
@@ -1000,7 +1000,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t r = at_lds(rows0 + st * 512 + (key0 + r0 + i * step) * 4);
                         now[i] = make_uint4(0, 0, 0, 0);
-                        if (r != AT_NONE) now[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
+                        if (r != AT_NONE) now[i] = __ldcg(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
                     }
                     if (kind[0]) convert();
 #pragma unroll
@@ -1013,7 +1013,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 };
                 auto page_of = [&](uint32_t kt) -> int32_t {
                     const int32_t key = (int32_t)(kt * AT_KEYS + lt);
-                    return key < lo || key >= hi ? -1 : __ldg(table + (key >> a.pages.page_shift));
+                    return key < lo || key >= hi ? -1 : ld_now(table + (key >> a.pages.page_shift));
                 };
                 uint32_t kst = stage;
                 // A thread a key, each step a tile ahead of the next: its page, then its
@@ -1151,7 +1151,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                             y = k & (ps - 1);
                             z = nowhere;
                             if ((int32_t)(k + box) > lo && (int32_t)k < hi) {
-                                const int32_t page = __ldg(table + (k >> a.pages.page_shift));
+                                const int32_t page = ld_now(table + (k >> a.pages.page_shift));
                                 if (page >= 0 && ((uint64_t)(uint32_t)page << a.pages.page_shift) < a.pages.slots)
                                     z = (uint32_t)page * a.kv_heads + head;
                                 else
