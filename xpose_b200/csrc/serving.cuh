@@ -12,7 +12,7 @@
 // codes leave in the same pass.
 //
 // All three are bound by memory: 16381 tokens x 32 heads of 128 rotated in 51 us
-// (5.3 TB/s), 8191 x 8 rows of 128 written in e4m3 and 32768 x 8 read in 53 us (4.8
+// (5.3 TB/s), 8191 x 8 rows of 128 written in e4m3 and 32768 x 8 read in 52 us (4.9
 // TB/s for the two launches); 64 rows take 3 us, a launch.
 #pragma once
 #include <cuda_bf16.h>
