@@ -1,8 +1,10 @@
 // Torch tensors to the serving entry points of include/xp_cuda.h: the checks
 // of xpose_b200/serving.py in C++, because a decode step's kernels take less
 // time than the same checks in Python. Every function returns None, or
-// (status, message) for the caller to raise.
+// (status, message) for the caller to raise. The tensors of a call are all on
+// one device, which is the current one while the call is enqueued.
 #include <Python.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -17,15 +19,31 @@ struct Bad {
 };
 [[noreturn]] void bad(const std::string& m) { throw Bad{m}; }
 
-const at::Tensor& tensor(PyObject* o, const char* name) {
+// The device of one call: that of the first tensor looked at.
+struct Device {
+    int index = -1;
+    c10::cuda::OptionalCUDAGuard guard;
+    // torch's current stream there, for which the device is made the current one
+    void* stream() {
+        guard.set_index((c10::DeviceIndex)index);
+        return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)index).stream();
+    }
+};
+
+const at::Tensor& tensor(Device& d, PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) bad(std::string("'") + name + "' must be a tensor");
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!t.is_cuda()) bad(std::string("'") + name + "' must be a CUDA tensor");
+    const int index = t.device().index();
+    if (d.index < 0) d.index = index;
+    if (index != d.index)
+        bad(std::string("'") + name + "' is on device " + std::to_string(index) + ", others of the call on device " +
+            std::to_string(d.index));
     return t;
 }
 
-xp_rows rows(PyObject* o, const char* name) {
-    const at::Tensor& t = tensor(o, name);
+xp_rows rows(Device& d, PyObject* o, const char* name) {
+    const at::Tensor& t = tensor(d, o, name);
     xp_rows r{};
     switch (t.scalar_type()) {
         case at::kFloat: r.dtype = XP_F32; break;
@@ -47,16 +65,16 @@ xp_rows rows(PyObject* o, const char* name) {
 }
 
 // a contiguous tensor of n values (n < 0: any number)
-void* flat(PyObject* o, const char* name, at::ScalarType type, int64_t n) {
-    const at::Tensor& t = tensor(o, name);
+void* flat(Device& d, PyObject* o, const char* name, at::ScalarType type, int64_t n) {
+    const at::Tensor& t = tensor(d, o, name);
     if (t.scalar_type() != type || !t.is_contiguous() || (n >= 0 && t.numel() != n))
         bad(std::string("'") + name + "' must be contiguous, of type " + c10::toString(type) +
             (n >= 0 ? " and of " + std::to_string(n) + " values" : std::string()));
     return t.data_ptr();
 }
 
-xp_pages pages(PyObject* const* a) {  // k, v, k_scale, v_scale
-    const at::Tensor &k = tensor(a[0], "k_pages"), &v = tensor(a[1], "v_pages");
+xp_pages pages(Device& d, PyObject* const* a) {  // k, v, k_scale, v_scale
+    const at::Tensor &k = tensor(d, a[0], "k_pages"), &v = tensor(d, a[1], "v_pages");
     xp_pages p{};
     switch (k.scalar_type()) {
         case at::kHalf: p.dtype = XP_F16; break;
@@ -78,17 +96,17 @@ xp_pages pages(PyObject* const* a) {  // k, v, k_scale, v_scale
     if (k.element_size() == 1) {
         if (a[2] == Py_None || a[3] == Py_None) bad("8-bit pages need k_scale and v_scale");
         const int64_t n = k.size(0) * k.size(1) * k.size(2);
-        p.k_scale = static_cast<float*>(flat(a[2], "k_scale", at::kFloat, n));
-        p.v_scale = static_cast<float*>(flat(a[3], "v_scale", at::kFloat, n));
+        p.k_scale = static_cast<float*>(flat(d, a[2], "k_scale", at::kFloat, n));
+        p.v_scale = static_cast<float*>(flat(d, a[3], "v_scale", at::kFloat, n));
     }
     return p;
 }
 
-xp_rotary rotary(PyObject* positions, PyObject* turns, PyObject* layout, PyObject* magnitude, PyObject* inverse,
-                 uint32_t tokens) {
+xp_rotary rotary(Device& d, PyObject* positions, PyObject* turns, PyObject* layout, PyObject* magnitude,
+                 PyObject* inverse, uint32_t tokens) {
     xp_rotary r{};
-    r.turns = static_cast<const uint64_t*>(flat(turns, "turns", at::kLong, -1));
-    r.positions = static_cast<const int32_t*>(flat(positions, "positions", at::kInt, tokens));
+    r.turns = static_cast<const uint64_t*>(flat(d, turns, "turns", at::kLong, -1));
+    r.positions = static_cast<const int32_t*>(flat(d, positions, "positions", at::kInt, tokens));
     const int64_t n = THPVariable_Unpack(turns).numel();
     if (n > 0x3FFFFFFF) bad("'turns' is too long");
     r.rot_dim = (uint32_t)(2 * n);
@@ -98,18 +116,16 @@ xp_rotary rotary(PyObject* positions, PyObject* turns, PyObject* layout, PyObjec
     return r;
 }
 
-void* stream_of(PyObject* o) { return c10::cuda::getCurrentCUDAStream(THPVariable_Unpack(o).device().index()).stream(); }
-
-void* scratch(PyObject* o) {
-    const at::Tensor& t = tensor(o, "scratch");
+void* scratch(Device& d, PyObject* o) {
+    const at::Tensor& t = tensor(d, o, "scratch");
     if (!t.is_contiguous() || t.nbytes() < XP_SERVING_SCRATCH_BYTES)
         bad("'scratch' must be contiguous and of " + std::to_string(XP_SERVING_SCRATCH_BYTES) + " bytes (new_scratch)");
     return t.data_ptr();
 }
 
-float* lse_of(PyObject* o, const xp_rows& q) {
+float* lse_of(Device& d, PyObject* o, const xp_rows& q) {
     if (o == Py_None) return nullptr;
-    return static_cast<float*>(flat(o, "lse", at::kFloat, (int64_t)q.tokens * q.heads));
+    return static_cast<float*>(flat(d, o, "lse", at::kFloat, (int64_t)q.tokens * q.heads));
 }
 
 uint32_t count(PyObject* o, const char* name) {
@@ -125,11 +141,12 @@ PyObject* failed(int status, const std::string& message) {
     return Py_BuildValue("(is)", status, message.c_str());
 }
 
-// Runs f, which returns an xp_status, and turns what goes wrong into a result.
+// Runs f(device), which returns an xp_status, and turns what goes wrong into a result.
 template <class F> PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F f) {
     if (got != want) return failed(XP_ERR_ARITY, "expects " + std::to_string(want) + " arguments");
     try {
-        const xp_status s = f();
+        Device d;
+        const xp_status s = f(d);
         if (PyErr_Occurred()) return nullptr;
         if (s != XP_OK) return failed(s, xp_last_error());
         Py_RETURN_NONE;
@@ -142,53 +159,56 @@ template <class F> PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F f) {
 }
 
 PyObject* py_rope_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 7, [&] {
-        const xp_rows out = rows(a[0], "out"), in = rows(a[1], "x");
-        const xp_rotary r = rotary(a[2], a[3], a[4], a[5], a[6], in.tokens);
-        return xp_rope_rows(stream_of(a[1]), &out, &in, &r);
+    return guarded(n, 7, [&](Device& d) {
+        const xp_rows out = rows(d, a[0], "out"), in = rows(d, a[1], "x");
+        const xp_rotary r = rotary(d, a[2], a[3], a[4], a[5], a[6], in.tokens);
+        return xp_rope_rows(d.stream(), &out, &in, &r);
     });
 }
 PyObject* py_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 11, [&] {
-        const xp_pages p = pages(a);
-        const xp_rows k = rows(a[4], "k"), v = rows(a[5], "v");
-        const auto* slots = static_cast<const int64_t*>(flat(a[6], "slots", at::kLong, k.tokens));
-        if (a[8] == Py_None) return xp_kv_write(stream_of(a[4]), &p, &k, &v, slots, nullptr);
-        const xp_rotary r = rotary(a[7], a[8], a[9], a[10], Py_False, k.tokens);
-        return xp_kv_write(stream_of(a[4]), &p, &k, &v, slots, &r);
+    return guarded(n, 11, [&](Device& d) {
+        const xp_pages p = pages(d, a);
+        const xp_rows k = rows(d, a[4], "k"), v = rows(d, a[5], "v");
+        const auto* slots = static_cast<const int64_t*>(flat(d, a[6], "slots", at::kLong, k.tokens));
+        if (a[8] == Py_None) return xp_kv_write(d.stream(), &p, &k, &v, slots, nullptr);
+        const xp_rotary r = rotary(d, a[7], a[8], a[9], a[10], Py_False, k.tokens);
+        return xp_kv_write(d.stream(), &p, &k, &v, slots, &r);
     });
 }
 PyObject* py_kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 7, [&] {
-        const xp_pages p = pages(a);
-        const xp_rows k = rows(a[4], "k"), v = rows(a[5], "v");
-        return xp_kv_read(stream_of(a[4]), &p, &k, &v, static_cast<const int64_t*>(flat(a[6], "slots", at::kLong, k.tokens)));
+    return guarded(n, 7, [&](Device& d) {
+        const xp_pages p = pages(d, a);
+        const xp_rows k = rows(d, a[4], "k"), v = rows(d, a[5], "v");
+        return xp_kv_read(d.stream(), &p, &k, &v, static_cast<const int64_t*>(flat(d, a[6], "slots", at::kLong, k.tokens)));
     });
 }
 PyObject* py_attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 9, [&] {
-        const xp_rows out = rows(a[0], "out"), q = rows(a[1], "q"), k = rows(a[2], "k"), v = rows(a[3], "v");
-        const auto* starts = static_cast<const int32_t*>(flat(a[4], "starts", at::kInt, -1));
+    return guarded(n, 9, [&](Device& d) {
+        const xp_rows out = rows(d, a[0], "out"), q = rows(d, a[1], "q"), k = rows(d, a[2], "k"), v = rows(d, a[3], "v");
+        const auto* starts = static_cast<const int32_t*>(flat(d, a[4], "starts", at::kInt, -1));
         const int64_t batch = THPVariable_Unpack(a[4]).numel() - 1;
         if (batch < 0 || batch > 0x7FFFFFFF) bad("'starts' must have one value more than there are sequences");
-        return xp_attention_packed(stream_of(a[1]), &out, &q, &k, &v, starts, (uint32_t)batch, count(a[6], "window"),
-                                   (float)PyFloat_AsDouble(a[7]), lse_of(a[8], q), scratch(a[5]));
+        float* const lse = lse_of(d, a[8], q);
+        void* const work = scratch(d, a[5]);
+        return xp_attention_packed(d.stream(), &out, &q, &k, &v, starts, (uint32_t)batch, count(a[6], "window"),
+                                   (float)PyFloat_AsDouble(a[7]), lse, work);
     });
 }
 PyObject* py_attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 14, [&] {
-        const xp_rows out = rows(a[0], "out"), q = rows(a[1], "q");
-        const xp_pages p = pages(a + 2);
-        const auto* lens = static_cast<const int32_t*>(flat(a[7], "kv_lens", at::kInt, -1));
+    return guarded(n, 14, [&](Device& d) {
+        const xp_rows out = rows(d, a[0], "out"), q = rows(d, a[1], "q");
+        const xp_pages p = pages(d, a + 2);
+        const auto* lens = static_cast<const int32_t*>(flat(d, a[7], "kv_lens", at::kInt, -1));
         const int64_t batch = THPVariable_Unpack(a[7]).numel();
-        const at::Tensor& t = tensor(a[6], "table");
+        const at::Tensor& t = tensor(d, a[6], "table");
         if (t.dim() != 2 || t.size(0) != batch || batch > 0x7FFFFFFF || t.size(1) > 0x7FFFFFFF)
             bad("'table' must be [sequences, pages of a sequence]");
-        const auto* table = static_cast<const int32_t*>(flat(a[6], "table", at::kInt, -1));
-        const auto* starts = static_cast<const int32_t*>(flat(a[8], "starts", at::kInt, batch + 1));
-        return xp_attention_paged(stream_of(a[1]), &out, &q, &p, table, (uint32_t)t.size(1), lens, starts, (uint32_t)batch,
-                                  count(a[9], "q_most"), count(a[11], "window"), (float)PyFloat_AsDouble(a[12]),
-                                  lse_of(a[13], q), scratch(a[10]));
+        const auto* table = static_cast<const int32_t*>(flat(d, a[6], "table", at::kInt, -1));
+        const auto* starts = static_cast<const int32_t*>(flat(d, a[8], "starts", at::kInt, batch + 1));
+        float* const lse = lse_of(d, a[13], q);
+        void* const work = scratch(d, a[10]);
+        return xp_attention_paged(d.stream(), &out, &q, &p, table, (uint32_t)t.size(1), lens, starts, (uint32_t)batch,
+                                  count(a[9], "q_most"), count(a[11], "window"), (float)PyFloat_AsDouble(a[12]), lse, work);
     });
 }
 
