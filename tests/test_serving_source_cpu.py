@@ -1,0 +1,39 @@
+"""Rules of the serving kernels that no run can show safely, read from their
+source: what happens to the others when one wait runs out, and what orders the
+two ways in which memory is reached."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xpose_b200", "csrc")
+
+
+def source(name):
+    text = open(os.path.join(CSRC, name)).read()
+    return re.sub(r"/\*.*?\*/|//[^\n]*", "", text, flags=re.S)
+
+
+def body(text, name):
+    """The braces' content of the function that is defined as `name`."""
+    at = text.index("{", re.search(r"\b" + name + r"\((?=[^;]*?\{)", text).start())
+    depth = 0
+    for i in range(at, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if not depth:
+            return text[at:i + 1]
+    raise AssertionError(name)
+
+
+def test_tile_kernel_warps_that_part_meet_again_only_at_the_end():
+    """After a wait ran out the warps leave their loops at different places: a
+    barrier that counts threads among them would wait for ever."""
+    kernel = body(source("serving_tile.cuh"), "attn_tile_kernel")
+    parted = kernel[kernel.index("if (warp < NQ * 4)"):]
+    assert not re.search(r"\bbar(rier)?\.(cta\.)?(sync|red|arrive)", parted)
+    assert len(re.findall(r"__syncthreads\w*\(", parted)) == 1
+    assert parted.index("__syncthreads(") > max(m.start() for m in re.finditer(r"\bat_wait\w*\(", parted))
+
+
+def test_tile_kernel_row_numbers_are_none_until_given():
+    """... and what a loader then reads as a row's number is a row of the cache or none."""
+    kernel = body(source("serving_tile.cuh"), "attn_tile_kernel")
+    assert re.search(r"G::row_off \+ i \* 4\) = AT_NONE;", kernel[:kernel.index("if (warp < NQ * 4)")])

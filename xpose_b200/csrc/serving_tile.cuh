@@ -175,7 +175,9 @@ XP_DEV bool at_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 // Bounded: a wait that runs out reports it and lets every later wait of the
-// CTA pass, so the kernel ends (with unspecified output).
+// CTA pass, so the kernel ends (with unspecified output). Once a CTA's warps
+// have parted, each leaves on its own, so they meet in no barrier of threads
+// before the last one.
 XP_DEV void at_wait(uint32_t bar, uint32_t parity, volatile uint32_t* dead, uint32_t* err) {
     uint32_t it = 0;
     while (!at_try(bar, parity)) {
@@ -525,7 +527,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     // which the swizzled layouts need, without a byte lost
     extern __shared__ __align__(1024) unsigned char sm[];
     const uint32_t smb = smem_u32(sm);
-    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 15 + 2 * NSEG;
+    constexpr int NSEG = 4, NBAR = 4 * NSLOT + 16 + 2 * NSEG;
     struct Small {
         AtPlan plan;
         AtSeg segs[NSEG];
@@ -552,6 +554,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     const uint32_t b_qh = b_qfree + 16;             // [NQ] ... made fp16
     const uint32_t b_ph = b_qh + 16;                // [2] P's first 64 keys made (b_p: all), by S buffer
     const uint32_t b_end = b_ph + 16;               // products in flight after a failed wait
+    const uint32_t b_rows = b_end + 8;              // 8-bit pages: row numbers and scales of a tile given to the loaders
 
     if (smb & 1023) {  // cannot be multiplied from
         if (tid == 0) atomicOr(a.err, SERVE_ERR_WAIT);
@@ -577,6 +580,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             mbar_init(m + 8 + NSEG + i, NQ * 4 + G::NLD * 4 + 2);
         }
         for (int i = 0; i < 7; ++i) mbar_init(m + 8 + 2 * NSEG + i, i >= 2 && i < 6 ? 4 : 1);
+        mbar_init(m + 15 + 2 * NSEG, 4 * G::NLD);
         fence_mbar_init();
         s_dead = 0;
         for (int i = 0; i < 4; ++i) s_bad[i] = 0;
@@ -584,6 +588,11 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     if (warp == LAST) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&small.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if constexpr (G::Q8) {
+        // after a failed wait a loader may meet row numbers that were never given: no row
+        for (uint32_t i = tid; i < NSTAGE * 128; i += G::THREADS)
+            *reinterpret_cast<uint32_t*>(sm + G::row_off + i * 4) = AT_NONE;
     }
     pdl_wait();  // everything above may run under the kernel before this one
     at_clear<T, D>(a, G::THREADS);
@@ -949,6 +958,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             constexpr uint32_t SUB = G::PIECE / 16384 / G::NLD;
             static_assert(G::NLD == 1 || SUB == 1, "loaders");
             uint32_t given = 0, stage = 0;   // parts given to the tensor core
+            uint32_t rows_phase = 0;
             // the codes of the two parts issued last (0 older), and what they are: 0 none, 1 K, 2 V
             uint4 raw[2][4];
             uint32_t kind[2] = {0, 0};
@@ -1056,7 +1066,11 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         // weight of 0 must not meet it
                         sc[256 + lt] = !has ? 1.0f : vs == vs ? 1.0f / vs : 0.0f;
                     }
-                    asm volatile("bar.sync 1, %0;" ::"n"(128 * G::NLD) : "memory");
+                    // not a barrier of threads: after a failed wait some loaders have left
+                    __syncwarp();
+                    if (lane == 0) at_arrive(b_rows);
+                    at_wait(b_rows, rows_phase, &s_dead, err);
+                    rows_phase ^= 1;
                     fetch(t + 1);
                 };
                 for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) {
