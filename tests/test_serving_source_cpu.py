@@ -37,3 +37,15 @@ def test_tile_kernel_row_numbers_are_none_until_given():
     """... and what a loader then reads as a row's number is a row of the cache or none."""
     kernel = body(source("serving_tile.cuh"), "attn_tile_kernel")
     assert re.search(r"G::row_off \+ i \* 4\) = AT_NONE;", kernel[:kernel.index("if (warp < NQ * 4)")])
+
+
+def test_few_row_kernel_orders_its_parts_before_the_copies_that_read_them():
+    """Parts are written to global memory by ordinary stores and read by bulk
+    copies: a fence between the two proxies after the stores, and after the
+    ticket that says they are all there, of all memory and not of shared alone."""
+    kernel = body(source("serving_few.cuh"), "attn_few_kernel")
+    ticket, copy = kernel.index("atomicAdd(w.tickets"), kernel.index("bulk_g2s(")
+    last_part = max(m.start() for m in re.finditer(r"__stcg\(", kernel))
+    assert last_part < ticket < copy
+    assert "fence_proxy_async_all();" in kernel[last_part:ticket]
+    assert "fence_proxy_async_all();" in kernel[kernel.index("if (s_last)", ticket + 100):copy]

@@ -731,6 +731,7 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
         if (!whole) {
             const uint32_t c0 = g.c0, nparts = g.parts;
             constexpr uint32_t PER = (ROWS * (D / 4) + 127) / 128;  // float4 of a thread
+            fence_proxy_async_all();  // the last CTA reads the parts by bulk copies
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -760,7 +761,9 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 for (uint32_t i0 = 0; i0 < nparts; i0 += fit) {
                     const uint32_t m = min(nparts - i0, fit);
                     __syncthreads();
-                    fence_proxy_async();  // what the threads wrote in the buffer, before the copies write there
+                    // what other CTAs wrote as parts before the copies read it, and what
+                    // the threads wrote in the buffer before the copies write there
+                    fence_proxy_async_all();
                     if (tid == 0)
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&s_part)),
                                      "r"(m * bytes) : "memory");

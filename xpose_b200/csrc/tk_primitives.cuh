@@ -26,6 +26,9 @@ XP_DEV void mbar_init(uint64_t* bar, uint32_t count) {
 }
 XP_DEV void fence_mbar_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 XP_DEV void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// of global memory too: other CTAs' ordinary writes (ordered before this thread
+// by an acquire) before this thread's bulk copies read them
+XP_DEV void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
 XP_DEV void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)

@@ -210,9 +210,6 @@ XP_DEV float tk_block_sum(float v, float* red) {
 XP_DEV void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// generic-proxy global writes of other CTAs (ordered before this thread by an
-// acquire) before this thread's async-proxy (bulk copy) reads
-XP_DEV void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
 // Fixed point in units of 2^-32: |v| < 2^31 is exact to 2^-33. An
 // out-of-range (or NaN) value sets TK_ERR_RANGE and contributes 0.
