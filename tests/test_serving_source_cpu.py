@@ -49,3 +49,11 @@ def test_few_row_kernel_orders_its_parts_before_the_copies_that_read_them():
     assert last_part < ticket < copy
     assert "fence_proxy_async_all();" in kernel[last_part:ticket]
     assert "fence_proxy_async_all();" in kernel[kernel.index("if (s_last)", ticket + 100):copy]
+
+
+def test_tile_kernel_orders_its_plan_before_the_copies_that_take_its_place():
+    """The plan is made by ordinary stores in the memory where Q then arrives by
+    TMA: every thread's stores, a fence, a barrier, and only then the copies."""
+    kernel = body(source("serving_tile.cuh"), "attn_tile_kernel")
+    assert re.search(r"at_make_plan<.*?;\s*fence_proxy_async\(\);\s*(at_fence_before\(\);)?\s*__syncthreads\(\);", kernel)
+    assert kernel.index("__syncthreads();", kernel.index("at_make_plan<")) < kernel.index("at_tma(")

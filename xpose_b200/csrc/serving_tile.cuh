@@ -597,6 +597,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     pdl_wait();  // everything above may run under the kernel before this one
     at_clear<T, D>(a, G::THREADS);
     at_make_plan<G::THREADS>(a, w, reinterpret_cast<uint32_t*>(sm), s_sums, &s_plan);
+    fence_proxy_async();  // the plan's words before the copies of Q that take their place
     at_fence_before();
     __syncthreads();
     at_fence_after();
