@@ -57,3 +57,14 @@ def test_tile_kernel_orders_its_plan_before_the_copies_that_take_its_place():
     kernel = body(source("serving_tile.cuh"), "attn_tile_kernel")
     assert re.search(r"at_make_plan<.*?;\s*fence_proxy_async\(\);\s*(at_fence_before\(\);)?\s*__syncthreads\(\);", kernel)
     assert kernel.index("__syncthreads();", kernel.index("at_make_plan<")) < kernel.index("at_tma(")
+
+
+def test_loads_stay_behind_the_wait_for_the_kernel_before():
+    """A grid that starts under the kernel before it reads nothing of that
+    kernel's until it has waited: its loads in assembly are volatile, as the wait
+    is, and no intrinsic stands in for them whose order the compiler may choose."""
+    for name in ("serving.cuh", "serving_attn.cuh", "serving_few.cuh", "serving_tile.cuh"):
+        text = source(name)
+        for m in re.finditer(r"\basm\s*(volatile)?\s*\(\s*\"([^\"]*)", text):
+            assert m[1] or not re.match(r"\s*(ld|cp|atom|red)\b", m[2]), m[0]
+        assert not re.search(r"\b__ld(g|cg|ca|cs|lu|cv)\b", text), name

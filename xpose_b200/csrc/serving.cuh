@@ -53,9 +53,11 @@ struct Raw32 { uint32_t w[8]; };
 XP_DEV Raw32 load_raw32(const void* a, const void* b, bool side) {
     Raw32 r;
     if (side) {
-        asm("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-            : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
-            : "l"(a));
+        asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"  // in order with pdl_wait()
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                       "=r"(r.w[7])
+                     : "l"(a)
+                     : "memory");
     } else {
         const uint4 x = *static_cast<const uint4*>(a), y = *static_cast<const uint4*>(b);
         r = Raw32{{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}};
@@ -103,6 +105,27 @@ template <class T> XP_DEV T ld_now(const T* p) {
     T x;
     asm volatile("ld.global.b64 %0, [%1];" : "=l"(x) : "l"(p));
     return x;
+}
+
+// ... and data that is read once, past the L1 cache
+XP_DEV uint4 ld_once(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+XP_DEV float4 ld_once(const float4* p) {
+    const uint4 v = ld_once(reinterpret_cast<const uint4*>(p));
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+XP_DEV float2 ld_once(const float2* p) {
+    float2 v;
+    asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+    return v;
+}
+XP_DEV uint32_t ld_once(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
 }
 
 struct RowsArg {

@@ -1011,7 +1011,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t r = at_lds(rows0 + st * 512 + (key0 + r0 + i * step) * 4);
                         now[i] = make_uint4(0, 0, 0, 0);
-                        if (r != AT_NONE) now[i] = __ldcg(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
+                        if (r != AT_NONE) now[i] = ld_once(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
                     }
                     if (kind[0]) convert();
 #pragma unroll
@@ -1326,11 +1326,11 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
-    const uint4 head = __ldcg(reinterpret_cast<const uint4*>(w.heads) + 2 * c0 + 1);
+    const uint4 head = ld_once(reinterpret_cast<const uint4*>(w.heads) + 2 * c0 + 1);
     if (head.x != AT_FIRST) return;
     uint32_t parts = 1;
     for (uint32_t j = c0 + 1; j < ctas; j += 32) {
-        const uint32_t kind = j + lane < ctas ? __ldcg(w.heads + (size_t)(2 * (j + lane)) * 4) : (uint32_t)AT_LAST;
+        const uint32_t kind = j + lane < ctas ? ld_once(w.heads + (size_t)(2 * (j + lane)) * 4) : (uint32_t)AT_LAST;
         const uint32_t last = __ballot_sync(0xffffffffu, kind == AT_LAST);
         parts += last ? __ffs(last) : 32;
         if (last) break;
@@ -1348,9 +1348,9 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
             v[i] = make_float2(0.0f, 0.0f);
             if (i0 + i < parts) {
                 const float4* p = reinterpret_cast<const float4*>(part(i0 + i)) + (size_t)col * ROWS + row;
-                v[i] = __ldcg(reinterpret_cast<const float2*>(part(i0 + i) + (size_t)ROWS * D * 4) + row);
-                x[i][0] = __ldcg(p);
-                x[i][1] = __ldcg(p + ROWS);
+                v[i] = ld_once(reinterpret_cast<const float2*>(part(i0 + i) + (size_t)ROWS * D * 4) + row);
+                x[i][0] = ld_once(p);
+                x[i][1] = ld_once(p + ROWS);
             }
         }
         float top = m;
