@@ -482,8 +482,10 @@ typedef struct xp_rows {
 } xp_rows;
 /* A paged cache: k and v are [num_pages][kv_heads][page_size][head_dim]
  * contiguous; 8-bit pages have one fp32 scale a row, [num_pages][kv_heads]
- * [page_size], and the value of a code is code * scale. page_size is a power
- * of two from 8 to 256; head_dim 64, 128 or 256. A row's slot number is
+ * [page_size], not negative, and the value of a code is code * scale (the
+ * attentions take v rows with a scale below 2^-106, zero among them, for rows
+ * of zeros). page_size is a power of two from 8 to 256; head_dim 64, 128 or
+ * 256. A row's slot number is
  * page * page_size + row. */
 typedef struct xp_pages {
     void *k, *v;

@@ -4,9 +4,17 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
+import serving_ref as R  # noqa: E402
+from test_gpu_serving import check_attention, gen, ints, make_cache, randn  # noqa: E402
 from xpose_b200 import serving as S  # noqa: E402
 
-F16, I8 = torch.float16, torch.int8
+F16, BF16 = torch.float16, torch.bfloat16
+I8, FP8 = torch.int8, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def scratch():
+    return S.new_scratch()
 
 
 def test_tensors_of_a_device_that_is_not_the_current_one():
@@ -32,3 +40,90 @@ def test_tensors_of_a_device_that_is_not_the_current_one():
         outs.append((a.cpu(), b.cpu()))
     for x, y in zip(*outs):
         assert torch.equal(x, y)
+
+def paged(scratch, cache, q, kv, scale=0.0, window=0, page=16):
+    """attention_paged of q's tokens, the newest of kv keys in `cache`, against the 64-bit form."""
+    kp, vp, ks, vs = cache
+    n, dim = q.shape[0], q.shape[2]
+    table = torch.arange(-(-kv // page), dtype=torch.int32, device="cuda")[None].contiguous()
+    out, lse = torch.full_like(q, float("nan")), torch.empty(n, q.shape[1], device="cuda")
+    S.attention_paged(out, q, kp, vp, ks, vs, table, ints([kv]), ints([0, n]), n, scratch, scale=scale, window=window,
+                      lse=lse)
+    assert S.error_word(scratch) == 0
+    slots = torch.arange(kv, device="cuda")
+    k, v = R.rows_of(kp, ks, slots), R.rows_of(vp, vs, slots)
+    return out, lse, R.attend(q, k, v, kv - n, window, scale or dim ** -0.5), v
+
+
+@pytest.mark.parametrize("cache", [I8, FP8])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,window", [(1, 0), (4, 0), (8, 50), (30, 0), (70, 100)])
+def test_paged_value_scales_of_zero_and_next_to_it(scratch, cache, dtype, dim, n, window):
+    """A value is code * scale whatever the code: rows whose scale is zero or has
+    no finite inverse are rows of (next to) nothing, which weigh as any other."""
+    g = gen(dim + n)
+    kv = 300
+    pages = make_cache(g, 20, 16, 1, dim, cache)
+    vs, ks = pages[3].view(-1), pages[2].view(-1)
+    vs[7:40] = 0.0                     # some of a tile, some of a step
+    vs[48:64], vs[64:70] = 2.0 ** -130, 2.0 ** -149
+    vs[70:74], vs[74:78] = 2.0 ** -126, 2.0 ** -107
+    vs[128:256] = 0.0                  # a whole tile
+    vs[kv - 1] = vs[kv - n // 2] = 0.0  # only some rows see it
+    ks[100:105] = 0.0
+    q = randn(g, n, 2, dim, dtype=dtype)
+    out, lse, (want, mag, wlse), v = paged(scratch, pages, q, kv, window=window)
+    check_attention(out, lse, want, mag, wlse, dtype, kv, float(v.abs().max()))
+    vs[:] = 0.0
+    out, lse, (_, _, wlse), _ = paged(scratch, pages, q, kv, window=window)
+    assert not out.any() and ((lse.double() - wlse).abs() <= 2.0 ** -12 + 2.0 ** -22 * wlse.abs()).all()
+
+
+@pytest.mark.parametrize("cache", [I8, FP8])
+@pytest.mark.parametrize("n", [1, 30])
+def test_paged_rows_of_zeros_keep_their_weight_beside_large_values(scratch, cache, n):
+    """Two thousand keys without values, each e^-12 of one key with values near 3e4, take 1.2 % of its weight."""
+    kv, dim = 2048, 64
+    pages = S.new_pages(kv // 16, 16, 1, dim, cache)
+    k, v = torch.zeros(kv, 1, dim, device="cuda"), torch.zeros(kv, 1, dim, device="cuda")
+    k[5, 0, 0] = 12.0
+    v[5] = 3e4
+    S.kv_write(*pages, k, v, torch.arange(kv, device="cuda"))
+    q = torch.zeros(n, 1, dim, dtype=BF16, device="cuda")
+    q[:, 0, 0] = 1.0
+    out, lse, (want, mag, wlse), v = paged(scratch, pages, q, kv, scale=1.0)
+    assert float(want[-1].max()) < 0.99 * 3e4
+    check_attention(out, lse, want, mag, wlse, BF16, 0, 0.0)
+
+
+@pytest.mark.parametrize("cache", [I8, FP8])
+@pytest.mark.parametrize("n", [1, 30])
+def test_paged_codes_of_nan_under_a_scale_of_zero_are_zeros(scratch, cache, n):
+    """A row that was never written holds any codes."""
+    g = gen(39)
+    kv, dim = 300, 128
+    pages = make_cache(g, 20, 16, 1, dim, cache)
+    pages[3].view(-1)[40:60] = 0.0
+    clean = paged(scratch, pages, q := randn(g, n, 2, dim, dtype=BF16), kv)[0]
+    pages[1].view(torch.uint8).view(-1, dim)[40:60] = 0x7F
+    assert torch.isfinite(clean).all()
+    table = torch.arange(19, dtype=torch.int32, device="cuda")[None].contiguous()
+    out = torch.empty_like(q)
+    S.attention_paged(out, q, *pages, table, ints([kv]), ints([0, n]), n, scratch)
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("cache", [I8, FP8])
+@pytest.mark.parametrize("scale", [2.0 ** -106, 2.0 ** 120, 2.0 ** 126, 2.0 ** 127])
+@pytest.mark.parametrize("n", [1, 30])
+def test_paged_value_scales_of_any_size(scratch, cache, scale, n):
+    """... and those whose inverse is subnormal, or whose values are near the ends of fp32."""
+    g = gen(40)
+    kv, dim = 300, 64
+    pages = make_cache(g, 20, 16, 1, dim, cache)
+    v = torch.randint(-1, 2, pages[1].shape, generator=g, device="cuda").float()
+    pages[1].view(torch.uint8).copy_(v.to(cache).view(torch.uint8))
+    pages[3].fill_(scale)
+    out, lse, (want, mag, wlse), v = paged(scratch, pages, randn(g, n, 2, dim, dtype=BF16), kv)
+    check_attention(out, lse, want, mag, wlse, BF16, kv, scale)

@@ -262,6 +262,10 @@ XP_DEV uint64_t page_row(const PagesArg& p, uint64_t slot, uint32_t head) {
 }
 
 constexpr float CACHE_FLOOR = 0x1p-100f;  // smallest row maximum told from zero
+// Values with a scale below this count as zeros in attention: those of a row
+// whose maximum is at most CACHE_FLOOR, and of scales that have no normal inverse.
+constexpr float CACHE_NOTHING = 0x1p-106f;
+static_assert(CACHE_FLOOR / 127.0f < CACHE_NOTHING, "int8 has the larger scales");
 
 // A lane's 8 values of a row, four at d[0] and four at d[1], into its place;
 // LANES lanes hold the row.

@@ -484,16 +484,21 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
             }
             // ---- weights: keys 16 b + lg (values 0, 1) and 8 more (2, 3), rows 2 lq (0, 2) and 2 lq + 1 ----
             float rv[KG][2];
+            uint32_t nones = 0;  // 8-bit pages: a bit a key without values
 #pragma unroll
             for (int b = 0; b < KG; ++b) rv[b][0] = rv[b][1] = 1.0f;
             if constexpr (Q8) {
-                // a lane a key: its scale, log2 of v's and its inverse; where there
-                // is no key or no page (codes and scales of zero) the value is zero. A scale
-                // of NaN makes the weights of those who see the key NaN; the others' weight
-                // of 0 must not meet it
+                // a lane a key: its scale, log2 of v's and its inverse. Where there is no
+                // key or no page (scales of zero), and where v's scale is next to zero, the
+                // value is zero: the weight counts with a scale of 1 and multiplies zeros.
+                // A scale of NaN makes the weights of those who see the key NaN; the others'
+                // weight of 0 must not meet it
                 const uint32_t sc = scales + stage * (2 * KPS * 4) + (lane & (KPS - 1)) * 4;
                 const float ks0 = __uint_as_float(at_lds(sc)), vs0 = __uint_as_float(at_lds(sc + KPS * 4));
-                const float lv0 = vs0 == 0.0f ? 0.0f : fw_lg2(vs0), rv0 = vs0 == 0.0f ? 1.0f : vs0 == vs0 ? fw_rcp(vs0) : 0.0f;
+                const bool none = fabsf(vs0) < CACHE_NOTHING;
+                nones = __ballot_sync(0xffffffffu, none);
+                const float lv0 = none ? 0.0f : fw_lg2(vs0);
+                const float rv0 = none ? 1.0f : vs0 == vs0 ? fw_rcp(vs0 * 0x1p-10f) * 0x1p-10f : 0.0f;  // may be subnormal
 #pragma unroll
                 for (int b = 0; b < KG; ++b)
 #pragma unroll
@@ -566,20 +571,20 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 const uint32_t r = lane & 15, c0 = lane >> 4;
 #pragma unroll
                 for (int b = 0; b < KG; ++b) {
-                    // rows that are no keys may hold anything, codes of NaN among it
+                    // rows without values, and those that are no keys, may hold anything, codes of NaN among it
                     uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-                    if (partial) {
+                    if (nones) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const int32_t key = kb + 16 * b + 8 * h + 2 * (int32_t)lq;
-                            keep[h] = (key >= lo && key < hi ? 0xFFFFu : 0u) | (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u);
+                            const uint32_t two = nones >> (16 * b + 8 * h + 2 * lq);
+                            keep[h] = (two & 1 ? 0u : 0xFFFFu) | (two & 2 ? 0u : 0xFFFF0000u);
                         }
                     }
 #pragma unroll
                     for (int d = 0; d < KS; d += 2) {
                         uint32_t x[4];
                         fw_ldmt(sv + fw_at<RB, KPS>(16 * b + r, d + c0), x);
-                        if (partial) {
+                        if (nones) {
                             x[0] &= keep[0];
                             x[1] &= keep[1];
                             x[2] &= keep[0];

@@ -28,7 +28,9 @@
 // are turned into exact 16-bit values by the loader threads; their scales
 // never touch them: with t_ij = s_ij ks_j + log2 vs_j the weight that
 // multiplies v's code is 2^(t - m), and l adds 2^(t - m) / vs_j. A weight is
-// then rounded relative to the largest contribution, whatever the scales.
+// then rounded relative to the largest contribution, whatever the scales. Rows
+// whose scale is zero or next to it have no such weight: their codes are read as
+// zeros with a scale of 1.
 //
 // Work is split evenly: every CTA takes the same number of (row tile, key
 // tile) units, so the last tile of a call does not run alone. A row tile that
@@ -80,8 +82,8 @@ template <class T, class C, int W> struct AtCfg {
     // shared memory
     static constexpr int q_off = 0;
     static constexpr int ring_off = NQ * W * 16384;
-    static constexpr int row_off = ring_off + NSLOT * PIECE;       // [NSTAGE][128] row numbers, 8-bit pages
-    static constexpr int sc_off = row_off + (Q8 ? NSTAGE * 512 : 0);  // [NSTAGE][3][128] floats, 8-bit pages
+    static constexpr int row_off = ring_off + NSLOT * PIECE;       // [NSTAGE][2][128] row numbers of k and v, 8-bit pages
+    static constexpr int sc_off = row_off + (Q8 ? NSTAGE * 1024 : 0);  // [NSTAGE][3][128] floats, 8-bit pages
     static constexpr int bar_off = sc_off + (Q8 ? NSTAGE * 1536 : 0);
     static constexpr int smem = bar_off + 1024;                       // barriers, plan, row tiles, flags
 };
@@ -591,7 +593,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     }
     if constexpr (G::Q8) {
         // after a failed wait a loader may meet row numbers that were never given: no row
-        for (uint32_t i = tid; i < NSTAGE * 128; i += G::THREADS)
+        for (uint32_t i = tid; i < NSTAGE * 256; i += G::THREADS)
             *reinterpret_cast<uint32_t*>(sm + G::row_off + i * 4) = AT_NONE;
     }
     pdl_wait();  // everything above may run under the kernel before this one
@@ -1009,7 +1011,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     uint4 now[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t r = at_lds(rows0 + st * 512 + (key0 + r0 + i * step) * 4);
+                        const uint32_t r = at_lds(rows0 + (st * 2 + (is_v ? 1 : 0)) * 512 + (key0 + r0 + i * step) * 4);
                         now[i] = make_uint4(0, 0, 0, 0);
                         if (r != AT_NONE) now[i] = ld_once(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
                     }
@@ -1058,14 +1060,17 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 // the row numbers and scales of key tile t into stage kst
                 auto resolve = [&](uint32_t t) {
                     if (lw == 0) {
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 512 + lt * 4), "r"(r) : "memory");
+                        // a missing page: scores and values of zero; a scale next to zero: values of zero
+                        const bool has = r != AT_NONE, some = has && !(fabsf(vs) < CACHE_NOTHING);
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 1024 + lt * 4), "r"(r) : "memory");
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(rows0 + kst * 1024 + 512 + lt * 4), "r"(some ? r : AT_NONE)
+                                     : "memory");
                         float* sc = reinterpret_cast<float*>(sm + G::sc_off) + kst * 384;
-                        const bool has = r != AT_NONE;  // a missing page: scores and values of zero
                         sc[lt] = has ? ks * a.scale_log2 : 0.0f;
-                        sc[128 + lt] = has ? log2f(vs) : 0.0f;
+                        sc[128 + lt] = some ? log2f(vs) : 0.0f;
                         // a scale of NaN makes the weights of those who see the key NaN; the others'
                         // weight of 0 must not meet it
-                        sc[256 + lt] = !has ? 1.0f : vs == vs ? 1.0f / vs : 0.0f;
+                        sc[256 + lt] = !some ? 1.0f : vs == vs ? 1.0f / vs : 0.0f;
                     }
                     // not a barrier of threads: after a failed wait some loaders have left
                     __syncwarp();
