@@ -127,3 +127,27 @@ def test_paged_value_scales_of_any_size(scratch, cache, scale, n):
     pages[3].fill_(scale)
     out, lse, (want, mag, wlse), v = paged(scratch, pages, randn(g, n, 2, dim, dtype=BF16), kv)
     check_attention(out, lse, want, mag, wlse, BF16, kv, scale)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,window", [(4, 0), (4, 100), (8, 0), (60, 0), (60, 100), (200, 0), (1, 100)])
+def test_paged_codes_that_are_nan_reach_those_who_see_them(scratch, dtype, dim, n, window):
+    """e4m3 has codes of NaN. With an ordinary scale beside them they are NaN in
+    their own place, for the new tokens that see the key and for nobody else."""
+    g = gen(41 + dim)
+    kv, page = 700, 16
+    pages = make_cache(g, 44, page, 1, dim, FP8)
+    kb, vb = (t.view(torch.uint8).view(44, page, dim) for t in pages[:2])
+    at = lambda j: (j // page, j % page)  # noqa: E731
+    vb[at(698)][3], vb[at(699)][dim - 1] = 0x7F, 0xFF
+    vb[at(kv - n + 1)][17] = 0x7F
+    kb[at(697)][1] = 0xFF
+    vb[at(kv - n - window + 2 if window else 5)][0] = 0x7F
+    q = randn(g, n, 2, dim, dtype=dtype)
+    out, _, (want, mag, _), v = paged(scratch, pages, q, kv, window=window)
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), fine)
+    assert fine.any() or n == 1 or not window  # a token before the NaN keys is left as it is
+    top = float(torch.nan_to_num(v).abs().max())
+    assert ((out.double() - want).abs() <= R.attention_bound(want, mag, dtype, kv, top))[fine].all()

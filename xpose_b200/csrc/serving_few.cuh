@@ -567,6 +567,51 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                 }
             // ---- O^T += V^T P^T ----
             const uint32_t sv = st + G::HALF;
+            if constexpr (std::is_same_v<C, fp8c>) {
+                // where some row does not see what another sees: codes of NaN only to the rows
+                // that see them, out of the step's V and into their sums
+                if ((kb < flo && lo < flo) || (kb + KPS > fhi && fhi < hi)) {
+                    uint32_t odd = 0;
+#pragma unroll 1
+                    for (uint32_t c = lane * 16; c < (uint32_t)G::HALF; c += 512) {
+                        const uint4 v = at_lds16(sv + c);
+                        odd |= at_odd8(v.x) | at_odd8(v.y) | at_odd8(v.z) | at_odd8(v.w);
+                    }
+                    if (__any_sync(0xffffffffu, odd != 0)) {
+#pragma unroll
+                        for (int d = 0; d < KS; ++d)
+                            for (uint32_t j = 0; j < (uint32_t)KPS; ++j) {
+                                if (nones >> j & 1) continue;
+                                const int32_t key = kb + (int32_t)j;
+                                // the lane's two dims
+                                uint16_t two;
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(two) : "r"(sv + fw_at<RB, KPS>(j, d) + lg * 2) : "memory");
+#pragma unroll
+                                for (int half = 0; half < 2; ++half) {
+                                    if ((two >> (8 * half) & 0x7F) != 0x7F) continue;
+#pragma unroll
+                                    for (int i = 0; i < NR; ++i)
+#pragma unroll
+                                        for (int q = 0; q < 2; ++q)
+                                            if (key >= klo[i][q] && key < khi[i][q])
+                                                o[d][i][2 * half + q] = __uint_as_float(0x7FC00000u);
+                                }
+                            }
+                        __syncwarp();
+#pragma unroll 1
+                        for (uint32_t c = lane * 16; c < (uint32_t)G::HALF; c += 512) {
+                            uint4 v = at_lds16(sv + c);
+                            v.x &= ~((at_odd8(v.x) >> 7) * 0xFFu);
+                            v.y &= ~((at_odd8(v.y) >> 7) * 0xFFu);
+                            v.z &= ~((at_odd8(v.z) >> 7) * 0xFFu);
+                            v.w &= ~((at_odd8(v.w) >> 7) * 0xFFu);
+                            at_sts16(sv + c, v);
+                        }
+                        fence_proxy_async();  // before the next copy over them
+                        __syncwarp();
+                    }
+                }
+            }
             if constexpr (Q8) {
                 const uint32_t r = lane & 15, c0 = lane >> 4;
 #pragma unroll

@@ -24,7 +24,7 @@
 // last page or the next sequence holds past the tile's keys must not be
 // multiplied even by 0 (it may be NaN): in the few V tiles where some row does
 // not see some key, loader threads put zeros there, and take infinities and
-// NaN of v out; those go to the rows that do see them at the end. 8-bit codes
+// NaN of v out (codes of NaN, too); those go to the rows that do see them at the end. 8-bit codes
 // are turned into exact 16-bit values by the loader threads; their scales
 // never touch them: with t_ij = s_ij ks_j + log2 vs_j the weight that
 // multiplies v's code is 2^(t - m), and l adds 2^(t - m) / vs_j. A weight is
@@ -506,6 +506,8 @@ XP_DEV bool at_look(const ServeAttnArgs& a, int32_t lo, int32_t hi, int32_t p0, 
     const int64_t k0 = (int64_t)key, k1 = k0 + n;
     return k0 < lo || k1 > hi || k1 > (int64_t)p0 + 1 || (a.window && k0 < (int64_t)hi - (int64_t)a.window);
 }
+// The top bits of bytes that are codes of NaN (all lower bits set)
+XP_DEV uint32_t at_odd8(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 // Bits 15 and 31: an infinity or NaN in either half (all exponent bits set, so
 // one more carries out of them)
 template <class T> XP_DEV uint32_t at_odd16(uint32_t w) {
@@ -525,6 +527,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     constexpr uint32_t LAST = NQ * 4 + G::NLD * 4;  // first warp of the last warpgroup
     using M = std::conditional_t<G::Q8, __half, T>;
     constexpr bool RESCALE = G::Q8 && std::is_same_v<T, bf16>;
+    constexpr bool ODD8 = std::is_same_v<C, fp8c>;  // 8-bit pages, and some codes are NaN
     // no static shared memory: the dynamic part then starts on a 1 KB boundary,
     // which the swizzled layouts need, without a byte lost
     extern __shared__ __align__(1024) unsigned char sm[];
@@ -800,7 +803,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 at_wait(b_o + 8 * wg, (npv - 1) & 1, &s_dead, err);
                 at_fence_after();
             }
-            const bool bad = !G::Q8 && *reinterpret_cast<volatile uint32_t*>(&s_bad[seg & 3]) == seg + 1;
+            const bool bad = (!G::Q8 || ODD8) && *reinterpret_cast<volatile uint32_t*>(&s_bad[seg & 3]) == seg + 1;
             const bool whole = g.kind == AT_FULL;
             const float inv = l != 0.0f ? 1.0f / l : 0.0f;   // l is 0 where the row saw nothing
             const uint32_t slot = 2 * blockIdx.x + (g.kind == AT_FIRST ? 1 : 0);
@@ -823,19 +826,26 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         const int32_t j0 = max((int32_t)key0, klo);
                         const int32_t j1 = min(min((int32_t)(key0 + G::VKEYS), khi), g.hi);
                         for (int32_t j = j0; j < j1; ++j) {
-                            const T* vp;
+                            const C* vp;
                             if (a.pages.k) {
                                 const int32_t page = ld_now(a.table + (uint64_t)g.b * a.table_width + (j >> a.pages.page_shift));
                                 const uint64_t sl = ((uint64_t)(uint32_t)page << a.pages.page_shift) + (j & ((1u << a.pages.page_shift) - 1));
                                 if (page < 0 || sl >= a.pages.slots) continue;
-                                vp = static_cast<const T*>(a.pages.v) + page_row(a.pages, sl, g.h) * D + c;
+                                const uint64_t r = page_row(a.pages, sl, g.h);
+                                if (ODD8 && fabsf(a.pages.vs[r]) < CACHE_NOTHING) continue;  // a row of zeros
+                                vp = static_cast<const C*>(a.pages.v) + r * D + c;
                             } else {
-                                vp = static_cast<const T*>(a.v.data) + (int64_t)(g.s.q0 + j) * a.v.ts + (int64_t)g.h * a.v.hs + c;
+                                vp = reinterpret_cast<const C*>(static_cast<const T*>(a.v.data) + (int64_t)(g.s.q0 + j) * a.v.ts +
+                                                                (int64_t)g.h * a.v.hs + c);
                             }
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
-                                const float v = to_f32(vp[i]);
-                                if (!(fabsf(v) <= 3.4028235e38f)) o[i] += v;
+                                if constexpr (G::Q8) {
+                                    if (ODD8 && (reinterpret_cast<const uint8_t*>(vp)[i] & 0x7F) == 0x7F) o[i] = __uint_as_float(0x7FC00000u);
+                                } else {
+                                    const float v = to_f32(vp[i]);
+                                    if (!(fabsf(v) <= 3.4028235e38f)) o[i] += v;
+                                }
                             }
                         }
                     }
@@ -962,7 +972,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             static_assert(G::NLD == 1 || SUB == 1, "loaders");
             uint32_t given = 0, stage = 0;   // parts given to the tensor core
             uint32_t rows_phase = 0;
-            // the codes of the two parts issued last (0 older), and what they are: 0 none, 1 K, 2 V
+            // the codes of the two parts issued last (0 older), and what they are: 0 none, 1 K, 2 V,
+            // 3 V of a piece that needs a look
             uint4 raw[2][4];
             uint32_t kind[2] = {0, 0};
             const uint32_t rows0 = smb + G::row_off;
@@ -975,6 +986,22 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const uint32_t sub = G::NLD == 2 ? lw : turn;
                 const uint32_t base = smb + G::ring_off + slot * G::PIECE;
                 if (turn == 0 && index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
+                if (ODD8 && kind[0] == 3) {
+                    // codes of NaN out of the product: they go to the rows that see them at the end
+                    uint32_t odd = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) odd |= at_odd8(raw[0][i].x) | at_odd8(raw[0][i].y) | at_odd8(raw[0][i].z) | at_odd8(raw[0][i].w);
+                    if (odd) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            raw[0][i].x &= ~((at_odd8(raw[0][i].x) >> 7) * 0xFFu);
+                            raw[0][i].y &= ~((at_odd8(raw[0][i].y) >> 7) * 0xFFu);
+                            raw[0][i].z &= ~((at_odd8(raw[0][i].z) >> 7) * 0xFFu);
+                            raw[0][i].w &= ~((at_odd8(raw[0][i].w) >> 7) * 0xFFu);
+                        }
+                        s_bad[seg & 3] = seg + 1;
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint2 x0 = at_codes<M>(raw[0][i].x, C{}), x1 = at_codes<M>(raw[0][i].y, C{});
@@ -1003,7 +1030,9 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const int32_t lo = g.lo, hi = g.hi;
                 const uint32_t n = g.n, k0 = g.k0, head = g.h;
                 const int32_t* const table = a.table + (uint64_t)g.b * a.table_width;
-                auto piece = [&](bool is_v, uint32_t c, uint32_t st) {
+                const int32_t p0 = g.p0;
+                // part c of key tile t of K or V, its rows and scales in stage st
+                auto piece = [&](bool is_v, uint32_t c, uint32_t t, uint32_t st) {
                     const uint32_t u = is_v ? lt % VU : lt % KU, r0 = is_v ? lt / VU : lt / KU;
                     const uint32_t step = is_v ? 128 / VU : 128 / KU, key0 = is_v ? c * (AT_KEYS / W) : 0;
                     const uint32_t d = (is_v ? u : c * KU + u) * 16;
@@ -1022,7 +1051,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         raw[1][i] = now[i];
                     }
                     kind[0] = kind[1];
-                    kind[1] = is_v ? 2 : 1;
+                    kind[1] = !is_v ? 1 : ODD8 && at_look(a, lo, hi, p0, (k0 + t) * AT_KEYS + c * G::NP / W * G::VKEYS, G::VKEYS) ? 3 : 2;
                 };
                 auto page_of = [&](uint32_t kt) -> int32_t {
                     const int32_t key = (int32_t)(kt * AT_KEYS + lt);
@@ -1081,15 +1110,15 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 };
                 for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) {
                     resolve(t);
-                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, kst);
+                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, t, kst);
                     kst = kst + 1 == NSTAGE ? 0 : kst + 1;
                 }
                 for (uint32_t t = 0; t < n; ++t) {
-                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(true, c, stage);
+                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(true, c, t, stage);
                     stage = stage + 1 == NSTAGE ? 0 : stage + 1;
                     if (t + G::LAG < n) {
                         resolve(t + G::LAG);
-                        for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, kst);
+                        for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, t + G::LAG, kst);
                         kst = kst + 1 == NSTAGE ? 0 : kst + 1;
                     }
                 }
