@@ -556,8 +556,11 @@ xp_status xp_attention_packed(void* stream, const xp_rows* out, const xp_rows* q
  * tokens' own included, already written) are in pages table[b * table_width
  * ..], and new token i of n sits at position kv_lens[b] - n + i. A token whose
  * position is negative sees nothing and gets zeros (lse -inf). q_most: the
- * most new tokens of any sequence. 16-bit pages have q's type. The rest is as
- * for xp_attention_packed. */
+ * most new tokens of any sequence. 16-bit pages have q's type. Over 8-bit pages
+ * a row of q is multiplied with the codes in fp16, bf16 rows after a power of
+ * two that fits them to it: values below 2^-24 of the row's largest are lost,
+ * and q . codes has to be within fp32's range. The rest is as for
+ * xp_attention_packed. */
 xp_status xp_attention_paged(void* stream, const xp_rows* out, const xp_rows* q, const xp_pages* pages,
                              const int32_t* table, uint32_t table_width, const int32_t* kv_lens,
                              const int32_t* starts, uint32_t batch, uint32_t q_most, uint32_t window, float scale,

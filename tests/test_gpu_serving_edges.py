@@ -151,3 +151,24 @@ def test_paged_codes_that_are_nan_reach_those_who_see_them(scratch, dtype, dim, 
     assert fine.any() or n == 1 or not window  # a token before the NaN keys is left as it is
     top = float(torch.nan_to_num(v).abs().max())
     assert ((out.double() - want).abs() <= R.attention_bound(want, mag, dtype, kv, top))[fine].all()
+
+
+@pytest.mark.parametrize("cache", [I8, FP8])
+@pytest.mark.parametrize("exponent", [122, 123, 126, 127])
+@pytest.mark.parametrize("n", [1, 40])
+def test_paged_largest_finite_queries(scratch, cache, exponent, n):
+    """bf16 queries up to the type's largest, over keys of -1, 0 and 1 in the
+    places where they are: the dot products stay within fp32."""
+    g = gen(43)
+    kv, dim = 300, 64
+    pages = make_cache(g, 20, 16, 1, dim, cache)
+    k = torch.randint(-1, 2, (20, 1, 16, dim), generator=g, device="cuda").float()
+    k[..., 1:] = 0
+    pages[0].view(torch.uint8).copy_(k.to(cache).view(torch.uint8))
+    pages[2].fill_(1.0)
+    q = torch.zeros(n, 2, dim, device="cuda")
+    q[..., 0] = (torch.rand(n, 2, generator=g, device="cuda") * 0.9 + 1.0) * 2.0 ** 60
+    q = (q * 2.0 ** (exponent - 60)).to(BF16)
+    assert torch.isfinite(q).all()
+    out, lse, (want, mag, wlse), v = paged(scratch, pages, q, kv, scale=2.0 ** -(exponent - 1))
+    check_attention(out, lse, want, mag, wlse, BF16, kv, float(v.abs().max()))

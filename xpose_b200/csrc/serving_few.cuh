@@ -385,9 +385,7 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                         for (int j = 0; j < 2; ++j) top = max(top, max(qf[s][i][j] & 0x7F80u, (qf[s][i][j] >> 16) & 0x7F80u));
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    // 2^(127 - e) brings it to [1, 2); rows of zeros and tiny values, or of infinities, as they are
-                    const uint32_t e = top >> 7;
-                    const float f = e > 20 && e < 250 ? __uint_as_float((254u - e) << 23) : 1.0f;
+                    const float f = at_row_factor(top >> 7);
 #pragma unroll
                     for (int s = 0; s < KS; ++s)
 #pragma unroll

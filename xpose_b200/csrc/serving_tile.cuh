@@ -226,6 +226,9 @@ XP_DEV float2 at_mul2(float2 a, float2 b) {
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
 }
+// What brings a bf16 row whose largest exponent is e to [1, 2) (the largest
+// rows to [2, 4); rows of zeros and subnormals stay)
+XP_DEV float at_row_factor(uint32_t e) { return e ? __uint_as_float((uint32_t)max(254 - (int32_t)e, 1) << 23) : 1.0f; }
 template <class T> XP_DEV uint32_t at_pack(float lo, float hi) {
     uint32_t r;
     if constexpr (std::is_same_v<T, bf16>) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -665,8 +668,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         top = max(top, max(o, h >> 16));
                     }
                     const uint32_t e = top >> 7;
-                    float f = 1.0f;
-                    if (e > 20 && e < 250 && (e < 123 || e > 141)) f = __uint_as_float((254u - e) << 23);
+                    const float f = e < 123 || e > 141 ? at_row_factor(e) : 1.0f;
                     rs = 1.0f / f;
                     rescaled = __any_sync(0xffffffffu, f != 1.0f);
 #pragma unroll 4
