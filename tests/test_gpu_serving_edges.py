@@ -172,3 +172,36 @@ def test_paged_largest_finite_queries(scratch, cache, exponent, n):
     assert torch.isfinite(q).all()
     out, lse, (want, mag, wlse), v = paged(scratch, pages, q, kv, scale=2.0 ** -(exponent - 1))
     check_attention(out, lse, want, mag, wlse, BF16, kv, float(v.abs().max()))
+
+
+@pytest.mark.parametrize("pages", [True, False])
+def test_256_wide_tiles_one_after_the_other_never_lose_a_wait(pages):
+    """Thousands of calls in a row, whose row tiles end at all moments: no wait
+    runs out, whichever warp comes late to the last products of its tile."""
+    g = gen(51)
+    new, kv = [512, 37, 60, 101, 331], [8192, 600, 1000, 2300, 5000]
+    scratch, starts, n = S.new_scratch(), [0], sum(new)
+    for m in new:
+        starts.append(starts[-1] + m)
+    q = randn(g, n, 4, 256, dtype=BF16)
+    out = torch.empty_like(q)
+    if pages:
+        held = [-(-m // 16) for m in kv]
+        cache = make_cache(g, sum(held), 16, 1, 256, I8)
+        table = torch.full((len(kv), max(held)), -1, dtype=torch.int32)
+        order = torch.randperm(sum(held), generator=g, device="cuda", dtype=torch.int32).cpu()
+        for b, m in enumerate(held):
+            table[b, :m] = order[sum(held[:b]):sum(held[:b]) + m]
+        table, lens = table.cuda(), ints(kv)
+        call = lambda: S.attention_paged(out, q, *cache, table, lens, ints_starts, 512, scratch)  # noqa: E731
+    else:
+        k, v = randn(g, n, 1, 256, dtype=BF16), randn(g, n, 1, 256, dtype=BF16)
+        call = lambda: S.attention_packed(out, q, k, v, ints_starts, scratch, window=300)  # noqa: E731
+    ints_starts = ints(starts)
+    call()
+    first = out.clone()
+    for _ in range(10):
+        for _ in range(1000):
+            call()
+        assert S.error_word(scratch) == 0
+        assert torch.equal(out, first)

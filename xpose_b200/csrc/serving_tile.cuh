@@ -556,7 +556,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     const uint32_t b_clean = b_raw + NSLOT * 8;     // [NSLOT] ... looked over
     const uint32_t b_q = b_clean + NSLOT * 8;       // [NQ] Q is in
     const uint32_t b_s = b_q + 16, b_p = b_s + 16;  // [2] S made, P made (by S buffer)
-    const uint32_t b_o = b_p + 16;                  // [NQ] P V added
+    const uint32_t b_o = b_p + 16;                  // [2] P V added, by S buffer
     const uint32_t b_seg = b_o + 16, b_free = b_seg + NSEG * 8;  // [NSEG] a row tile given, done with
     const uint32_t b_qfree = b_free + NSEG * 8;     // [NQ] Q multiplied for the last time
     const uint32_t b_qh = b_qfree + 16;             // [NQ] ... made fp16
@@ -635,7 +635,15 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             w.heads[(2 * blockIdx.x + 1) * 4] = AT_FULL;
         }
         const uint32_t qrow0 = wg * w.sub_tokens;  // first token of this row tile in its CTA's tile
-        uint32_t stage = 0, s_phase = 0, npv = 0, q_phase = 0;  // s_phase: a bit for each S buffer
+        // Phases are told apart by their parity alone, so a wait must be neither a
+        // phase early nor two late: each warp waits for every phase of a barrier,
+        // in turn, and arrives for the next only after that. s_phase, o_phase: a bit
+        // for each S buffer
+        uint32_t stage = 0, s_phase = 0, o_phase = 0, q_phase = 0;
+        auto take_o = [&](uint32_t buf) {
+            at_wait(b_o + 8 * buf, o_phase >> buf & 1, &s_dead, err);
+            o_phase ^= 1u << buf;
+        };
         for (;; done()) {
             const AtSeg& g = take();
             if (g.kind == AT_END || s_dead) break;
@@ -693,6 +701,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const uint32_t s_tm = tmem + lanes + buf * 128;
                 at_wait(b_s + 8 * buf, s_phase >> buf & 1, &s_dead, err);
                 s_phase ^= 1u << buf;
+                if (t >= (uint32_t)G::NB) take_o(buf);  // added before S was made over its P
                 at_fence_after();
                 float s[128];
                 {
@@ -742,8 +751,10 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     if (up) m = ref = mx;
                     if (t != 0) {
                         // O so far by the same factor, once the product before this one is in it
-                        at_wait(b_o + 8 * wg, (npv - 1) & 1, &s_dead, err);
-                        at_fence_after();
+                        if (NQ == 1) {
+                            at_wait(b_o + 8 * (buf ^ 1), o_phase >> (buf ^ 1) & 1, &s_dead, err);
+                            at_fence_after();
+                        }
 #pragma unroll 1
                         for (int c = 0; c < D; c += 16) {  // few at a time: S fills the registers
                             float o[16];
@@ -795,14 +806,12 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     __syncwarp();
                     if (lane == 0) at_arrive((half ? b_p : b_ph) + 8 * buf);  // a half is multiplied while the other is made
                 }
-                ++npv;
                 stage = stage + 1 == NSTAGE ? 0 : stage + 1;
             }
             // ---- the row tile's result ----
             const float l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
             if (g.n) {
-                if (NQ == 1 && g.n > 1) at_wait(b_o + 8 * wg, (npv - 2) & 1, &s_dead, err);
-                at_wait(b_o + 8 * wg, (npv - 1) & 1, &s_dead, err);
+                for (uint32_t t = max(g.n, (uint32_t)G::NB) - G::NB; t < g.n; ++t) take_o(NQ == 2 ? wg : (t & 1));
                 at_fence_after();
             }
             const bool bad = (!G::Q8 || ODD8) && *reinterpret_cast<volatile uint32_t*>(&s_bad[seg & 3]) == seg + 1;
@@ -1302,7 +1311,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                             }
                             if (lead) {
                                 if (last) at_commit(b_empty + 8 * slot);
-                                if (c == G::NP - 1) at_commit(b_o + 8 * qi);
+                                if (c == G::NP - 1) at_commit(b_o + 8 * buf);
                             }
                             __syncwarp();
                             slot = slot + 1 == NSLOT ? 0 : slot + 1;
