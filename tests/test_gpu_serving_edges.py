@@ -205,3 +205,23 @@ def test_256_wide_tiles_one_after_the_other_never_lose_a_wait(pages):
             call()
         assert S.error_word(scratch) == 0
         assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("cache", [I8, FP8])
+@pytest.mark.parametrize("exponent", [-40, -4, -3, -1, 0, 3, 14, 15])
+@pytest.mark.parametrize("n", [1, 50])
+def test_paged_queries_of_mixed_sizes(scratch, cache, exponent, n):
+    """bf16 queries whose scores come from values 2^-16 of the row's largest,
+    which meets keys of zero there: they enter whole, wherever the largest is."""
+    g = gen(47)
+    kv, dim = 300, 64
+    pages = make_cache(g, 20, 16, 1, dim, cache)
+    pages[0][..., 0].view(torch.uint8).zero_()
+    k = R.rows_of(pages[0], pages[2], torch.arange(kv, device="cuda"))
+    q = (torch.rand(n, 2, dim, generator=g, device="cuda") + 1.0) * 2.0 ** -16
+    q *= torch.randint(0, 2, q.shape, generator=g, device="cuda") * 2 - 1
+    q[..., 0] = 1.0
+    q = (q * 2.0 ** exponent).to(BF16)
+    scale = 4.0 / float((q.double()[:, 0] @ k[:, 0].T).std())  # scores of a few
+    out, lse, (want, mag, wlse), v = paged(scratch, pages, q, kv, scale=float(torch.tensor(scale, dtype=torch.float32)))
+    check_attention(out, lse, want, mag, wlse, BF16, kv, float(v.abs().max()))

@@ -662,8 +662,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             bool rescaled = false;
             if constexpr (RESCALE) {
                 if (n) {
-                    // this row as fp16; by a power of two into its range where it is not (the
-                    // row's largest outside 2^-4 .. 2^15), exact down to 2^-24 of the largest
+                    // this row as fp16; by a power of two into its range where its largest is
+                    // below 1 or above 2^15: exact down to 2^-24 of the largest
                     at_wait(b_q + 8 * wg, q_phase, &s_dead, err);
                     q_phase ^= 1;
                     const uint32_t base = smb + G::q_off + wg * W * 16384 + row * 128;
@@ -676,7 +676,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         top = max(top, max(o, h >> 16));
                     }
                     const uint32_t e = top >> 7;
-                    const float f = e < 123 || e > 141 ? at_row_factor(e) : 1.0f;
+                    const float f = e < 127 || e > 141 ? at_row_factor(e) : 1.0f;
                     rs = 1.0f / f;
                     rescaled = __any_sync(0xffffffffu, f != 1.0f);
 #pragma unroll 4
