@@ -57,3 +57,21 @@ def test_one_tensor_on_another_device_is_refused(call, odd):
 @pytest.mark.parametrize("call,odd", [(c, n) for c in CALLS for n, a in arguments(c).items() if isinstance(a, tuple)])
 def test_a_tensor_on_the_host_is_refused(call, odd):
     refused(call, make(call, lambda name: "cpu" if name == odd else "cuda:0"), f"'{odd}'", "CUDA")
+
+
+@pytest.mark.parametrize("call,name", [("rope_rows", "magnitude"), ("kv_write", "magnitude"),
+                                       ("attention_packed", "scale"), ("attention_paged", "scale")])
+@pytest.mark.parametrize("value", ["one", None, [1.0]])
+def test_what_is_no_number_is_refused_before_anything_is_enqueued(call, name, value):
+    refused(call, make(call) | {name: value}, f"'{name}'", "number")
+
+
+@pytest.mark.parametrize("call,name", [("attention_packed", "window"), ("attention_paged", "window"),
+                                       ("attention_paged", "q_most")])
+@pytest.mark.parametrize("value", ["one", None, 1.5, -1, 1 << 31])
+def test_what_is_no_count_is_refused(call, name, value):
+    refused(call, make(call) | {name: value}, f"'{name}'", "whole number")
+
+
+def test_a_direction_without_truth_value_is_refused():
+    refused("rope_rows", make("rope_rows") | {"inverse": torch.ones(2)}, "'inverse'")

@@ -73,6 +73,12 @@ void* flat(Device& d, PyObject* o, const char* name, at::ScalarType type, int64_
     return t.data_ptr();
 }
 
+float number(PyObject* o, const char* name) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) bad(std::string("'") + name + "' must be a number");
+    return (float)v;
+}
+
 xp_pages pages(Device& d, PyObject* const* a) {  // k, v, k_scale, v_scale
     const at::Tensor &k = tensor(d, a[0], "k_pages"), &v = tensor(d, a[1], "v_pages");
     xp_pages p{};
@@ -111,8 +117,10 @@ xp_rotary rotary(Device& d, PyObject* positions, PyObject* turns, PyObject* layo
     if (n > 0x3FFFFFFF) bad("'turns' is too long");
     r.rot_dim = (uint32_t)(2 * n);
     r.layout = (uint32_t)PyLong_AsLong(layout);
-    r.magnitude = (float)PyFloat_AsDouble(magnitude);
-    r.inverse = PyObject_IsTrue(inverse) ? 1u : 0u;
+    r.magnitude = number(magnitude, "magnitude");
+    const int back = PyObject_IsTrue(inverse);
+    if (back < 0) bad("'inverse' must be true or false");
+    r.inverse = (uint32_t)back;
     return r;
 }
 
@@ -190,8 +198,9 @@ PyObject* py_attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (batch < 0 || batch > 0x7FFFFFFF) bad("'starts' must have one value more than there are sequences");
         float* const lse = lse_of(d, a[8], q);
         void* const work = scratch(d, a[5]);
-        return xp_attention_packed(d.stream(), &out, &q, &k, &v, starts, (uint32_t)batch, count(a[6], "window"),
-                                   (float)PyFloat_AsDouble(a[7]), lse, work);
+        const uint32_t window = count(a[6], "window");
+        const float scale = number(a[7], "scale");
+        return xp_attention_packed(d.stream(), &out, &q, &k, &v, starts, (uint32_t)batch, window, scale, lse, work);
     });
 }
 PyObject* py_attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -207,8 +216,10 @@ PyObject* py_attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const auto* starts = static_cast<const int32_t*>(flat(d, a[8], "starts", at::kInt, batch + 1));
         float* const lse = lse_of(d, a[13], q);
         void* const work = scratch(d, a[10]);
-        return xp_attention_paged(d.stream(), &out, &q, &p, table, (uint32_t)t.size(1), lens, starts, (uint32_t)batch,
-                                  count(a[9], "q_most"), count(a[11], "window"), (float)PyFloat_AsDouble(a[12]), lse, work);
+        const uint32_t most = count(a[9], "q_most"), window = count(a[11], "window");
+        const float scale = number(a[12], "scale");
+        return xp_attention_paged(d.stream(), &out, &q, &p, table, (uint32_t)t.size(1), lens, starts, (uint32_t)batch, most,
+                                  window, scale, lse, work);
     });
 }
 
