@@ -473,7 +473,8 @@ void xp_bdec_destroy(xp_bdec* b);
 typedef enum xp_dtype { XP_F32 = 0, XP_F16 = 1, XP_BF16 = 2, XP_INT8 = 3, XP_FP8_E4M3 = 4 } xp_dtype;
 /* Rows of heads: value d of head h of token t is element
  * t * token_stride + h * head_stride + d of `data` (strides in elements, so a
- * slice of a fused q|k|v product needs no copy). F32, F16 or BF16. */
+ * slice of a fused q|k|v product needs no copy). F32, F16 or BF16. Rows that a
+ * call writes must not overlap. */
 typedef struct xp_rows {
     void* data;
     int64_t token_stride, head_stride;

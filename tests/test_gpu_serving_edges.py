@@ -1,5 +1,7 @@
 """The serving operators at their edges: scales, codes, queries and devices that
 ordinary use seldom meets, against the plain 64-bit forms."""
+import random
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -225,3 +227,28 @@ def test_paged_queries_of_mixed_sizes(scratch, cache, exponent, n):
     scale = 4.0 / float((q.double()[:, 0] @ k[:, 0].T).std())  # scores of a few
     out, lse, (want, mag, wlse), v = paged(scratch, pages, q, kv, scale=float(torch.tensor(scale, dtype=torch.float32)))
     check_attention(out, lse, want, mag, wlse, BF16, kv, float(v.abs().max()))
+
+
+def test_rows_may_lie_in_any_order_that_keeps_them_apart():
+    """Random strides: what overlaps is refused, all else is written, each row in its place."""
+    r, g = random.Random(5), gen(53)
+    turns, _ = S.rope_turns(16, 1e4)
+    seen = [0, 0]
+    for _ in range(300):
+        tokens, heads = r.randint(1, 6), r.randint(1, 6)
+        ts, hs = r.randint(0, 12) * 8, r.randint(0, 12) * 8
+        at = [t * ts + h * hs for t in range(tokens) for h in range(heads)]
+        apart = all(abs(a - b) >= 16 for i, a in enumerate(at) for b in at[:i])
+        seen[apart] += 1
+        space = torch.zeros(max(at) + 16, device="cuda")
+        out = space.as_strided((tokens, heads, 16), (ts, hs, 1))
+        x = randn(g, tokens, heads, 16)
+        pos = torch.arange(tokens, dtype=torch.int32, device="cuda") * 77
+        if apart:
+            want = S.rope_rows(torch.empty_like(x), x, pos, turns)
+            assert torch.equal(S.rope_rows(out, x, pos, turns), want)
+            assert space.count_nonzero() == want.count_nonzero()
+        else:
+            with pytest.raises(S.XpError, match="overlap"):
+                S.rope_rows(out, x, pos, turns)
+    assert min(seen) > 30

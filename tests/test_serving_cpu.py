@@ -135,3 +135,21 @@ def test_attention_paged_refuses(kw, word):
 
 def test_attention_paged_refuses_no_pages():
     refused(lib().xp_attention_paged(None, ref(rows()), ref(rows()), None, P, 1, P, P, 1, 1, 0, 0.0, None, P), "'pages'")
+
+
+# rows that overlap: one for all, a stride below the head's size, or both axes together
+OVERLAP = [dict(ts=0), dict(hs=0), dict(ts=64), dict(hs=64), dict(hs=-64), dict(ts=128, hs=256, heads=2),
+           dict(ts=384, hs=512, heads=4, tokens=5), dict(ts=3 * 128, hs=-2 * 128 - 64, heads=4, tokens=9)]
+
+
+@pytest.mark.parametrize("layout", OVERLAP)
+def test_rows_that_are_written_must_not_overlap(layout):
+    x = {"heads": 4, "tokens": 4} | layout
+    good, bad = rows(heads=x["heads"], tokens=x["tokens"]), rows(**x)
+    refused(lib().xp_rope_rows(None, ref(bad), ref(good), ref(rotary())), "rope_rows", "'out' overlap")
+    p = pages(kv=x["heads"])
+    refused(lib().xp_kv_read(None, ref(p), ref(bad), ref(good), P), "kv_read", "'k' overlap")
+    refused(lib().xp_kv_read(None, ref(p), ref(good), ref(bad), P), "kv_read", "'v' overlap")
+    one = rows(heads=1, tokens=x["tokens"])
+    refused(packed(out=bad, q=good, k=one, v=one), "attention_packed", "'out' overlap")
+    refused(paged(out=bad, q=good), "attention_paged", "'out' overlap")

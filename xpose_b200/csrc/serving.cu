@@ -36,6 +36,30 @@ xp_status check_rows(const char* who, const char* name, const xp_rows* r, uint32
             "%s: the rows of '%s' must be aligned to %zu bytes", who, name, align * bytes_of(r->dtype));
     return XP_OK;
 }
+// Two of r's rows have an element in common: |dt ts + dh hs| < dim for some pair
+// of distances that are not both zero.
+bool rows_overlap(const xp_rows* r) {
+    using wide = unsigned __int128;
+    // a: the axis of fewer rows
+    wide a = (wide)(r->head_stride < 0 ? -(__int128)r->head_stride : r->head_stride), na = r->heads;
+    wide b = (wide)(r->token_stride < 0 ? -(__int128)r->token_stride : r->token_stride), nb = r->tokens;
+    if (na > nb) {
+        std::swap(a, b);
+        std::swap(na, nb);
+    }
+    const wide dim = r->dim;
+    if ((na > 1 && a < dim) || (nb > 1 && b < dim)) return true;
+    if (na <= 1 || nb <= 1 || b >= (na - 1) * a + dim || a >= (nb - 1) * b + dim) return false;  // the usual layouts
+    for (wide i = 1; i < na; ++i) {
+        const wide j = i * a / b;  // the distances along the other axis that come nearest
+        if ((j > 0 && j < nb && i * a - j * b < dim) || (j + 1 < nb && (j + 1) * b - i * a < dim)) return true;
+    }
+    return false;
+}
+xp_status check_written(const char* who, const char* name, const xp_rows* r) {
+    REQUIRE(!rows_overlap(r), "%s: rows of '%s' overlap, and each is written", who, name);
+    return XP_OK;
+}
 bool same_shape(const xp_rows* a, const xp_rows* b) {
     return a->tokens == b->tokens && a->heads == b->heads && a->dim == b->dim && a->dtype == b->dtype;
 }
@@ -277,6 +301,7 @@ xp_status xp_rope_rows(void* stream, const xp_rows* out, const xp_rows* in, cons
     REQUIRE(rope, "%s: argument 'rope' is null", who);
     REQUIRE(same_shape(out, in), "%s: 'out' and 'in' differ in shape or type", who);
     TRY(check_rope(who, rope, in->dim, 2));
+    TRY(check_written(who, "out", out));
     if (in->tokens == 0) return XP_OK;
     TRY(check_rope_data(who, rope));
     // vectors of 16 bytes where every row allows them, else one pair a thread
@@ -343,6 +368,8 @@ xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, cons
     const uint32_t vec = (uint32_t)(16 / bytes_of(k->dtype));
     TRY(check_rows(who, "k", k, vec));
     TRY(check_rows(who, "v", v, vec));
+    TRY(check_written(who, "k", k));
+    TRY(check_written(who, "v", v));
     REQUIRE(same_shape(k, v) && k->heads == pages->kv_heads && k->dim == pages->head_dim,
             "%s: 'k', 'v' and the pages differ in shape or type", who);
     if (k->tokens == 0) return XP_OK;
@@ -375,6 +402,7 @@ xp_status attention(const char* who, void* stream, const xp_rows* out, const xp_
                 q->head_stride >= 0,
             "%s: 'q' needs positive strides", who);
     REQUIRE(same_shape(q, out), "%s: 'q' and 'out' differ in shape or type", who);
+    TRY(check_written(who, "out", out));
     REQUIRE(q->dim == 64 || q->dim == 128 || q->dim == 256, "%s: dim must be 64, 128 or 256 (got %u)", who, q->dim);
     uint32_t kv_heads, cache;
     if (pages) {
