@@ -153,3 +153,9 @@ def test_rows_that_are_written_must_not_overlap(layout):
     one = rows(heads=1, tokens=x["tokens"])
     refused(packed(out=bad, q=good, k=one, v=one), "attention_packed", "'out' overlap")
     refused(paged(out=bad, q=good), "attention_paged", "'out' overlap")
+
+
+@pytest.mark.parametrize("layout", [dict(ts=1024), dict(hs=256, ts=1024), dict(ts=128, hs=512)])
+def test_rope_rows_in_place_keeps_its_strides(layout):
+    """Rows of one place in two orders: a thread would read what another has written."""
+    refused(lib().xp_rope_rows(None, ref(rows(**layout)), ref(rows()), ref(rotary())), "rope_rows", "strides")

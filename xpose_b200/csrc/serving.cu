@@ -302,6 +302,10 @@ xp_status xp_rope_rows(void* stream, const xp_rows* out, const xp_rows* in, cons
     REQUIRE(same_shape(out, in), "%s: 'out' and 'in' differ in shape or type", who);
     TRY(check_rope(who, rope, in->dim, 2));
     TRY(check_written(who, "out", out));
+    REQUIRE(out->data != in->data || in->tokens == 0 ||
+                ((in->tokens == 1 || out->token_stride == in->token_stride) &&
+                 (in->heads == 1 || out->head_stride == in->head_stride)),
+            "%s: 'out' and 'in' share their data but not their strides", who);
     if (in->tokens == 0) return XP_OK;
     TRY(check_rope_data(who, rope));
     // vectors of 16 bytes where every row allows them, else one pair a thread
