@@ -534,7 +534,7 @@ xp_status xp_kv_write(void* stream, const xp_pages* pages, const xp_rows* k, con
 xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, const xp_rows* v, const int64_t* slots);
 /* Scratch of the two attentions: 16-byte aligned, zeroed once, one call at a
  * time. Its uint32 at byte 4 is a sticky error word: 1 = a length past its
- * table row (clamped), 2 = a page outside the cache (its rows read as zeros),
+ * table row or 2^31 - 256 keys (clamped), 2 = a page outside the cache (its rows read as zeros),
  * 4 = a wait ran out (the output is unspecified; zero the scratch again), 8 = a
  * sequence had more than q_most new tokens (the rest were left out). */
 #define XP_SERVING_SCRATCH_BYTES (48u << 20)

@@ -252,3 +252,29 @@ def test_rows_may_lie_in_any_order_that_keeps_them_apart():
             with pytest.raises(S.XpError, match="overlap"):
                 S.rope_rows(out, x, pos, turns)
     assert min(seen) > 30
+
+
+@pytest.mark.parametrize("cache", [F16, I8])
+@pytest.mark.parametrize("n", [1, 40])
+def test_paged_lengths_up_to_the_last_whole_tile_below_2_31(scratch, cache, n):
+    """The last tile of 2^31 - 256 keys is read as any other; what lies beyond is
+    reported as past the table."""
+    g = gen(55)
+    page, dim = 8, 64
+    pages = make_cache(g, 3, page, 1, dim, cache)
+    table = torch.zeros(1, (1 << 28) - 1, dtype=torch.int32, device="cuda")
+    table[0, ((1 << 31) - 256) // page - 20:] = 1  # the last keys of the long sequence: page 1, the others page 0
+    q = randn(g, n, 2, dim, dtype=F16)
+
+    def run(t, kv):
+        out = torch.full_like(q, float("nan"))
+        S.attention_paged(out, q, *pages, t, ints([kv]), ints([0, n]), n, scratch, window=250)
+        return out, S.error_word(scratch)
+
+    short = torch.zeros(1, 64, dtype=torch.int32, device="cuda")
+    short[0, 44:] = 1
+    want, word = run(short, 512)
+    assert word == 0
+    for kv, reported in (((1 << 31) - 256, 0), ((1 << 31) - 255, 1), ((1 << 31) - 8, 1)):
+        out, word = run(table, kv)
+        assert word == reported and torch.equal(out, want)

@@ -12,6 +12,9 @@ constexpr uint32_t SERVE_ERR_PAGE = 2u;    // a page outside the cache
 constexpr uint32_t SERVE_ERR_WAIT = 4u;    // a wait ran out
 constexpr uint32_t SERVE_ERR_NEW = 8u;     // more new tokens than q_most
 
+// keys of a sequence: the end of its last tile or unit stays within 32 bits with a sign
+constexpr uint64_t SERVE_MAX_KEYS = 0x7FFFFF00u;
+
 struct ServeAttnArgs {
     RowsArg out, q, k, v;      // k, v: packed only
     PagesArg pages;            // paged only (pages.k != nullptr)
@@ -34,7 +37,7 @@ XP_DEV Seq seq_of(const ServeAttnArgs& a, uint32_t b) {
     s.q0 = (uint32_t)min(max(lo, 0), (int32_t)a.tokens);
     s.nq = (uint32_t)max(min(max(hi, 0), (int32_t)a.tokens) - (int32_t)s.q0, 0);
     if (a.pages.k) {
-        const uint64_t most = (uint64_t)a.table_width << a.pages.page_shift;
+        const uint64_t most = min((uint64_t)a.table_width << a.pages.page_shift, SERVE_MAX_KEYS);
         const int32_t n = max(ld_now(a.kv_lens + b), 0);
         s.nkv = (uint32_t)min((uint64_t)n, most);
         if ((uint64_t)n > most) atomicOr(a.err, SERVE_ERR_LENGTH);
