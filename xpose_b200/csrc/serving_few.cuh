@@ -82,7 +82,7 @@ XP_DEV uint2 fw_codes_t(uint32_t w, int8c) {
     const __half2 x = __hsub2(reinterpret_cast<__half2&>(a), bias), y = __hsub2(reinterpret_cast<__half2&>(b), bias);
     return make_uint2(reinterpret_cast<const uint32_t&>(x), reinterpret_cast<const uint32_t&>(y));
 }
-XP_DEV uint2 fw_codes_t(uint32_t w, fp8c) { return at_codes<__half>(__byte_perm(w, 0, 0x3120), fp8c{}); }
+XP_DEV uint2 fw_codes_t(uint32_t w, fp8c) { return at_codes(__byte_perm(w, 0, 0x3120), fp8c{}); }
 // where 16 bytes c of row r of a step's K or V lie: blocks of 128 bytes of every
 // row, in the 128-byte swizzle of the copy (rows of 64 bytes: the 64-byte one),
 // so eight rows' equal chunks are in eight bank groups
@@ -457,8 +457,8 @@ attn_few_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant__
                     for (int k = 0; k < KS; k += 2) {
                         uint32_t x[4];
                         fw_ldm(st + fw_at<RB, KPS>(r, k + c0), x);
-                        const uint2 y0 = at_codes<M>(x[0], C{}), y1 = at_codes<M>(x[1], C{});
-                        const uint2 y2 = at_codes<M>(x[2], C{}), y3 = at_codes<M>(x[3], C{});
+                        const uint2 y0 = at_codes(x[0], C{}), y1 = at_codes(x[1], C{});
+                        const uint2 y2 = at_codes(x[2], C{}), y3 = at_codes(x[3], C{});
                         const uint32_t a0[4] = {y0.x, y1.x, y0.y, y1.y}, a1[4] = {y2.x, y3.x, y2.y, y3.y};
 #pragma unroll
                         for (int i = 0; i < NR; ++i) {

@@ -235,38 +235,19 @@ template <class T> XP_DEV uint32_t at_pack(float lo, float hi) {
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// 4 codes -> 4 exact 16-bit values
-template <class T> XP_DEV uint2 at_codes(uint32_t w, int8c) {
-    uint2 r;
-    if constexpr (std::is_same_v<T, bf16>) {
-        // a biased code as the low bits of 2^23: exact fp32, then exact bf16 (8 bits)
-        const uint32_t u = w ^ 0x80808080u;
-        const float f0 = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)) - 8388736.0f;
-        const float f1 = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441)) - 8388736.0f;
-        const float f2 = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)) - 8388736.0f;
-        const float f3 = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - 8388736.0f;
-        r.x = at_pack<bf16>(f0, f1);
-        r.y = at_pack<bf16>(f2, f3);
-    } else {
-        // ... and of 2^10: 1024 + 128 + code, exact fp16
-        const uint32_t u = w ^ 0x80808080u;
-        const __half2 bias = __half2half2(__ushort_as_half(0x6480));
-        uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(reinterpret_cast<__half2&>(a), bias), y = __hsub2(reinterpret_cast<__half2&>(b), bias);
-        r.x = reinterpret_cast<const uint32_t&>(x);
-        r.y = reinterpret_cast<const uint32_t&>(y);
-    }
-    return r;
+// 4 codes -> 4 exact fp16 values
+XP_DEV uint2 at_codes(uint32_t w, int8c) {
+    // a biased code as the low bits of 2^10: 1024 + 128 + code, exact
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(reinterpret_cast<__half2&>(a), bias), y = __hsub2(reinterpret_cast<__half2&>(b), bias);
+    return make_uint2(reinterpret_cast<const uint32_t&>(x), reinterpret_cast<const uint32_t&>(y));
 }
-template <class T> XP_DEV uint2 at_codes(uint32_t w, fp8c) {
+XP_DEV uint2 at_codes(uint32_t w, fp8c) {
     uint32_t a, b;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"((uint16_t)w));
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"((uint16_t)(w >> 16)));
-    if constexpr (std::is_same_v<T, bf16>) {
-        const float2 x = __half22float2(reinterpret_cast<__half2&>(a)), y = __half22float2(reinterpret_cast<__half2&>(b));
-        a = at_pack<bf16>(x.x, x.y);
-        b = at_pack<bf16>(y.x, y.y);
-    }
     return make_uint2(a, b);
 }
 XP_DEV void at_tma(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
@@ -1015,8 +996,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint2 x0 = at_codes<M>(raw[0][i].x, C{}), x1 = at_codes<M>(raw[0][i].y, C{});
-                    const uint2 x2 = at_codes<M>(raw[0][i].z, C{}), x3 = at_codes<M>(raw[0][i].w, C{});
+                    const uint2 x0 = at_codes(raw[0][i].x, C{}), x1 = at_codes(raw[0][i].y, C{});
+                    const uint2 x2 = at_codes(raw[0][i].z, C{}), x3 = at_codes(raw[0][i].w, C{});
                     uint32_t d0, d1;
                     if (kind[0] == 1) {
                         const uint32_t r = lt / KU + i * (128 / KU), c = sub * 8 + 2 * (lt % KU);
