@@ -68,3 +68,14 @@ def test_loads_stay_behind_the_wait_for_the_kernel_before():
         for m in re.finditer(r"\basm\s*(volatile)?\s*\(\s*\"([^\"]*)", text):
             assert m[1] or not re.match(r"\s*(ld|cp|atom|red)\b", m[2]), m[0]
         assert not re.search(r"\b__ld(g|cg|ca|cs|lu|cv)\b", text), name
+
+
+def test_tile_kernel_leaves_no_older_list_for_the_join():
+    """Every way out of the kernel waits for the kernel before it, so that the
+    next one may rely on that, and replaces the parts that an earlier call listed."""
+    kernel = body(source("serving_tile.cuh"), "attn_tile_kernel")
+    for m in re.finditer(r"\breturn;", kernel[:kernel.index("at_make_plan<")]):
+        block = kernel[kernel.rindex("if (smb", 0, m.start()):m.start()]
+        assert block.index("pdl_wait();") < block.index("w.heads[")
+    parted = kernel[kernel.index("if (warp < NQ * 4)"):]
+    assert parted.index("w.heads[") < parted.index("take()")

@@ -546,7 +546,11 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
     const uint32_t b_rows = b_end + 8;              // 8-bit pages: row numbers and scales of a tile given to the loaders
 
     if (smb & 1023) {  // cannot be multiplied from
-        if (tid == 0) atomicOr(a.err, SERVE_ERR_WAIT);
+        pdl_wait();
+        if (tid == 0) {
+            w.heads[(2 * blockIdx.x) * 4] = w.heads[(2 * blockIdx.x + 1) * 4] = AT_FULL;  // nothing to join
+            atomicOr(a.err, SERVE_ERR_WAIT);
+        }
         return;
     }
     if (tid == 0) {
