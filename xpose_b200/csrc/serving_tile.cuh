@@ -620,10 +620,13 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             w.heads[(2 * blockIdx.x + 1) * 4] = AT_FULL;
         }
         const uint32_t qrow0 = wg * w.sub_tokens;  // first token of this row tile in its CTA's tile
-        // Phases are told apart by their parity alone, so a wait must be neither a
-        // phase early nor two late: each warp waits for every phase of a barrier,
-        // in turn, and arrives for the next only after that. s_phase, o_phase: a bit
-        // for each S buffer
+        // Phases are told apart by their parity alone, so a wait must come neither
+        // before the phase ahead of its own has ended nor after the one behind it.
+        // b_o: the product of the tile NB earlier, whose P shares this S buffer, ended
+        // before S was made there (one thread issues and commits them in this order),
+        // so no wait is spent on it: in front of the scores it took up to a tenth. The
+        // next one on the buffer needs this warp's P. s_phase, o_phase: a bit for each
+        // S buffer
         uint32_t stage = 0, s_phase = 0, o_phase = 0, q_phase = 0;
         auto take_o = [&](uint32_t buf) {
             at_wait(b_o + 8 * buf, o_phase >> buf & 1, &s_dead, err);
@@ -686,7 +689,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const uint32_t s_tm = tmem + lanes + buf * 128;
                 at_wait(b_s + 8 * buf, s_phase >> buf & 1, &s_dead, err);
                 s_phase ^= 1u << buf;
-                if (t >= (uint32_t)G::NB) take_o(buf);  // added before S was made over its P
+                if (t >= (uint32_t)G::NB) o_phase ^= 1u << buf;
                 at_fence_after();
                 float s[128];
                 {
@@ -968,8 +971,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
             static_assert(G::NLD == 1 || SUB == 1, "loaders");
             uint32_t given = 0, stage = 0;   // parts given to the tensor core
             uint32_t rows_phase = 0;
-            // the codes of the two parts issued last (0 older), and what they are: 0 none, 1 K, 2 V,
-            // 3 V of a piece that needs a look
+            // the codes of the two parts issued last (0 older), and what they are: 0 none, 1 K, 2 V
             uint4 raw[2][4];
             uint32_t kind[2] = {0, 0};
             const uint32_t rows0 = smb + G::row_off;
@@ -982,22 +984,6 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const uint32_t sub = G::NLD == 2 ? lw : turn;
                 const uint32_t base = smb + G::ring_off + slot * G::PIECE;
                 if (turn == 0 && index >= (uint32_t)NSLOT) at_wait(b_empty + 8 * slot, (index / NSLOT - 1) & 1, &s_dead, err);
-                if (ODD8 && kind[0] == 3) {
-                    // codes of NaN out of the product: they go to the rows that see them at the end
-                    uint32_t odd = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) odd |= at_odd8(raw[0][i].x) | at_odd8(raw[0][i].y) | at_odd8(raw[0][i].z) | at_odd8(raw[0][i].w);
-                    if (odd) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            raw[0][i].x &= ~((at_odd8(raw[0][i].x) >> 7) * 0xFFu);
-                            raw[0][i].y &= ~((at_odd8(raw[0][i].y) >> 7) * 0xFFu);
-                            raw[0][i].z &= ~((at_odd8(raw[0][i].z) >> 7) * 0xFFu);
-                            raw[0][i].w &= ~((at_odd8(raw[0][i].w) >> 7) * 0xFFu);
-                        }
-                        s_bad[seg & 3] = seg + 1;
-                    }
-                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint2 x0 = at_codes(raw[0][i].x, C{}), x1 = at_codes(raw[0][i].y, C{});
@@ -1041,13 +1027,29 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         if (r != AT_NONE) now[i] = ld_once(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
                     }
                     if (kind[0]) convert();
+                    if (ODD8 && is_v && at_look(a, lo, hi, p0, (k0 + t) * AT_KEYS + c * G::NP / W * G::VKEYS, G::VKEYS)) {
+                        // codes of NaN out of the product: they go to the rows that see them at the end
+                        uint32_t odd = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) odd |= at_odd8(now[i].x) | at_odd8(now[i].y) | at_odd8(now[i].z) | at_odd8(now[i].w);
+                        if (odd) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                now[i].x &= ~((at_odd8(now[i].x) >> 7) * 0xFFu);
+                                now[i].y &= ~((at_odd8(now[i].y) >> 7) * 0xFFu);
+                                now[i].z &= ~((at_odd8(now[i].z) >> 7) * 0xFFu);
+                                now[i].w &= ~((at_odd8(now[i].w) >> 7) * 0xFFu);
+                            }
+                            s_bad[seg & 3] = seg + 1;
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         raw[0][i] = raw[1][i];
                         raw[1][i] = now[i];
                     }
                     kind[0] = kind[1];
-                    kind[1] = !is_v ? 1 : ODD8 && at_look(a, lo, hi, p0, (k0 + t) * AT_KEYS + c * G::NP / W * G::VKEYS, G::VKEYS) ? 3 : 2;
+                    kind[1] = is_v ? 2 : 1;
                 };
                 auto page_of = [&](uint32_t kt) -> int32_t {
                     const int32_t key = (int32_t)(kt * AT_KEYS + lt);
