@@ -37,12 +37,13 @@
 // two or more CTAs share leaves partial sums (O, m, l) that a second, small
 // launch joins in a fixed order.
 //
-// Measured: 2048 tokens over 32768 keys, 16 / 2 heads of 128, bf16: 484 us, 1.10
-// PFLOP/s (440 to 505 us as the power limit has it), bound by the softmax of a
-// row tile, which its own products wait for;
-// a prompt of 8192, 4 / 1 heads of 256: 141 us, 0.97 PFLOP/s, bound by shared
-// memory (320 KB of operands and copies for 2048 cycles of products); 12 prompts
-// of 33 to 2048, 32 / 8 heads of 128, fp16: 115 us, 0.62 PFLOP/s.
+// Measured, a call (and its kernels alone, replayed from a graph): 2048 tokens over
+// 32768 keys, 16 / 2 heads of 128, bf16: 484 us, 1.10 PFLOP/s (419 to 480 us as the
+// power limit has it), bound by the softmax of a row tile, which its own products
+// wait for; a prompt of 8192, 4 / 1 heads of 256: 155 us, 0.89 PFLOP/s (151), bound
+// by shared memory (320 KB of operands and copies for 2048 cycles of products); 12
+// prompts of 33 to 2048, 32 / 8 heads of 128, fp16: 124 us, 0.58 PFLOP/s (110); 5
+// chunks of 37 to 512 over int8 pages, 4 / 1 heads of 256: 52 us (50).
 #pragma once
 #include <cuda.h>
 
@@ -74,9 +75,12 @@ template <class T, class C, int W> struct AtCfg {
     static constexpr int NSTAGE = W == 1 ? 8 : 4; // tiles whose row numbers and scales are kept
     static constexpr int NLD = Q8 && W == 4 ? 2 : 1;  // loader warpgroups
     static constexpr int THREADS = 128 * NQ + 128 * NLD + 128;
-    // registers of a softmax, a loader and the last warpgroup: THREADS / 128 shares of the launch's
-    static constexpr int R_SOFT = NQ == 2 ? 184 : NLD == 2 ? 208 : 232;
-    static constexpr int R_LOAD = NQ == 2 ? 80 : NLD == 2 ? 104 : 136;
+    // registers of a softmax, a loader and the last warpgroup: THREADS / 128 shares of the launch's.
+    // Loaders of 128-wide e4m3 heads get 96: with 80 the look for codes of NaN spills. Prompt chunks
+    // take 139 us with 96, 148 with 80; int8 153 and 140, 64-wide heads of both 65 and 61
+    static constexpr bool MORE = W == 2 && std::is_same_v<C, fp8c>;
+    static constexpr int R_SOFT = MORE ? 176 : NQ == 2 ? 184 : NLD == 2 ? 208 : 232;
+    static constexpr int R_LOAD = MORE ? 96 : NQ == 2 ? 80 : NLD == 2 ? 104 : 136;
     static constexpr int R_REST = NQ == 2 ? 64 : NLD == 2 ? 96 : 136;
     static_assert(NQ * R_SOFT + NLD * R_LOAD + R_REST <= THREADS / 128 * (65536 / THREADS / 8 * 8), "registers");
     // shared memory
@@ -821,7 +825,8 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                     at_wait_ld();
                     for (uint32_t t = 0; t < g.n * G::NP; ++t) {
                         const uint32_t key0 = g.k0 * AT_KEYS + t * G::VKEYS;
-                        if (!real || !at_look(a, g.lo, g.hi, g.p0, key0, G::VKEYS)) continue;
+                        // what was looked over: pieces, and of codes whole tiles
+                        if (!real || !at_look(a, g.lo, g.hi, g.p0, ODD8 ? key0 / AT_KEYS * AT_KEYS : key0, ODD8 ? AT_KEYS : G::VKEYS)) continue;
                         const int32_t j0 = max((int32_t)key0, klo);
                         const int32_t j1 = min(min((int32_t)(key0 + G::VKEYS), khi), g.hi);
                         for (int32_t j = j0; j < j1; ++j) {
@@ -1012,9 +1017,11 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 const int32_t lo = g.lo, hi = g.hi;
                 const uint32_t n = g.n, k0 = g.k0, head = g.h;
                 const int32_t* const table = a.table + (uint64_t)g.b * a.table_width;
-                const int32_t p0 = g.p0;
-                // part c of key tile t of K or V, its rows and scales in stage st
-                auto piece = [&](bool is_v, uint32_t c, uint32_t t, uint32_t st) {
+                // tiles [calm0, calm1) of V need no look
+                const int32_t calm0 = (int32_t)(((int64_t)max((int64_t)lo, a.window ? (int64_t)hi - (int64_t)a.window : 0) + AT_KEYS - 1) >> AT_SHIFT) - (int32_t)k0;
+                const int32_t calm1 = (min(hi, g.p0 + 1) >> AT_SHIFT) - (int32_t)k0;
+                // part c of a tile of K or V, its rows and scales in stage st
+                auto piece = [&](bool is_v, uint32_t c, uint32_t st, bool look) {
                     const uint32_t u = is_v ? lt % VU : lt % KU, r0 = is_v ? lt / VU : lt / KU;
                     const uint32_t step = is_v ? 128 / VU : 128 / KU, key0 = is_v ? c * (AT_KEYS / W) : 0;
                     const uint32_t d = (is_v ? u : c * KU + u) * 16;
@@ -1027,7 +1034,7 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                         if (r != AT_NONE) now[i] = ld_once(reinterpret_cast<const uint4*>(src + (int64_t)r * D));
                     }
                     if (kind[0]) convert();
-                    if (ODD8 && is_v && at_look(a, lo, hi, p0, (k0 + t) * AT_KEYS + c * G::NP / W * G::VKEYS, G::VKEYS)) {
+                    if (ODD8 && look) {
                         // codes of NaN out of the product: they go to the rows that see them at the end
                         uint32_t odd = 0;
 #pragma unroll
@@ -1108,15 +1115,15 @@ attn_tile_kernel(const __grid_constant__ ServeAttnArgs a, const __grid_constant_
                 };
                 for (uint32_t t = 0; t < (uint32_t)G::LAG && t < n; ++t) {
                     resolve(t);
-                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, t, kst);
+                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, kst, false);
                     kst = kst + 1 == NSTAGE ? 0 : kst + 1;
                 }
                 for (uint32_t t = 0; t < n; ++t) {
-                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(true, c, t, stage);
+                    for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(true, c, stage, ODD8 && ((int32_t)t < calm0 || (int32_t)t >= calm1));
                     stage = stage + 1 == NSTAGE ? 0 : stage + 1;
                     if (t + G::LAG < n) {
                         resolve(t + G::LAG);
-                        for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, t + G::LAG, kst);
+                        for (uint32_t c = lw; c < (uint32_t)W; c += G::NLD) piece(false, c, kst, false);
                         kst = kst + 1 == NSTAGE ? 0 : kst + 1;
                     }
                 }
