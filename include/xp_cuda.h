@@ -534,9 +534,10 @@ xp_status xp_kv_write(void* stream, const xp_pages* pages, const xp_rows* k, con
 xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, const xp_rows* v, const int64_t* slots);
 /* Scratch of the two attentions: 16-byte aligned, zeroed once, one call at a
  * time. Its uint32 at byte 4 is a sticky error word: 1 = a length past its
- * table row or 2^31 - 256 keys (clamped), 2 = a page outside the cache (its rows read as zeros),
- * 4 = a wait ran out (the output is unspecified; zero the scratch again), 8 = a
- * sequence had more than q_most new tokens (the rest were left out). */
+ * table row or past 2^31 - 256 keys (clamped), 2 = a page outside the cache (its
+ * rows read as zeros), 4 = a wait ran out (the output is unspecified; zero the
+ * scratch again), 8 = a sequence had more than q_most new tokens (the rest were
+ * left out). */
 #define XP_SERVING_SCRATCH_BYTES (48u << 20)
 /* Causal attention over whole prompts packed one after the other: sequence b
  * is tokens starts[b] .. starts[b + 1] - 1 (device, [batch + 1]), and a token
@@ -547,8 +548,8 @@ xp_status xp_kv_read(void* stream, const xp_pages* pages, const xp_rows* k, cons
  * are multiples of 16 bytes; q, k and v have positive ones, but k and v may
  * have a head stride of 0 (one head for all). lse (may be NULL): [tokens][heads]
  * natural log of the sum of the exponentiated scores, -inf for a token in no
- * sequence (before starts[0], or from starts[batch] on), whose output is zero. What other sequences and later tokens hold,
- * NaN included, does not matter. */
+ * sequence (before starts[0], or from starts[batch] on), whose output is zero.
+ * What other sequences and later tokens hold, NaN included, does not matter. */
 xp_status xp_attention_packed(void* stream, const xp_rows* out, const xp_rows* q, const xp_rows* k, const xp_rows* v,
                               const int32_t* starts, uint32_t batch, uint32_t window, float scale, float* lse,
                               void* scratch);

@@ -13,7 +13,7 @@
 //
 // All three are bound by memory: 16381 tokens x 32 heads of 128 rotated in 51 us
 // (5.3 TB/s), 8191 x 8 rows of 128 written in e4m3 and 32768 x 8 read in 52 us (4.9
-// TB/s for the two launches); 64 rows take 3 us, a launch.
+// TB/s for the two launches); 64 rows take 2.5 us on the device, 3.3 a call.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -18,9 +18,10 @@
 // finish adds the parts, in their order. (Chunks that CTAs take as they get free
 // measured slower: adding the sums of a chunk costs as much as eight units.)
 //
-// Measured: 64 sequences of 64 to 16384 keys, 32 / 8 heads of 128, e4m3: 78 us,
-// 4.4 TB/s of 342 MB, bound by the instructions of 8 warps an SM; one token over
-// 4096 keys, 4 / 1 heads of 256, fp16: 15 us, a chain of round trips.
+// Measured (a call; the device takes the same): 64 sequences of 64 to 16384 keys,
+// 32 / 8 heads of 128, e4m3: 80 us, 4.2 TB/s of 342 MB, bound by the instructions
+// of 8 warps an SM; one token over 4096 keys, 4 / 1 heads of 256, fp16: 15.5 us, a
+// chain of round trips.
 #pragma once
 #include "serving_tile.cuh"
 

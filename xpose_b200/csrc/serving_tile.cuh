@@ -38,11 +38,11 @@
 // launch joins in a fixed order.
 //
 // Measured, a call (and its kernels alone, replayed from a graph): 2048 tokens over
-// 32768 keys, 16 / 2 heads of 128, bf16: 484 us, 1.10 PFLOP/s (419 to 480 us as the
+// 32768 keys, 16 / 2 heads of 128, bf16: 482 us, 1.11 PFLOP/s (408 to 492 us as the
 // power limit has it), bound by the softmax of a row tile, which its own products
-// wait for; a prompt of 8192, 4 / 1 heads of 256: 155 us, 0.89 PFLOP/s (151), bound
+// wait for; a prompt of 8192, 4 / 1 heads of 256: 154 us, 0.89 PFLOP/s (143 to 151), bound
 // by shared memory (320 KB of operands and copies for 2048 cycles of products); 12
-// prompts of 33 to 2048, 32 / 8 heads of 128, fp16: 124 us, 0.58 PFLOP/s (110); 5
+// prompts of 33 to 2048, 32 / 8 heads of 128, fp16: 123 us, 0.58 PFLOP/s (107 to 110); 5
 // chunks of 37 to 512 over int8 pages, 4 / 1 heads of 256: 52 us (50).
 #pragma once
 #include <cuda.h>

@@ -5,7 +5,10 @@ Rotary positions (``rope_rows``), the quantising cache write and its read
 (``attention_packed``) or of new tokens over the pages (``attention_paged``):
 the ``xp_*`` calls of the same names in include/xp_cuda.h, whose comments give
 the exact rules. Every call is enqueued on torch's current stream of the
-tensors' device and allocates nothing; errors raise XpError.
+tensors' device, which is one for all of them, and allocates nothing; errors
+raise XpError. What only the device can see, a length past its table or a wait
+that ran out, is in the scratch's error word: read it (error_word) where a
+program waits for its results anyway.
 
     turns, magnitude = rope_turns(256, 1e6)
     k_pages, v_pages, k_scale, v_scale = new_pages(1024, 16, 1, 256, torch.int8)
